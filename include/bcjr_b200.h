@@ -287,6 +287,68 @@ BCJR_API int bcjr_viterbi(const float *seq, const float *cb, int B, int N, int L
  * decode_hyb_batch (src/codes/ref.py:116-128); bit-identical to both. */
 BCJR_API int bcjr_hyb_codebook(const float *lut, int Q, int L, float *cb_out, bcjr_stream_t stream);
 
+/*
+ * Linear layers around the quantizers: products grouped by expert (16-bit
+ * types) and an 8-bit floating point product with a scale for each block of
+ * 128.  No counterpart in the reference, whose QuantizedLinear multiplies with
+ * torch (src/qat/quantized_linear.py:309-315) and whose MoE layers loop over
+ * the experts (src/qat/qat_moe_layer.py).
+ *
+ * Common to the entry points: T rows (0 <= T < 2^31 - 256) in E groups
+ * (1 <= E <= 1024); group e holds rows offsets[e] .. offsets[e + 1] - 1.
+ * `offsets` has E + 1 elements of offsets_bytes (4 or 8) in device memory and
+ * is read on the device; NULL means one group of all rows (E = 1).  Bounds
+ * outside [0, T] are clamped and a decreasing bound counts as its
+ * predecessor.  Features N (out) and K (in) are multiples of 16, the tile of
+ * the quantizers.  w is E x N x K, contiguous; row matrices are row-major with
+ * ld elements between rows (a multiple of 16 bytes); bases 16-byte aligned.
+ * Sums are fp32 and rounded once to the output type; results do not depend on
+ * the run (no atomics).  `status` is one device int: 0, or BCJR_ERR_TIMEOUT if
+ * a bounded device-side wait gave up (bcjr_ws_status reads it; the outputs
+ * concerned are NaN).  It is written by every call with T > 0, so calls that
+ * overlap need one each.
+ */
+enum { BCJR_BF16 = 0, BCJR_F16 = 1, BCJR_F32 = 2 };
+
+/* transpose_w 0: out (T x N) = rows (T x K) times w[e]^T; 1: out (T x K) =
+ * rows (T x N) times w[e], the gradient of the first with respect to its
+ * rows.  Rows of no group are zero in `out`, which is contiguous.  dtype
+ * BCJR_BF16 or BCJR_F16 for rows, w and out. */
+BCJR_API int bcjr_grouped_mm(const void *rows, long ld_rows, const void *w, const void *offsets,
+                             int offsets_bytes, long T, int E, int N, int K, int dtype,
+                             int transpose_w, void *out, int *status, bcjr_stream_t stream);
+
+/* dw[e] (N x K) = dy[group e]^T (N x T_e) times x[group e] (T_e x K); zero for
+ * an empty group. */
+BCJR_API int bcjr_grouped_wgrad(const void *dy, long ld_dy, const void *x, long ld_x,
+                                const void *offsets, int offsets_bytes, long T, int E, int N,
+                                int K, int dtype, void *dw, int *status, bcjr_stream_t stream);
+
+/* e4m3 quantizers (dtype of the input: BCJR_BF16, BCJR_F16 or BCJR_F32).
+ * With amax = max(max |x|, 2^-100) over a block: scale = amax * (1/448), q =
+ * e4m3(x * (448 * (1/amax))), every step in fp32, round to nearest even.  A block that holds a NaN
+ * is NaN, scale and values; one that holds an infinity has scale infinity, NaN
+ * in the infinity's place and zeros elsewhere.
+ * rows: a block is 128 consecutive elements of a row (the last one of a row
+ *   shorter when k is not a multiple of 128); the scale of row t, block j is
+ *   written to scale[t * scale_row + j * scale_block]; q is rows x k.
+ * blocks: 128 x 128 of each of the E matrices N x K; scale is E x
+ *   ceil(N / 128) x ceil(K / 128), q E x N x K. */
+BCJR_API int bcjr_fp8_quantize_rows(const void *x, long ld, long rows, int k, int dtype, void *q,
+                                    float *scale, long scale_row, long scale_block,
+                                    bcjr_stream_t stream);
+BCJR_API int bcjr_fp8_quantize_blocks(const void *w, int E, int N, int K, int dtype, void *q,
+                                      float *scale, bcjr_stream_t stream);
+
+/* bcjr_grouped_mm over such operands: rows quantized by rows along the
+ * contraction, w by blocks; out_dtype BCJR_BF16 or BCJR_F16.  The product of
+ * a row scale and a weight scale is formed in fp32 (it must not underflow). */
+BCJR_API int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long scale_row,
+                         long scale_block, const void *w, const float *w_scale,
+                         const void *offsets, int offsets_bytes, long T, int E, int N, int K,
+                         int transpose_w, void *out, int out_dtype, int *status,
+                         bcjr_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -16,5 +16,12 @@ from .bcjr import (  # noqa: F401
     bcjr_soft_forward,
     build_pred_succ_tables,
 )
+from .linear import (  # noqa: F401
+    fp8_linear,
+    fp8_matmul,
+    fp8_quantize_rows,
+    fp8_quantize_weight,
+    grouped_linear,
+)
 
 __version__ = "0.1.0"

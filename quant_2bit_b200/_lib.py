@@ -33,6 +33,7 @@ OPT_L16_BACKWARD_CLUSTER = 4
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _SZ = ctypes.c_size_t
+_L = ctypes.c_long
 SIGNATURES = {
     "bcjr_version": ([], _I),
     "bcjr_set_test_option": ([_I, _I], _I),
@@ -54,6 +55,11 @@ SIGNATURES = {
     "bcjr_viterbi_launches": ([_I, _I, _I, _I, _I], _I),
     "bcjr_viterbi": ([_P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _SZ, _P], _I),
     "bcjr_hyb_codebook": ([_P, _I, _I, _P, _P], _I),
+    "bcjr_grouped_mm": ([_P, _L, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P, _P, _P], _I),
+    "bcjr_grouped_wgrad": ([_P, _L, _P, _L, _P, _I, _L, _I, _I, _I, _I, _P, _P, _P], _I),
+    "bcjr_fp8_quantize_rows": ([_P, _L, _L, _I, _I, _P, _P, _L, _L, _P], _I),
+    "bcjr_fp8_quantize_blocks": ([_P, _I, _I, _I, _I, _P, _P, _P], _I),
+    "bcjr_fp8_mm": ([_P, _L, _P, _L, _L, _P, _P, _P, _I, _L, _I, _I, _I, _I, _P, _I, _P, _P], _I),
     "bcjr_probe_mufu": ([_P, _I, ctypes.POINTER(ctypes.c_double), _P], _I),
 }
 

@@ -1,0 +1,275 @@
+// 8-bit floating point (e4m3) linear layers with one fp32 scale for each
+// block of 128: the two quantizers and the product.
+//
+//   rows    segment (t, j) = x[t, 128 j .. 128 j + 127]
+//   blocks  block (i, j)   = w[128 i .. 128 i + 127, 128 j .. 128 j + 127]
+//   amax = max(max |x|, 2^-100),  scale = amax (1/448),  q = e4m3(x (448 (1/amax)))
+//
+// with fp32 products and reciprocals rounded to nearest, so that the same
+// elementary operations give the same bits anywhere.  448 is the largest e4m3
+// value; q is off by at most half a step, 2^-4 relative above the subnormals;
+// 2^-100 keeps the reciprocal finite for blocks of zeros.
+//
+//   forward  out[t, n] = sum_j xs[t, j] ws[n / 128, j] sum_{k in j} xq[t, k] wq[n, k]
+//   dgrad    out[t, k] = sum_i gs[t, i] ws[i, k / 128] sum_{n in i} gq[t, n] wq[n, k]
+//
+// The inner sums run on the tensor cores into fp32 accumulators, one for each
+// block of 128; the outer sum is fp32 in registers (kernel: bcjr_mm.cuh).
+#include "../../include/bcjr_b200.h"
+#include "bcjr_kernels.h"
+#include "bcjr_mm.cuh"
+
+namespace bcjr {
+namespace mm {
+namespace {
+
+constexpr float kMax = 448.f;
+
+// Maximum that keeps a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float block_amax(float a) { return max_nan(a, 0x1p-100f); }
+__device__ __forceinline__ float block_scale(float amax) { return __fmul_rn(amax, 1.f / kMax); }
+__device__ __forceinline__ float block_inv(float amax) { return __fmul_rn(kMax, __frcp_rn(amax)); }
+
+template <typename T> __device__ __forceinline__ void load8(const T *p, float (&v)[8]);
+template <> __device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
+    const float4 a = __ldcs(reinterpret_cast<const float4 *>(p));
+    const float4 b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+template <> __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) {
+    const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = __uint_as_float(w[i] << 16);
+        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+}
+template <> __device__ __forceinline__ void load8(const __half *p, float (&v)[8]) {
+    const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+    }
+}
+
+__device__ __forceinline__ float amax8(const float (&v)[8]) {
+    float m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
+    return m;
+}
+__device__ __forceinline__ uint2 to_e4m3(const float (&v)[8], float inv) {
+    uint16_t h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
+            : "=h"(h[i])
+            : "f"(__fmul_rn(v[2 * i + 1], inv)), "f"(__fmul_rn(v[2 * i], inv)));
+    return make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
+}
+
+constexpr int kQThreads = 256, kUnroll = 4;
+
+// 16 lanes per segment, 8 elements per lane (the width is a multiple of 16);
+// kUnroll segments of a thread are loaded before the first is used.
+template <typename T>
+__global__ void __launch_bounds__(kQThreads)
+quantize_rows(const T *__restrict__ x, long ld, long rows, int k, uint8_t *__restrict__ q,
+              float *__restrict__ scale, long s_row, long s_blk) {
+    const int nb = (k + 127) / 128, sub = threadIdx.x & 15;
+    const long segs = rows * nb, groups = kQThreads / 16;
+    const long first = (blockIdx.x * groups * kUnroll) + (threadIdx.x >> 4);
+    float v[kUnroll][8];
+    long row[kUnroll];
+    int blk[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        const long s = first + u * groups;
+        row[u] = s / nb;
+        blk[u] = int(s - row[u] * nb);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
+        if (s < segs && blk[u] * 128 + sub * 8 < k) load8(x + row[u] * ld + blk[u] * 128 + sub * 8, v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+        float m = amax8(v[u]);
+#pragma unroll
+        for (int d = 8; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+        m = block_amax(m);
+        const long s = first + u * groups;
+        if (s >= segs) continue;
+        const int c = blk[u] * 128 + sub * 8;
+        if (c < k) *reinterpret_cast<uint2 *>(q + row[u] * k + c) = to_e4m3(v[u], block_inv(m));
+        if (sub == 0) scale[row[u] * s_row + blk[u] * s_blk] = block_scale(m);
+    }
+}
+
+// One block of 128 x 128 per thread block, held in registers between its
+// maximum and its rounding: read once.
+template <typename T>
+__global__ void __launch_bounds__(kQThreads)
+quantize_blocks(const T *__restrict__ w, int n, int k, uint8_t *__restrict__ q,
+                float *__restrict__ scale) {
+    __shared__ float part[kQThreads / 32];
+    const int kb = (k + 127) / 128, nb = (n + 127) / 128;
+    const long id = blockIdx.x, e = id / (long(nb) * kb);
+    const int in = int(id - e * nb * kb), bi = in / kb, bj = in - bi * kb;
+    const int c = bj * 128 + (threadIdx.x & 15) * 8, r0 = bi * 128 + (threadIdx.x >> 4);
+    const long base = e * n * long(k);
+    float v[8][8], m = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        if (r0 + 16 * i < n && c < k) load8(w + base + (r0 + 16 * i) * long(k) + c, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max_nan(m, amax8(v[i]));
+#pragma unroll
+    for (int d = 16; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kQThreads / 32; ++i) m = max_nan(m, part[i]);
+    m = block_amax(m);
+    const float inv = block_inv(m);
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (r0 + 16 * i < n && c < k)
+            *reinterpret_cast<uint2 *>(q + base + (r0 + 16 * i) * long(k) + c) = to_e4m3(v[i], inv);
+    if (threadIdx.x == 0) scale[id] = block_scale(m);
+}
+
+template <typename T>
+cudaError_t run_rows(const void *x, long ld, long rows, int k, void *q, float *scale, long s_row,
+                     long s_blk, cudaStream_t st) {
+    const long per = long(kQThreads / 16) * kUnroll, segs = rows * ((k + 127) / 128);
+    quantize_rows<T><<<unsigned((segs + per - 1) / per), kQThreads, 0, st>>>(
+        static_cast<const T *>(x), ld, rows, k, static_cast<uint8_t *>(q), scale, s_row, s_blk);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t run_blocks(const void *w, long blocks, int n, int k, void *q, float *scale, cudaStream_t st) {
+    quantize_blocks<T><<<unsigned(blocks), kQThreads, 0, st>>>(static_cast<const T *>(w), n, k,
+                                                               static_cast<uint8_t *>(q), scale);
+    return cudaGetLastError();
+}
+
+template <typename OUT>
+cudaError_t run_mm(const Call &c) {
+    const bool small = c.p.T <= 64;
+    if (c.which == kForward)
+        return small ? launch<kE4M3, OUT, kForward, 64, 8>(c) : launch<kE4M3, OUT, kForward, 256, 4>(c);
+    return small ? launch<kE4M3, OUT, kDgrad, 64, 8>(c) : launch<kE4M3, OUT, kDgrad, 256, 4>(c);
+}
+
+bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+bool float_type(int d) { return d == BCJR_BF16 || d == BCJR_F16 || d == BCJR_F32; }
+int status_of(cudaError_t e) {
+    return e == cudaSuccess ? BCJR_OK : e == cudaErrorInvalidDevice ? BCJR_ERR_DEVICE : BCJR_ERR_LAUNCH;
+}
+
+}  // namespace
+}  // namespace mm
+}  // namespace bcjr
+
+using namespace bcjr::mm;
+
+extern "C" {
+
+int bcjr_fp8_quantize_rows(const void *x, long ld, long rows, int k, int dtype, void *q,
+                           float *scale, long scale_row, long scale_block, bcjr_stream_t stream) {
+    if (rows < 0 || rows > 0x7fffff00L || k < 16 || k % 16 || k > (1 << 24) || ld < k || scale_row < 0 ||
+        scale_block < 0)
+        return BCJR_ERR_BAD_SHAPE;
+    if (!float_type(dtype)) return BCJR_ERR_UNSUPPORTED;
+    if (rows == 0) return BCJR_OK;
+    if (!x || !q || !scale) return BCJR_ERR_NULL_POINTER;
+    if (!aligned(x, 16) || ld % (dtype == BCJR_F32 ? 4 : 8) || !aligned(q, 8) || !aligned(scale, 4))
+        return BCJR_ERR_ALIGNMENT;
+    if (rows * ((k + 127L) / 128) > (1L << 36)) return BCJR_ERR_BAD_SHAPE;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case BCJR_BF16: return status_of(run_rows<__nv_bfloat16>(x, ld, rows, k, q, scale, scale_row, scale_block, st));
+        case BCJR_F16: return status_of(run_rows<__half>(x, ld, rows, k, q, scale, scale_row, scale_block, st));
+        default: return status_of(run_rows<float>(x, ld, rows, k, q, scale, scale_row, scale_block, st));
+    }
+}
+
+int bcjr_fp8_quantize_blocks(const void *w, int E, int N, int K, int dtype, void *q, float *scale,
+                             bcjr_stream_t stream) {
+    if (E < 0 || N < 1 || N > (1 << 24) || K < 16 || K % 16 || K > (1 << 24)) return BCJR_ERR_BAD_SHAPE;
+    if (!float_type(dtype)) return BCJR_ERR_UNSUPPORTED;
+    const long blocks = long(E) * ((N + 127) / 128) * ((K + 127) / 128);
+    if (blocks > 0x7fffffffL) return BCJR_ERR_BAD_SHAPE;
+    if (E == 0) return BCJR_OK;
+    if (!w || !q || !scale) return BCJR_ERR_NULL_POINTER;
+    if (!aligned(w, 16) || !aligned(q, 8) || !aligned(scale, 4)) return BCJR_ERR_ALIGNMENT;
+    cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    switch (dtype) {
+        case BCJR_BF16: return status_of(run_blocks<__nv_bfloat16>(w, blocks, N, K, q, scale, st));
+        case BCJR_F16: return status_of(run_blocks<__half>(w, blocks, N, K, q, scale, st));
+        default: return status_of(run_blocks<float>(w, blocks, N, K, q, scale, st));
+    }
+}
+
+int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long scale_row,
+                long scale_block, const void *w, const float *w_scale, const void *offsets,
+                int offsets_bytes, long T, int E, int N, int K, int transpose_w, void *out,
+                int out_dtype, int *status, bcjr_stream_t stream) {
+    if (T < 0 || T > 0x7fffff00L || E < 1 || E > kMaxGroups || N < 16 || K < 16 || N % 16 || K % 16 ||
+        N > (1 << 24) || K > (1 << 24))
+        return BCJR_ERR_BAD_SHAPE;
+    if (out_dtype != BCJR_BF16 && out_dtype != BCJR_F16) return BCJR_ERR_UNSUPPORTED;
+    if (offsets ? (offsets_bytes != 4 && offsets_bytes != 8) : E != 1) return BCJR_ERR_BAD_SHAPE;
+    if (T == 0) return BCJR_OK;
+    if (!rows || !rows_scale || !w || !w_scale || !out || !status) return BCJR_ERR_NULL_POINTER;
+    const int depth = transpose_w ? N : K, lanes = transpose_w ? K : N;
+    if (ld_rows < depth || ld_rows > (1L << 32) || scale_row < 0 || scale_block < 0) return BCJR_ERR_BAD_SHAPE;
+    if (!aligned(rows, 16) || ld_rows % 16 || !aligned(w, 16) || !aligned(out, 2) || !aligned(status, 4) ||
+        !aligned(rows_scale, 4) || !aligned(w_scale, 4) || (offsets && !aligned(offsets, size_t(offsets_bytes))))
+        return BCJR_ERR_ALIGNMENT;
+    const long kb = (K + 127) / 128, nb = (N + 127) / 128;
+    Call c = {};
+    c.kind = kE4M3;
+    c.which = transpose_w ? kDgrad : kForward;
+    c.a = w;
+    c.a_rows = N;
+    c.a_inner = K;
+    c.b = rows;
+    c.ld_b = ld_rows;
+    c.b_inner = depth;
+    c.stream = reinterpret_cast<cudaStream_t>(stream);
+    c.p.offsets = offsets;
+    c.p.offsets64 = offsets_bytes == 8;
+    c.p.T = int(T);
+    c.p.E = E;
+    c.p.lanes = lanes;
+    c.p.depth = depth;
+    c.p.out = out;
+    c.p.ldo = lanes;
+    c.p.xs = rows_scale;
+    c.p.xs_row = scale_row;
+    c.p.xs_blk = scale_block;
+    c.p.ws = w_scale;
+    c.p.ws_group = nb * kb;
+    c.p.ws_lane = transpose_w ? 1 : kb;
+    c.p.ws_blk = transpose_w ? kb : 1;
+    c.p.status = status;
+    c.p.drop = bcjr::test_option(bcjr::kOptDropSends);
+    return status_of(out_dtype == BCJR_BF16 ? run_mm<__nv_bfloat16>(c) : run_mm<__half>(c));
+}
+
+}  // extern "C"

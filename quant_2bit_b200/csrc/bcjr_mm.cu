@@ -1,0 +1,79 @@
+// Host helpers of the tensor-core products (bcjr_mm.cuh): operand maps and
+// the size of a persistent grid.
+#include "bcjr_mm.cuh"
+
+#include <mutex>
+
+#include "bcjr_kernels.h"
+
+namespace bcjr {
+namespace mm {
+
+namespace {
+typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                             const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                             const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                             CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// The driver's encoder, found through the runtime (the library does not link
+// libcuda, so it loads on machines without a driver).
+EncodeFn encoder() {
+    static std::mutex mu;
+    static EncodeFn fn = nullptr;
+    std::lock_guard<std::mutex> lk(mu);
+    if (!fn) {
+        void *p = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+            q == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeFn>(p);
+    }
+    return fn;
+}
+}  // namespace
+
+bool make_map(CUtensorMap *m, int kind, int rank, const void *base, const unsigned long long *dims,
+              const unsigned long long *strides, const unsigned *box) {
+    const EncodeFn fn = encoder();
+    if (!fn || rank < 2 || rank > 3) return false;
+    const CUtensorMapDataType type = kind == kBF16   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                     : kind == kF16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    cuuint64_t d[3], s[2];
+    cuuint32_t b[3], step[3] = {1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        b[i] = box[i];
+        if (i + 1 < rank) s[i] = strides[i];
+    }
+    return fn(m, type, cuuint32_t(rank), const_cast<void *>(base), d, s, b, step,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int grid_sms() {
+    static std::mutex mu;
+    static int sms[64], major[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    // The map encoder wants a current context, which a thread that has made no
+    // runtime call on the device yet (autograd's) does not have.
+    if (cudaSetDevice(dev) != cudaSuccess) return 0;
+    {
+        std::lock_guard<std::mutex> lk(mu);
+        if (!sms[dev]) {
+            int n = 0, mj = 0;
+            if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+                cudaDeviceGetAttribute(&mj, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
+                return 0;
+            major[dev] = mj;
+            sms[dev] = n;
+        }
+        if (major[dev] != 10) return 0;
+    }
+    const int n = sms[dev] - reserved_sms();
+    return n > 0 ? n : 1;
+}
+
+}  // namespace mm
+}  // namespace bcjr

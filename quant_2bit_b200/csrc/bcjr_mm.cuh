@@ -1,0 +1,676 @@
+// Tensor-core matrix products for the linear layers around the quantizers
+// (bcjr_grouped.cu: 16-bit types, bcjr_fp8.cu: e4m3 with block scales).
+//
+// One persistent kernel serves three products over row groups (experts) e
+// with rows [off_e, off_{e+1}) of the row matrices:
+//
+//   forward  out[t, n]    = sum_k X[t, k]  W[e, n, k]     t in group e
+//   dgrad    out[t, k]    = sum_n dY[t, n] W[e, n, k]
+//   wgrad    out[e, n, k] = sum_{t in e} dY[t, n] X[t, k]
+//
+// All three put the features of the output's innermost axis on the 128 lanes
+// of the accumulator and the other axis of the output on its columns:
+//
+//   D[lane, col] = sum_c A[lane, c] B[col, c]
+//     forward  A = W[e] (K-major)     B = X  (K-major)    lane = n, col = t
+//     dgrad    A = W[e]^T (MN-major)  B = dY (K-major)    lane = k, col = t
+//     wgrad    A = X^T (MN-major)     B = dY^T (MN-major) lane = k, col = n
+//
+// so that the ragged token count is the N of the matrix instruction, which is
+// any multiple of 16 up to 256 and is chosen per tile: one token and 256
+// tokens run the same code, and a group of 300 rows costs 304 columns, not
+// 3 x 128.
+#pragma once
+
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+namespace bcjr {
+namespace mm {
+
+enum { kBF16 = 0, kF16 = 1, kE4M3 = 2 };          // element type of A and B
+enum { kForward = 0, kDgrad = 1, kWgrad = 2 };    // which product
+
+constexpr int kLanes = 128;                       // M of the matrix instruction
+constexpr int kRowBytes = 128;                    // one swizzled shared-memory row
+constexpr int kEpiWarps = 8;
+constexpr int kThreads = (kEpiWarps + 2) * 32;    // + one TMA warp, one MMA warp
+constexpr int kMaxGroups = 1024;
+constexpr int kBoxRows = 64;                      // rows of one TMA box
+constexpr unsigned long long kWaitLimitNs = 1000000000ull;
+
+struct Params {
+    const void *offsets;      // E + 1 group bounds, or NULL: one group of all rows
+    int offsets64;            // offsets are int64 (else int32)
+    int T, E;                 // rows, groups
+    int lanes, cols;          // extent of the lane axis; of the column axis (wgrad)
+    int depth;                // extent of the contraction (forward, dgrad)
+    void *out;
+    long ldo;                 // elements between output rows (columns of D)
+    long out_group;           // elements between groups of the output (wgrad)
+    const float *xs;          // e4m3: row scales, element (row, block) at row xs_row + block xs_blk
+    long xs_row, xs_blk;
+    const float *ws;          // e4m3: weight scales, (group, lane block, contraction block)
+    long ws_group, ws_lane, ws_blk;
+    int *status;
+    int drop;                 // test option: the first load of block 0 is withheld
+};
+
+// ---------------------------------------------------------------------------
+// PTX wrappers.
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;"
+        " selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ unsigned long long now_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+// Bounded wait (about 1 s).  False when it gave up or another warp of the
+// block did; the block then finishes with NaN outputs and the status word
+// says BCJR_ERR_TIMEOUT.
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *fail,
+                                         int *status) {
+    if (bar_try(bar, parity)) return true;
+    const unsigned long long t0 = now_ns();
+    while (true) {
+        for (int i = 0; i < 16; ++i)
+            if (bar_try(bar, parity)) return true;
+        if (*fail) return false;
+        if (now_ns() - t0 > kWaitLimitNs) {
+            *fail = 1;
+            if (status) atomicExch(status, 8 /* BCJR_ERR_TIMEOUT */);
+            return false;
+        }
+    }
+}
+// The same for a whole warp: every lane gets the same answer.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *fail,
+                                          int *status) {
+    return __all_sync(0xffffffffu, bar_wait(bar, parity, fail, status));
+}
+__device__ __forceinline__ void tma2(uint32_t dst, const CUtensorMap *map, int x, int y,
+                                     uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void tma3(uint32_t dst, const CUtensorMap *map, int x, int y, int z,
+                                     uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+}
+template <int KIND>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                    uint32_t accumulate) {
+    if constexpr (KIND == kE4M3)
+        asm volatile(
+            "{ .reg .pred p; setp.ne.b32 p, %4, 0;"
+            " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p; }"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{ .reg .pred p; setp.ne.b32 p, %4, 0;"
+            " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+// The barrier gets one arrival when every matrix instruction issued so far by
+// this thread has completed.
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];"
+                 ::"r"(bar)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_alloc(uint32_t dst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(dst), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols)
+                 : "memory");
+}
+__device__ __forceinline__ void tc_fence_before() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+// 16 columns of this warp's 32 lanes: one lane and 16 columns per thread.
+__device__ __forceinline__ void tmem_ld16(float (&v)[16], uint32_t addr) {
+    uint32_t r[16];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15])
+        : "r"(addr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+
+// Shared-memory operand descriptor, 128-byte swizzle.  K-major: rows of the
+// M or N axis are 128-byte shared-memory rows, 8-row groups 1024 bytes apart.
+// MN-major: 128 bytes of the M or N axis are contiguous, one such row per
+// step of the contraction, 8-step groups 1024 bytes apart, and the next 128
+// bytes of the M or N axis `mn_stride` bytes further.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t mn_stride) {
+    uint64_t d = 0;
+    d |= static_cast<uint64_t>((addr & 0x3ffff) >> 4);
+    d |= static_cast<uint64_t>((mn_stride & 0x3ffff) >> 4) << 16;
+    d |= static_cast<uint64_t>(1024 >> 4) << 32;
+    d |= 1ull << 46;
+    d |= 2ull << 61;
+    return d;
+}
+
+template <int KIND, bool A_MN, bool B_MN>
+__device__ __forceinline__ uint32_t instr_desc(int n) {
+    const uint32_t fmt = KIND == kBF16 ? 1u : 0u;   // f16 0, bf16 1; e4m3 0
+    return (1u << 4) | (fmt << 7) | (fmt << 10) | (A_MN ? 1u << 15 : 0u) |
+           (B_MN ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
+           (static_cast<uint32_t>(kLanes >> 4) << 24);
+}
+
+// ---------------------------------------------------------------------------
+// Groups and tiles.
+
+// Group bounds as the kernel uses them: within [0, T] and not decreasing,
+// whatever the caller's memory holds, so no access can leave the matrices.
+// first[e] is the number of column tiles before group e (forward, dgrad).
+struct Groups {
+    int off[kMaxGroups + 1];
+    int first[kMaxGroups + 1];
+};
+
+template <int COLS>
+__device__ __forceinline__ int col_tiles(int rows) { return (rows + COLS - 1) / COLS; }
+
+// One warp fills `g`.
+template <int COLS>
+__device__ void load_groups(Groups &g, const Params &p, int lane) {
+    int high = 0, tiles = 0;        // last bound and tile count of the chunk before
+    for (int base = 0; base <= p.E; base += 32) {
+        const int e = base + lane;
+        int o = 0;
+        if (e <= p.E) {
+            if (!p.offsets) {
+                o = e == 0 ? 0 : p.T;
+            } else {
+                const long long v = p.offsets64
+                                        ? static_cast<const long long *>(p.offsets)[e]
+                                        : static_cast<long long>(static_cast<const int *>(p.offsets)[e]);
+                o = v < 0 ? 0 : v > p.T ? p.T : static_cast<int>(v);
+            }
+        }
+        if (o < high) o = high;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, o, d);
+            if (lane >= d && u > o) o = u;
+        }
+        int prev = __shfl_up_sync(0xffffffffu, o, 1);
+        if (lane == 0) prev = high;
+        // tiles of group e - 1, which ends at this bound
+        int n = (e >= 1 && e <= p.E) ? col_tiles<COLS>(o - prev) : 0;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, n, d);
+            if (lane >= d) n += u;
+        }
+        if (e <= p.E) {
+            g.off[e] = o;
+            g.first[e] = tiles + n;
+        }
+        high = __shfl_sync(0xffffffffu, o, 31);
+        tiles += __shfl_sync(0xffffffffu, n, 31);
+    }
+}
+
+struct Tile {
+    int group;
+    int lane_tile;
+    int col0;       // first output row (forward, dgrad: row of X; wgrad: n)
+    int valid;      // columns to write
+    int ncols;      // columns computed, a multiple of 16
+    int k0;         // first contraction index (wgrad: row of X)
+    int depth;      // contraction length (0: the output is zero)
+};
+
+// The tiles of a block, one after the other; every warp walks the same list.
+template <int WHICH, int COLS>
+struct Walk {
+    const Groups &g;
+    const Params &p;
+    int lane_tiles, total, tile, group;
+    __device__ Walk(const Groups &g_, const Params &p_) : g(g_), p(p_) {
+        lane_tiles = (p.lanes + kLanes - 1) / kLanes;
+        total = WHICH == kWgrad ? p.E * lane_tiles * col_tiles<COLS>(p.cols)
+                                : g.first[p.E] * lane_tiles;
+        tile = blockIdx.x;
+        group = 0;
+    }
+    __device__ bool next(Tile &t) {
+        if (tile >= total) return false;
+        if constexpr (WHICH == kWgrad) {
+            const int ct = col_tiles<COLS>(p.cols), per = lane_tiles * ct;
+            t.group = tile / per;
+            const int in = tile - t.group * per;
+            t.lane_tile = in / ct;
+            t.col0 = (in - t.lane_tile * ct) * COLS;
+            t.valid = min(COLS, p.cols - t.col0);
+            t.ncols = t.valid;               // cols is a multiple of 16
+            t.k0 = g.off[t.group];
+            t.depth = g.off[t.group + 1] - t.k0;
+        } else {
+            while (tile >= g.first[group + 1] * lane_tiles) ++group;
+            const int in = tile - g.first[group] * lane_tiles;
+            const int ct = g.first[group + 1] - g.first[group];
+            t.group = group;
+            t.lane_tile = in / ct;
+            const int c = in - t.lane_tile * ct;
+            const int rows = g.off[group + 1] - g.off[group];
+            // equal shares: no small tile at the end of a group
+            const int share = ((rows + ct - 1) / ct + 15) & ~15;
+            t.col0 = g.off[group] + c * share;
+            t.valid = min(share, g.off[group + 1] - t.col0);
+            t.ncols = (t.valid + 15) & ~15;
+            t.k0 = 0;
+            t.depth = p.depth;
+        }
+        tile += gridDim.x;
+        return true;
+    }
+};
+
+template <typename T> __device__ __forceinline__ T from_float(float v);
+template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
+template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+
+template <int COLS, int STAGES>
+struct Smem {
+    static constexpr int kA = kLanes * kRowBytes;
+    static constexpr int kB = COLS * kRowBytes;
+    static constexpr int kStage = kA + kB;
+    struct Ctl {
+        unsigned long long full[STAGES], empty[STAGES], tfull[2], tempty[2], done;
+        uint32_t tmem;
+        int fail;
+        float scale[2][COLS];
+        Groups groups;
+    };
+    static constexpr size_t bytes() { return 1024 + size_t(STAGES) * kStage + sizeof(Ctl); }
+};
+
+// KIND: element type; OUT: output type; WHICH: product; COLS: columns of a
+// tile; STAGES: depth of the shared-memory ring.
+template <int KIND, typename OUT, int WHICH, int COLS, int STAGES>
+__global__ void __launch_bounds__(kThreads, 1)
+mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
+          const __grid_constant__ Params p) {
+    constexpr bool A_MN = WHICH != kForward, B_MN = WHICH == kWgrad;
+    constexpr int ESIZE = KIND == kE4M3 ? 1 : 2;
+    constexpr int BK = kRowBytes / ESIZE;             // contraction per stage
+    constexpr int MNB = kRowBytes / ESIZE;            // M or N elements of one MN-major row
+    constexpr int SLICES = 4;                         // matrix instructions per stage
+    constexpr int KSLICE = BK / SLICES;
+    // bytes from one slice to the next
+    constexpr uint32_t A_STEP = A_MN ? KSLICE * kRowBytes : 32;
+    constexpr uint32_t B_STEP = B_MN ? KSLICE * kRowBytes : 32;
+    constexpr uint32_t MN_BLOCK = BK * kRowBytes;     // an MN-major block of BK rows
+    constexpr uint32_t TMEM_COLS = 2 * COLS < 32 ? 32 : 2 * COLS;
+    using S = Smem<COLS, STAGES>;
+    static_assert(!(KIND == kE4M3 && WHICH == kWgrad), "e4m3 has forward and dgrad");
+    static_assert(BK % kBoxRows == 0 && COLS % 16 == 0, "");
+
+    extern __shared__ unsigned char raw[];
+    unsigned char *buf = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    typename S::Ctl &ctl = *reinterpret_cast<typename S::Ctl *>(buf + size_t(STAGES) * S::kStage);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int *fail = &ctl.fail;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < STAGES; ++i) {
+            bar_init(smem_u32(&ctl.full[i]), 1);
+            bar_init(smem_u32(&ctl.empty[i]), 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            bar_init(smem_u32(&ctl.tfull[i]), 1);
+            bar_init(smem_u32(&ctl.tempty[i]), kEpiWarps);
+        }
+        bar_init(smem_u32(&ctl.done), 1);
+        ctl.fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (blockIdx.x == 0 && p.status) *p.status = 0;   // a failure is a second away
+    }
+    if (warp == kEpiWarps + 1) tmem_alloc(smem_u32(&ctl.tmem), TMEM_COLS);
+    if (warp == kEpiWarps) load_groups<COLS>(ctl.groups, p, lane);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl.tmem;
+    Walk<WHICH, COLS> walk(ctl.groups, p);
+    Tile t;
+
+    if (warp == kEpiWarps) {
+        // TMA producer
+        if (lane == 0) {
+            uint32_t it = 0;
+            bool ok = true;
+            while (ok && walk.next(t)) {
+                const int nkb = (t.depth + BK - 1) / BK;
+                const int bboxes = B_MN ? (t.ncols + MNB - 1) / MNB : (t.ncols + kBoxRows - 1) / kBoxRows;
+                const uint32_t bytes = S::kA + bboxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes);
+                for (int kb = 0; kb < nkb; ++kb, ++it) {
+                    const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
+                    if (!bar_wait(smem_u32(&ctl.empty[s]), ph ^ 1, fail, p.status)) {
+                        ok = false;
+                        break;
+                    }
+                    if (p.drop && blockIdx.x == 0 && it == 0) continue;
+                    const uint32_t bar = smem_u32(&ctl.full[s]);
+                    const uint32_t a = smem_u32(buf + s * S::kStage), b = a + S::kA;
+                    bar_expect(bar, bytes);
+                    const int kc = t.k0 + kb * BK;
+                    if constexpr (WHICH == kForward) {
+                        tma3(a, &ta, kc, t.lane_tile * kLanes, t.group, bar);
+                    } else if constexpr (WHICH == kDgrad) {
+#pragma unroll
+                        for (int j = 0; j < kLanes / MNB; ++j)
+                            tma3(a + j * MN_BLOCK, &ta, t.lane_tile * kLanes + j * MNB, kc, t.group, bar);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kLanes / MNB; ++j)
+                            tma2(a + j * MN_BLOCK, &ta, t.lane_tile * kLanes + j * MNB, kc, bar);
+                    }
+                    for (int j = 0; j < bboxes; ++j) {
+                        if constexpr (B_MN)
+                            tma2(b + j * MN_BLOCK, &tb, t.col0 + j * MNB, kc, bar);
+                        else
+                            tma2(b + j * kBoxRows * kRowBytes, &tb, kc, t.col0 + j * kBoxRows, bar);
+                    }
+                }
+            }
+            if (!ok) {
+                // copies in flight land before the block ends
+                volatile int never = 0;
+                for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+                    if (!(p.drop && blockIdx.x == 0 && i == 0))
+                        bar_wait(smem_u32(&ctl.full[i % STAGES]), (i / STAGES) & 1, &never, nullptr);
+            }
+        }
+    } else if (warp == kEpiWarps + 1) {
+        // MMA issuer
+        uint32_t it = 0, acc = 0;
+        bool ok = true;
+        while (ok && walk.next(t)) {
+            const int nkb = (t.depth + BK - 1) / BK;
+            if (nkb == 0) continue;
+            const uint32_t idesc = instr_desc<KIND, A_MN, B_MN>(t.ncols);
+            for (int kb = 0; kb < nkb; ++kb, ++it) {
+                // e4m3: every stage has an accumulator buffer of its own
+                // (scaled and added in fp32 registers); otherwise every tile
+                if (KIND == kE4M3 || kb == 0) {
+                    if (!warp_wait(smem_u32(&ctl.tempty[acc & 1]), ((acc >> 1) & 1) ^ 1, fail, p.status)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                }
+                const uint32_t s = it % STAGES;
+                if (!warp_wait(smem_u32(&ctl.full[s]), (it / STAGES) & 1, fail, p.status)) {
+                    ok = false;
+                    break;
+                }
+                unsigned char *a = buf + s * S::kStage, *b = a + S::kA;
+                if constexpr (WHICH == kWgrad) {
+                    const int rows = t.depth - kb * BK;
+                    if (rows < BK) {
+                        // rows of the next group (or behind the last one) do not
+                        // count, whatever they hold: both factors become zero
+                        const int cells = (BK - rows) * (kRowBytes / 16);
+                        const int blocks = kLanes / MNB + (t.ncols + MNB - 1) / MNB;
+                        for (int j = 0; j < blocks; ++j) {
+                            uint4 *z = reinterpret_cast<uint4 *>(a + j * MN_BLOCK + rows * kRowBytes);
+                            for (int i = lane; i < cells; i += 32) z[i] = make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                }
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint64_t da = operand_desc(smem_u32(a), MN_BLOCK);
+                    const uint64_t db = operand_desc(smem_u32(b), MN_BLOCK);
+                    const uint32_t d = tmem + (acc & 1) * COLS;
+#pragma unroll
+                    for (int j = 0; j < SLICES; ++j)
+                        mma<KIND>(d, da + ((j * A_STEP) >> 4), db + ((j * B_STEP) >> 4), idesc,
+                                  (KIND == kE4M3 ? j > 0 : (kb | j) > 0) ? 1u : 0u);
+                    mma_commit(smem_u32(&ctl.empty[s]));
+                    if (KIND == kE4M3 || kb == nkb - 1) mma_commit(smem_u32(&ctl.tfull[acc & 1]));
+                }
+                __syncwarp();
+                if (KIND == kE4M3 || kb == nkb - 1) ++acc;
+            }
+        }
+        // every matrix instruction has ended before the block frees its TMEM
+        if (lane == 0) mma_commit(smem_u32(&ctl.done));
+        volatile int never = 0;
+        bar_wait(smem_u32(&ctl.done), 0, &never, nullptr);
+    } else {
+        // epilogue: warp w reads lanes 32 (w % 4).., column chunks of 32 with
+        // index w / 4, w / 4 + 2, ...
+        constexpr int CHUNKS = COLS >= 64 ? COLS / 64 : 1;
+        const int quad = warp & 3, half = warp >> 2;
+        uint32_t acc = 0;
+        bool ok = true;
+        while (walk.next(t)) {
+            const int nkb = (t.depth + BK - 1) / BK;
+            const int feature = t.lane_tile * kLanes + quad * 32 + lane;
+            OUT *out = static_cast<OUT *>(p.out) + (WHICH == kWgrad ? t.group * p.out_group : 0) +
+                       static_cast<long>(t.col0) * p.ldo + feature;
+            const bool live = feature < p.lanes;
+            if constexpr (KIND == kE4M3) {
+                float sum[CHUNKS * 32];
+#pragma unroll
+                for (int i = 0; i < CHUNKS * 32; ++i) sum[i] = 0.f;
+                const int c = threadIdx.x;
+                const float *xs = p.xs + static_cast<long>(t.col0 + c) * p.xs_row;
+                const float *ws = p.ws + t.group * p.ws_group + t.lane_tile * p.ws_lane;
+                const bool scales = c < t.valid;
+                float next = scales ? xs[0] * ws[0] : 0.f;
+                for (int kb = 0; kb < nkb; ++kb, ++acc) {
+                    if (c < COLS) ctl.scale[acc & 1][c] = next;
+                    asm volatile("bar.sync 1, 256;" ::: "memory");
+                    if (kb + 1 < nkb)
+                        next = scales ? xs[(kb + 1) * p.xs_blk] * ws[(kb + 1) * p.ws_blk] : 0.f;
+                    if (ok) ok = warp_wait(smem_u32(&ctl.tfull[acc & 1]), (acc >> 1) & 1, fail, p.status);
+                    if (!ok) continue;
+                    __syncwarp();
+                    tc_fence_after();
+#pragma unroll
+                    for (int i = 0; i < CHUNKS; ++i) {
+                        const int c0 = (half + 2 * i) * 32;
+                        if (c0 < t.ncols) {
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) {
+                                float v[16];
+                                tmem_ld16(v, tmem + (static_cast<uint32_t>(quad * 32) << 16) +
+                                                 (acc & 1) * COLS + c0 + h * 16);
+                                tmem_wait_ld();
+                                const float4 *sc = reinterpret_cast<const float4 *>(&ctl.scale[acc & 1][c0 + h * 16]);
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    const float4 f = sc[q];
+                                    float *o = &sum[i * 32 + h * 16 + q * 4];
+                                    o[0] = fmaf(v[4 * q], f.x, o[0]);
+                                    o[1] = fmaf(v[4 * q + 1], f.y, o[1]);
+                                    o[2] = fmaf(v[4 * q + 2], f.z, o[2]);
+                                    o[3] = fmaf(v[4 * q + 3], f.w, o[3]);
+                                }
+                            }
+                        }
+                    }
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(smem_u32(&ctl.tempty[acc & 1]));
+                }
+                if (live) {
+#pragma unroll
+                    for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const int col = (half + 2 * i) * 32 + j;
+                            if (col < t.valid)
+                                out[col * p.ldo] = from_float<OUT>(ok ? sum[i * 32 + j] : __int_as_float(0x7fffffff));
+                        }
+                }
+            } else {
+                if (nkb && ok) ok = warp_wait(smem_u32(&ctl.tfull[acc & 1]), (acc >> 1) & 1, fail, p.status);
+                __syncwarp();
+                tc_fence_after();
+                for (int c0 = half * 32; c0 < t.ncols; c0 += 64) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v[16];
+                        if (nkb && ok) {
+                            tmem_ld16(v, tmem + (static_cast<uint32_t>(quad * 32) << 16) +
+                                             (acc & 1) * COLS + c0 + h * 16);
+                            tmem_wait_ld();
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) v[j] = ok ? 0.f : __int_as_float(0x7fffffff);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const int col = c0 + h * 16 + j;
+                            if (live && col < t.valid) out[col * p.ldo] = from_float<OUT>(v[j]);
+                        }
+                    }
+                }
+                if (nkb) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) bar_arrive(smem_u32(&ctl.tempty[acc & 1]));
+                    ++acc;
+                }
+            }
+        }
+        if constexpr (WHICH != kWgrad) {
+            // rows of no group are zero
+            const int lo = ctl.groups.off[0], hi = ctl.groups.off[p.E];
+            const long rows = static_cast<long>(lo) + (p.T - hi);
+            for (long r = blockIdx.x; r < rows; r += gridDim.x) {
+                OUT *o = static_cast<OUT *>(p.out) + (r < lo ? r : r - lo + hi) * p.ldo;
+                for (int f = threadIdx.x; f < p.lanes; f += kEpiWarps * 32) o[f] = from_float<OUT>(0.f);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kEpiWarps + 1) tmem_free(tmem, TMEM_COLS);
+}
+
+// ---------------------------------------------------------------------------
+// Host side (bcjr_mm.cu).
+
+// A tiled map of a matrix of `rank` axes (innermost first), `strides` in
+// bytes from the second axis on, 128-byte swizzle, zeros outside.
+bool make_map(CUtensorMap *m, int kind, int rank, const void *base, const unsigned long long *dims,
+              const unsigned long long *strides, const unsigned *box);
+// SMs of the current device for a persistent grid (less the reserved ones);
+// 0 when the device is not sm_100.
+int grid_sms();
+
+struct Call {
+    int kind, which;          // element type, product
+    const void *a, *b;        // weights (wgrad: X) and row matrix (wgrad: dY)
+    long ld_a, ld_b;          // elements between rows of wgrad's X; of the row matrix
+    long a_rows, a_inner;     // weight rows (N) and row length (K); wgrad: K in a_inner
+    long b_inner;             // row length of the row matrix
+    cudaStream_t stream;
+    Params p;
+};
+
+// Both operand maps of a call.
+template <int KIND, int WHICH>
+bool make_maps(const Call &c, CUtensorMap &ta, CUtensorMap &tb) {
+    constexpr unsigned es = KIND == kE4M3 ? 1 : 2, inner = kRowBytes / es;
+    using U = unsigned long long;
+    if (WHICH == kWgrad) {
+        const U dims[2] = {U(c.a_inner), U(c.p.T)}, st[1] = {U(c.ld_a) * es};
+        const unsigned box[2] = {inner, inner};
+        if (!make_map(&ta, KIND, 2, c.a, dims, st, box)) return false;
+    } else {
+        const U dims[3] = {U(c.a_inner), U(c.a_rows), U(c.p.E)};
+        const U st[2] = {U(c.a_inner) * es, U(c.a_inner) * U(c.a_rows) * es};
+        const unsigned box[3] = {inner, WHICH == kForward ? unsigned(kLanes) : inner, 1};
+        if (!make_map(&ta, KIND, 3, c.a, dims, st, box)) return false;
+    }
+    const U dims[2] = {U(c.b_inner), U(c.p.T)}, st[1] = {U(c.ld_b) * es};
+    const unsigned box[2] = {inner, WHICH == kWgrad ? inner : unsigned(kBoxRows)};
+    return make_map(&tb, KIND, 2, c.b, dims, st, box);
+}
+
+template <int KIND, typename OUT, int WHICH, int COLS, int STAGES>
+cudaError_t launch(const Call &c) {
+    CUtensorMap ta, tb;
+    const int sms = grid_sms();
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    if (!make_maps<KIND, WHICH>(c, ta, tb)) return cudaErrorInvalidValue;
+    auto *k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES>;
+    constexpr size_t bytes = Smem<COLS, STAGES>::bytes();
+    static_assert(bytes <= 232448, "shared memory of one block");
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (e != cudaSuccess) return e;
+    // no more blocks than there can be tiles
+    const long lane_tiles = (c.p.lanes + kLanes - 1) / kLanes;
+    const long col_tiles = WHICH == kWgrad ? long(c.p.E) * ((c.p.cols + COLS - 1) / COLS)
+                                           : c.p.T / COLS + (c.p.E < c.p.T ? c.p.E : c.p.T);
+    const long tiles = lane_tiles * (col_tiles > 0 ? col_tiles : 1);
+    k<<<unsigned(tiles < sms ? tiles : sms), kThreads, bytes, c.stream>>>(ta, tb, c.p);
+    return cudaGetLastError();
+}
+
+}  // namespace mm
+}  // namespace bcjr

@@ -1,0 +1,350 @@
+"""Linear layers over the quantizers' weights: products grouped by expert, and
+8-bit floating point with a scale for each block of 128.
+
+The reference's QuantizedLinear multiplies its quantized weight with torch
+(src/qat/quantized_linear.py:309-315), and its MoE layers loop over the experts
+(src/qat/qat_moe_layer.py).  Here one launch serves all experts of a layer
+(``quant.bcjr_quantize_layer`` quantizes them in one launch too), and layers
+that are not being trained -- the teacher, the frozen layers around the one in
+training -- can hold their weights in e4m3 and still pass gradients on.
+
+* ``grouped_linear(x, weight, offsets)``: rows sorted by expert, bf16 or fp16,
+  differentiable in ``x`` and ``weight``.
+* ``fp8_quantize_rows`` / ``fp8_quantize_weight``: e4m3 with one fp32 scale for
+  each 1 x 128 row segment / 128 x 128 block: with amax = max(max |x|, 2^-100)
+  over the block, scale = amax * (1/448) and q = e4m3(x * (448 * (1/amax))), in fp32.
+* ``fp8_matmul``: the product of two such operands, summed in fp32.
+* ``fp8_linear(x, q, scale)``: quantizes the rows of ``x`` and multiplies;
+  differentiable in ``x`` (straight through the rounding; the upstream gradient
+  is quantized by rows in the same way).
+
+Every op runs the sm_100a kernels of libbcjr_b200.so on the caller's current
+stream, reads ``offsets`` on the device only, and never synchronises.  There is
+no CPU path: CPU tensors raise RuntimeError, wrong shapes AssertionError, wrong
+types ValueError.  Feature counts are multiples of 16 (the quantizers' tile).
+"""
+import contextlib
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+
+_BLOCK = 128
+_TILE = 16
+_MAX_GROUPS = 1024
+_F8 = torch.float8_e4m3fn
+_DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _need_cuda(**tensors):
+    device = None
+    for name, t in tensors.items():
+        if t is None:
+            continue
+        if not (torch.is_tensor(t) and t.is_cuda):
+            raise RuntimeError(f"quant_2bit_b200: `{name}` must be a CUDA tensor (the B200 kernels "
+                               "have no CPU fallback)")
+        device = device or t.device
+        assert t.device == device, f"`{name}` is on {t.device}, not on {device}"
+    return device
+
+
+def _need_dtype(t, name, allowed):
+    if t.dtype not in allowed:
+        raise ValueError(f"`{name}` must be {' or '.join(str(d) for d in allowed)}, got {t.dtype}")
+
+
+def _need_features(n, name):
+    assert n >= _TILE and n % _TILE == 0, f"{name} must be a multiple of {_TILE}, got {n}"
+
+
+def _on(device):
+    if torch.cuda.current_device() == device.index:
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _stream(device):
+    return torch.cuda.current_stream(device).cuda_stream
+
+
+def _blocks(n):
+    return -(-n // _BLOCK)
+
+
+def _rows(t):
+    """(tensor, elements between rows) of a 2-D matrix as the kernels read it: the
+    matrix itself when its rows are contiguous and start on 16 bytes, else a
+    contiguous copy."""
+    step = t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    if t.stride(1) == 1 and step >= t.shape[1] and step * t.element_size() % 16 == 0 \
+            and t.data_ptr() % 16 == 0:
+        return t, step
+    return _dense(t), t.shape[1]
+
+
+def _dense(t):
+    """Contiguous and 16-byte aligned."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
+def _need_offsets(offsets, groups):
+    if offsets is None:
+        return None, 0, 0
+    _need_dtype(offsets, "offsets", (torch.int32, torch.int64))
+    assert offsets.dim() == 1 and offsets.shape[0] == groups + 1, \
+        f"offsets must have one more element than there are experts ({groups}), got {tuple(offsets.shape)}"
+    offsets = offsets.contiguous()
+    return offsets, offsets.data_ptr(), offsets.element_size()
+
+
+def _status(device):
+    return torch.empty(1, dtype=torch.int32, device=device)
+
+
+# --------------------------------------------------------------------------
+# bf16 / fp16, grouped by expert
+
+
+def _grouped_mm(rows, weight, offsets, transpose):
+    """rows times weight[e]^T, or times weight[e] when ``transpose``."""
+    E, N, K = weight.shape
+    T, dev = rows.shape[0], rows.device
+    out = torch.empty((T, K if transpose else N), dtype=rows.dtype, device=dev)
+    if T == 0:
+        return out
+    rows, ld = _rows(rows)
+    weight = _dense(weight)
+    offsets, off_ptr, off_size = _need_offsets(offsets, E)
+    with _on(dev):
+        st = _lib.load().bcjr_grouped_mm(rows.data_ptr(), ld, weight.data_ptr(), off_ptr, off_size,
+                                         T, E, N, K, _DTYPES[rows.dtype], int(transpose),
+                                         out.data_ptr(), _status(dev).data_ptr(), _stream(dev))
+    _lib.check(st, "bcjr_grouped_mm")
+    return out
+
+
+def _grouped_wgrad(dy, x, offsets, E):
+    (T, N), K, dev = dy.shape, x.shape[1], x.device
+    dw = torch.empty((E, N, K), dtype=x.dtype, device=dev)
+    dy, ld_dy = _rows(dy)
+    x, ld_x = _rows(x)
+    offsets, off_ptr, off_size = _need_offsets(offsets, E)
+    with _on(dev):
+        st = _lib.load().bcjr_grouped_wgrad(dy.data_ptr(), ld_dy, x.data_ptr(), ld_x, off_ptr,
+                                            off_size, T, E, N, K, _DTYPES[x.dtype], dw.data_ptr(),
+                                            _status(dev).data_ptr(), _stream(dev))
+    _lib.check(st, "bcjr_grouped_wgrad")
+    return dw
+
+
+class _GroupedLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, offsets):
+        ctx.save_for_backward(x, weight, offsets)
+        return _grouped_mm(x, weight, offsets, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, offsets = ctx.saved_tensors
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            dx = _grouped_mm(dy, weight, offsets, True)
+        if ctx.needs_input_grad[1]:
+            dw = _grouped_wgrad(dy, x, offsets, weight.shape[0])
+        return dx, dw, None
+
+
+def grouped_linear(x, weight, offsets):
+    """y[t] = weight[e] @ x[t] for every row t of group e, offsets[e] <= t <
+    offsets[e + 1].
+
+    x        (T, K) bf16 or fp16, rows sorted by expert; any row stride
+    weight   (E, N, K), x's dtype (``quant.bcjr_quantize_layer`` returns fp32:
+             stack and cast, as QuantizedLinear casts to its input's type)
+    offsets  (E + 1,) int32 or int64 on x's device, not decreasing, within
+             [0, T]; it is not read on the host, and the kernels clamp it
+
+    Returns (T, N).  Groups may be empty; rows before offsets[0] and from
+    offsets[E] on belong to no group: their output and gradient are zero.
+    Sums are fp32, rounded once; results do not change from run to run."""
+    _need_cuda(x=x, weight=weight, offsets=offsets)
+    _need_dtype(x, "x", (torch.bfloat16, torch.float16))
+    _need_dtype(weight, "weight", (x.dtype,))
+    assert x.dim() == 2 and weight.dim() == 3 and x.shape[1] == weight.shape[2], \
+        f"x must be (T, K) and weight (E, N, K), got {tuple(x.shape)} and {tuple(weight.shape)}"
+    assert 1 <= weight.shape[0] <= _MAX_GROUPS, f"1 to {_MAX_GROUPS} experts, got {weight.shape[0]}"
+    _need_features(weight.shape[1], "out features")
+    _need_features(weight.shape[2], "in features")
+    _need_offsets(offsets, weight.shape[0])
+    return _GroupedLinear.apply(x, weight, offsets)
+
+
+# --------------------------------------------------------------------------
+# e4m3 with block scales
+
+
+def _quantize_rows_into(x, q_ptr, scale_ptr, scale_row, scale_block):
+    x, ld = _rows(x)
+    dev = x.device
+    with _on(dev):
+        st = _lib.load().bcjr_fp8_quantize_rows(x.data_ptr(), ld, x.shape[0], x.shape[1],
+                                                _DTYPES[x.dtype], q_ptr, scale_ptr, scale_row,
+                                                scale_block, _stream(dev))
+    _lib.check(st, "bcjr_fp8_quantize_rows")
+
+
+def fp8_quantize_rows(x):
+    """(q, scale) of (..., K) bf16, fp16 or fp32: q e4m3 of x's shape, scale fp32
+    (..., ceil(K / 128)); q times its segment's scale stands for x.  Not
+    differentiable (``fp8_linear`` is)."""
+    _need_cuda(x=x)
+    _need_dtype(x, "x", tuple(_DTYPES))
+    assert x.dim() >= 1, "x must have at least one axis"
+    K = x.shape[-1]
+    _need_features(K, "the last axis")
+    q = torch.empty(x.shape, dtype=_F8, device=x.device)
+    scale = torch.empty((*x.shape[:-1], _blocks(K)), dtype=torch.float32, device=x.device)
+    if x.numel():
+        _quantize_rows_into(x.detach().reshape(-1, K), q.data_ptr(), scale.data_ptr(), _blocks(K), 1)
+    return q, scale
+
+
+def fp8_quantize_weight(weight):
+    """(q, scale) of a weight (N, K), or of E weights (E, N, K), bf16, fp16 or
+    fp32: q e4m3 of its shape, scale fp32 ([E,] ceil(N / 128), ceil(K / 128)),
+    one for each 128 x 128 block."""
+    _need_cuda(weight=weight)
+    _need_dtype(weight, "weight", tuple(_DTYPES))
+    assert weight.dim() in (2, 3), f"weight must be (N, K) or (E, N, K), got {tuple(weight.shape)}"
+    N, K = weight.shape[-2:]
+    E = weight.shape[0] if weight.dim() == 3 else 1
+    assert N >= 1, "weight must have rows"
+    _need_features(K, "in features")
+    dev = weight.device
+    w = _dense(weight.detach())
+    q = torch.empty(weight.shape, dtype=_F8, device=dev)
+    scale = torch.empty((*weight.shape[:-2], _blocks(N), _blocks(K)), dtype=torch.float32, device=dev)
+    with _on(dev):
+        st = _lib.load().bcjr_fp8_quantize_blocks(w.data_ptr(), E, N, K, _DTYPES[w.dtype],
+                                                  q.data_ptr(), scale.data_ptr(), _stream(dev))
+    _lib.check(st, "bcjr_fp8_quantize_blocks")
+    return q, scale
+
+
+def _need_fp8_weight(q, scale, offsets):
+    _need_dtype(q, "q", (_F8,))
+    _need_dtype(scale, "scale", (torch.float32,))
+    assert q.dim() == (2 if offsets is None else 3), \
+        f"q must be (N, K), or (E, N, K) with offsets, got {tuple(q.shape)}"
+    N, K = q.shape[-2:]
+    E = q.shape[0] if q.dim() == 3 else 1
+    assert 1 <= E <= _MAX_GROUPS, f"1 to {_MAX_GROUPS} experts, got {E}"
+    _need_features(N, "out features")
+    _need_features(K, "in features")
+    assert scale.shape == (*q.shape[:-2], _blocks(N), _blocks(K)), \
+        f"scale must be {(*q.shape[:-2], _blocks(N), _blocks(K))}, got {tuple(scale.shape)}"
+    assert not scale.requires_grad, "the scales of an e4m3 weight have no gradient"
+    _need_offsets(offsets, E)
+    return E, N, K
+
+
+def _fp8_mm(rows_ptr, ld, scale_ptr, scale_row, scale_block, q, scale, offsets, T, transpose, dtype):
+    N, K = q.shape[-2:]
+    E = q.shape[0] if q.dim() == 3 else 1
+    dev = q.device
+    q, scale = _dense(q), scale.contiguous()
+    out = torch.empty((T, K if transpose else N), dtype=dtype, device=dev)
+    offsets, off_ptr, off_size = _need_offsets(offsets, E)
+    with _on(dev):
+        st = _lib.load().bcjr_fp8_mm(rows_ptr, ld, scale_ptr, scale_row, scale_block, q.data_ptr(),
+                                     scale.data_ptr(), off_ptr, off_size, T, E, N, K,
+                                     int(transpose), out.data_ptr(), _DTYPES[dtype],
+                                     _status(dev).data_ptr(), _stream(dev))
+    _lib.check(st, "bcjr_fp8_mm")
+    return out
+
+
+def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
+    """Rows times a weight, both in e4m3: sum over blocks j of 128 of
+    x_scale[t, j] * scale[n // 128, j] * (xq[t, block j] . q[n, block j]).
+
+    xq, x_scale  (T, K) and (T, ceil(K / 128)), as ``fp8_quantize_rows`` returns
+    q, scale     (N, K) and its block scales, as ``fp8_quantize_weight`` returns;
+                 with ``offsets`` (see ``grouped_linear``) (E, N, K) and theirs
+    Returns (T, N) in ``out_dtype`` (bf16 or fp16).  Any fp32 scales are
+    accepted; the product of two scales is formed in fp32, so it should not
+    underflow."""
+    _need_cuda(xq=xq, x_scale=x_scale, q=q, scale=scale, offsets=offsets)
+    _need_dtype(xq, "xq", (_F8,))
+    _need_dtype(x_scale, "x_scale", (torch.float32,))
+    if out_dtype not in (torch.bfloat16, torch.float16):
+        raise ValueError(f"out_dtype must be torch.bfloat16 or torch.float16, got {out_dtype}")
+    E, N, K = _need_fp8_weight(q, scale, offsets)
+    assert xq.dim() == 2 and xq.shape[1] == K, f"xq must be (T, {K}), got {tuple(xq.shape)}"
+    assert x_scale.shape == (xq.shape[0], _blocks(K)), \
+        f"x_scale must be {(xq.shape[0], _blocks(K))}, got {tuple(x_scale.shape)}"
+    T = xq.shape[0]
+    if T == 0:
+        return torch.empty((0, N), dtype=out_dtype, device=xq.device)
+    xq, ld = _rows(xq)
+    if min(x_scale.stride()) < 0 or x_scale.stride(0) == 0 and T > 1:
+        x_scale = x_scale.contiguous()
+    return _fp8_mm(xq.data_ptr(), ld, x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1),
+                   q, scale, offsets, T, False, out_dtype)
+
+
+def _quantized_product(x, q, scale, offsets, transpose):
+    """x's rows, quantized, times the e4m3 weight (or its transpose).  The row
+    scales lie block by block, so that a tile reads those of its rows side by
+    side."""
+    T, C = x.shape
+    if T == 0:
+        return torch.empty((0, q.shape[-1] if transpose else q.shape[-2]), dtype=x.dtype,
+                           device=x.device)
+    body = -(-T * C // 16) * 16
+    ws = torch.empty(body + 4 * T * _blocks(C), dtype=torch.uint8, device=x.device)
+    rows, scales = ws.data_ptr(), ws.data_ptr() + body
+    _quantize_rows_into(x, rows, scales, 1, T)
+    return _fp8_mm(rows, C, scales, 1, T, q, scale, offsets, T, transpose, x.dtype)
+
+
+class _Fp8Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, q, scale, offsets):
+        ctx.save_for_backward(q, scale, offsets)
+        return _quantized_product(x, q, scale, offsets, False)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        q, scale, offsets = ctx.saved_tensors
+        dx = _quantized_product(dy, q, scale, offsets, True) if ctx.needs_input_grad[0] else None
+        return dx, None, None, None
+
+
+def fp8_linear(x, q, scale, offsets=None):
+    """x times an e4m3 weight: x's rows are quantized in segments of 128
+    (``fp8_quantize_rows``) and multiplied (``fp8_matmul``).
+
+    x         (..., K) bf16 or fp16; with ``offsets`` (T, K), rows sorted by expert
+    q, scale  (N, K) and its block scales, as ``fp8_quantize_weight`` returns;
+              with ``offsets`` (E, N, K) and theirs
+    Returns (..., N) in x's dtype.  Differentiable in x: the gradient of the
+    product with the stored weight, with the upstream gradient quantized in
+    row segments of 128; the rounding of x counts as the identity.  The weight
+    is constant."""
+    _need_cuda(x=x, q=q, scale=scale, offsets=offsets)
+    _need_dtype(x, "x", (torch.bfloat16, torch.float16))
+    E, N, K = _need_fp8_weight(q, scale, offsets)
+    assert x.dim() >= 1 and x.shape[-1] == K, f"x must be (..., {K}), got {tuple(x.shape)}"
+    assert offsets is None or x.dim() == 2, f"x must be (T, K) with offsets, got {tuple(x.shape)}"
+    if x.dim() == 2:
+        return _Fp8Linear.apply(x, q, scale, offsets)
+    return _Fp8Linear.apply(x.reshape(-1, K), q, scale, offsets).view(*x.shape[:-1], N)
+
+
+__all__ = ["grouped_linear", "fp8_quantize_rows", "fp8_quantize_weight", "fp8_matmul", "fp8_linear"]

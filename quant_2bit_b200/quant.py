@@ -28,6 +28,7 @@ import torch
 from . import _lib
 from .bcjr import (K_BITS, L_BITS, V_DIM, BcjrForwardBackwardMonolithic,
                    build_pred_succ_tables)
+from .linear import grouped_linear
 
 TX = 16
 TY = 16
@@ -267,9 +268,25 @@ def bcjr_quantize_layer(weights, signs_l, signs_r, codebook, T_temp, preds=None,
     return out
 
 
+def bcjr_experts_linear(x, offsets, weights, signs_l, signs_r, codebook, T_temp, preds=None,
+                        succs=None):
+    """The projection of an MoE layer whose experts are in BCJR mode: quantizes
+    the E weights (N, K) together (``bcjr_quantize_layer``) and multiplies the
+    rows of ``x`` (T, K), bf16 or fp16 and sorted by expert, with their expert's
+    weight (``linear.grouped_linear``; ``offsets`` as there).  What
+    QuantizedLinear.forward does for each expert (src/qat/quantized_linear.py:
+    204-211, :309-315; the quantized weight is cast to x's type there too), with
+    one launch of each kernel for all of them.  Returns (T, N); gradients flow
+    to x and to every weight."""
+    assert len(weights) >= 1, "at least one expert"
+    quantized = bcjr_quantize_layer(weights, signs_l, signs_r, codebook, T_temp, preds, succs)
+    return grouped_linear(x, torch.stack(quantized).to(x.dtype), offsets)
+
+
 __all__ = [
     "TX", "TY", "BCJR_CHUNK", "L_BITS", "K_BITS", "V_DIM", "make_sign_vector",
     "apply_rht_gpu", "apply_inverse_rht_gpu", "_tile_for_viterbi_gpu",
     "_untile_from_viterbi_gpu", "_bcjr_chunk_forward", "bcjr_quantize_tiles",
     "bcjr_quantize_weight_rotated", "bcjr_quantize_weight", "bcjr_quantize_layer",
+    "bcjr_experts_linear",
 ]

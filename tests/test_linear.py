@@ -1,0 +1,93 @@
+"""CPU tests of the linear layers' entry points: what the C ABI refuses before
+any device work, and that CPU tensors raise (there is no CPU path)."""
+import pytest
+import torch
+
+from quant_2bit_b200 import _lib
+
+OK, SHAPE, UNSUPPORTED, NULL, ALIGN = 0, 1, 2, 3, 4
+P = 1 << 20                       # stands for a device pointer: refused calls never use it
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from quant_2bit_b200 import build
+    build.build()
+    return _lib.load()
+
+
+def _mm(lib, rows=P, ld=64, w=P, off=P, off_size=4, T=8, E=2, N=32, K=64, dtype=0, tr=0, out=P,
+        status=P):
+    return lib.bcjr_grouped_mm(rows, ld, w, off, off_size, T, E, N, K, dtype, tr, out, status, None)
+
+
+def _wgrad(lib, dy=P, ld_dy=32, x=P, ld_x=64, off=P, off_size=4, T=8, E=2, N=32, K=64, dtype=0,
+           dw=P, status=P):
+    return lib.bcjr_grouped_wgrad(dy, ld_dy, x, ld_x, off, off_size, T, E, N, K, dtype, dw, status,
+                                  None)
+
+
+def _fp8(lib, rows=P, ld=64, xs=P, s_row=1, s_blk=8, w=P, ws=P, off=P, off_size=4, T=8, E=2, N=32,
+         K=64, tr=0, out=P, dtype=0, status=P):
+    return lib.bcjr_fp8_mm(rows, ld, xs, s_row, s_blk, w, ws, off, off_size, T, E, N, K, tr, out,
+                           dtype, status, None)
+
+
+@pytest.mark.parametrize("call", [_mm, _wgrad, _fp8])
+def test_products_refuse_bad_sizes(lib, call):
+    for bad in (dict(T=-1), dict(T=1 << 31), dict(E=0), dict(E=1025), dict(N=0), dict(N=24),
+                dict(K=8), dict(K=72), dict(off_size=2), dict(off=None), dict(N=1 << 25)):
+        assert call(lib, **bad) == SHAPE, bad
+    assert call(lib, dtype=2) == UNSUPPORTED
+    assert call(lib, dtype=-1) == UNSUPPORTED
+    assert call(lib, status=None) == NULL
+
+
+def test_products_refuse_bad_pointers_and_strides(lib):
+    assert _mm(lib, T=0, rows=None, out=None, status=None) == OK         # nothing to do
+    assert _fp8(lib, T=0, rows=None, xs=None, out=None, status=None) == OK
+    for call, names in ((_mm, ("rows", "w", "out")), (_wgrad, ("dy", "x", "dw")),
+                        (_fp8, ("rows", "xs", "w", "ws", "out"))):
+        for n in names:
+            assert call(lib, **{n: None}) == NULL, n
+    assert _mm(lib, ld=56) == SHAPE
+    assert _mm(lib, ld=68) == ALIGN
+    assert _mm(lib, tr=1, ld=24) == SHAPE
+    assert _mm(lib, rows=P + 8) == ALIGN
+    assert _mm(lib, w=P + 2) == ALIGN
+    assert _mm(lib, off=P + 4, off_size=8) == ALIGN
+    assert _wgrad(lib, ld_dy=16) == SHAPE
+    assert _wgrad(lib, ld_x=68) == ALIGN
+    assert _wgrad(lib, x=P + 8) == ALIGN
+    assert _fp8(lib, ld=72) == ALIGN
+    assert _fp8(lib, s_row=-1) == SHAPE
+    assert _fp8(lib, xs=P + 2) == ALIGN
+
+
+def test_quantizers_refuse(lib):
+    def rows(x=P, ld=64, n=8, k=64, dtype=0, q=P, s=P, s_row=1, s_blk=8):
+        return lib.bcjr_fp8_quantize_rows(x, ld, n, k, dtype, q, s, s_row, s_blk, None)
+
+    def blocks(w=P, E=1, N=8, K=64, dtype=0, q=P, s=P):
+        return lib.bcjr_fp8_quantize_blocks(w, E, N, K, dtype, q, s, None)
+
+    for bad in (dict(n=-1), dict(k=24), dict(k=0), dict(ld=48), dict(s_row=-1)):
+        assert rows(**bad) == SHAPE, bad
+    for bad in (dict(E=-1), dict(N=0), dict(K=24), dict(E=1 << 20, N=1 << 20)):
+        assert blocks(**bad) == SHAPE, bad
+    assert rows(dtype=3) == blocks(dtype=3) == UNSUPPORTED
+    assert rows(n=0, x=None) == blocks(E=0, w=None) == OK
+    assert rows(q=None) == blocks(s=None) == NULL
+    assert rows(x=P + 8) == rows(ld=68) == blocks(q=P + 4) == ALIGN
+
+
+def test_cpu_tensors_raise():
+    import quant_2bit_b200 as q
+    x, w = torch.zeros(4, 32, dtype=torch.bfloat16), torch.zeros(2, 16, 32, dtype=torch.bfloat16)
+    off = torch.tensor([0, 1, 4])
+    f8 = torch.zeros(16, 32).to(torch.float8_e4m3fn)
+    for f, args in ((q.grouped_linear, (x, w, off)), (q.fp8_quantize_rows, (x,)),
+                    (q.fp8_quantize_weight, (w,)), (q.fp8_linear, (x, f8, torch.ones(1, 1))),
+                    (q.fp8_matmul, (f8, torch.ones(16, 1), f8, torch.ones(1, 1)))):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            f(*args)
