@@ -238,7 +238,7 @@ int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long sc
     if (!rows || !rows_scale || !w || !w_scale || !out || !status) return BCJR_ERR_NULL_POINTER;
     const int depth = transpose_w ? N : K, lanes = transpose_w ? K : N;
     if (ld_rows < depth || ld_rows > (1L << 32) || scale_row < 0 || scale_block < 0) return BCJR_ERR_BAD_SHAPE;
-    if (!aligned(rows, 16) || ld_rows % 16 || !aligned(w, 16) || !aligned(out, 2) || !aligned(status, 4) ||
+    if (!aligned(rows, 16) || ld_rows % 16 || !aligned(w, 16) || !aligned(out, 16) || !aligned(status, 4) ||
         !aligned(rows_scale, 4) || !aligned(w_scale, 4) || (offsets && !aligned(offsets, size_t(offsets_bytes))))
         return BCJR_ERR_ALIGNMENT;
     const long kb = (K + 127) / 128, nb = (N + 127) / 128;

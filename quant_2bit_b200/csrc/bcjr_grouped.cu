@@ -47,7 +47,7 @@ int bcjr_grouped_mm(const void *rows, long ld_rows, const void *w, const void *o
     if (!rows || !w || !out || !status) return BCJR_ERR_NULL_POINTER;
     const int depth = transpose_w ? N : K, lanes = transpose_w ? K : N;
     if (ld_rows < depth || ld_rows > (1L << 32)) return BCJR_ERR_BAD_SHAPE;
-    if (!aligned(rows, 16) || ld_rows % 8 || !aligned(w, 16) || !aligned(out, 2) || !aligned(status, 4))
+    if (!aligned(rows, 16) || ld_rows % 8 || !aligned(w, 16) || !aligned(out, 16) || !aligned(status, 4))
         return BCJR_ERR_ALIGNMENT;
     Call c = {};
     c.kind = dtype == BCJR_BF16 ? kBF16 : kF16;
@@ -81,7 +81,7 @@ int bcjr_grouped_wgrad(const void *dy, long ld_dy, const void *x, long ld_x, con
     if (!dw || !status || (T > 0 && (!dy || !x))) return BCJR_ERR_NULL_POINTER;
     if (T > 0 && (ld_dy < N || ld_x < K || ld_dy > (1L << 32) || ld_x > (1L << 32)))
         return BCJR_ERR_BAD_SHAPE;
-    if (!aligned(dw, 2) || !aligned(status, 4)) return BCJR_ERR_ALIGNMENT;
+    if (!aligned(dw, 16) || !aligned(status, 4)) return BCJR_ERR_ALIGNMENT;
     if (T > 0 && (!aligned(dy, 16) || !aligned(x, 16) || ld_dy % 8 || ld_x % 8)) return BCJR_ERR_ALIGNMENT;
     cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
     if (T == 0)

@@ -38,7 +38,11 @@ enum { kForward = 0, kDgrad = 1, kWgrad = 2 };    // which product
 constexpr int kLanes = 128;                       // M of the matrix instruction
 constexpr int kRowBytes = 128;                    // one swizzled shared-memory row
 constexpr int kEpiWarps = 8;
-constexpr int kThreads = (kEpiWarps + 2) * 32;    // + one TMA warp, one MMA warp
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10;
+constexpr int kThreads = 384;                     // warp 11 has no role of its own
+constexpr int kChunk = 32;                        // columns that a half of the epilogue stores at once
+constexpr int kPitch = kLanes * 2 + 16;           // bytes of a staged output row: 16-byte pieces of
+                                                  // 8 rows fall into different banks
 constexpr int kMaxGroups = 1024;
 constexpr int kBoxRows = 64;                      // rows of one TMA box
 constexpr unsigned long long kWaitLimitNs = 1000000000ull;
@@ -172,19 +176,77 @@ __device__ __forceinline__ void tc_fence_after() {
 __device__ __forceinline__ void tmem_wait_ld() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
-// 16 columns of this warp's 32 lanes: one lane and 16 columns per thread.
-__device__ __forceinline__ void tmem_ld16(float (&v)[16], uint32_t addr) {
+// 16 lanes and 32 columns: v[4 j + i] of thread t is lane t / 4 + 8 (i / 2),
+// column 8 j + 2 (t % 4) + i % 2.
+__device__ __forceinline__ void tmem_ld(float (&v)[16], uint32_t addr) {
     uint32_t r[16];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
           "=r"(r[14]), "=r"(r[15])
-        : "r"(addr)
-        : "memory");
+        : "r"(addr));
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+}
+// The loaded registers may be used after this: it passes them through.
+__device__ __forceinline__ void tmem_wait(float (&a)[16], float (&b)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+f"(a[0]), "+f"(a[1]), "+f"(a[2]), "+f"(a[3]), "+f"(a[4]), "+f"(a[5]),
+                   "+f"(a[6]), "+f"(a[7]), "+f"(a[8]), "+f"(a[9]), "+f"(a[10]), "+f"(a[11]),
+                   "+f"(a[12]), "+f"(a[13]), "+f"(a[14]), "+f"(a[15])
+                 :
+                 : "memory");
+#pragma unroll
+    for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(b[i]));
+}
+// Four 8 x 8 blocks of 16-bit values, transposed on the way: thread t gives
+// row t / 4, columns 2 (t % 4).. of each; the address of thread 8 m + c
+// receives column c of block m.
+__device__ __forceinline__ void st_transposed(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                              uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};"
+                 ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                 ::"l"(dst), "r"(src), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() {
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+template <int LEFT> __device__ __forceinline__ void bulk_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() {
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+}
+// 4 bytes global -> shared, or zero.
+__device__ __forceinline__ void copy4(uint32_t dst, const float *src, bool real) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
+                 ::"r"(dst), "l"(src), "r"(real ? 4 : 0)
+                 : "memory");
+}
+// One arrival of this thread on `bar` when its copies so far have landed.
+__device__ __forceinline__ void copy_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void fence_async() {
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+// Registers of this warpgroup from here on.
+template <int N> __device__ __forceinline__ void regs_down() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N> __device__ __forceinline__ void regs_up() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+// The 128 threads of one half of the epilogue.
+__device__ __forceinline__ void half_sync(int half) {
+    asm volatile("bar.sync %0, 128;" ::"r"(half + 1) : "memory");
 }
 
 // Shared-memory operand descriptor, 128-byte swizzle.  K-major: rows of the
@@ -224,23 +286,23 @@ struct Groups {
 template <int COLS>
 __device__ __forceinline__ int col_tiles(int rows) { return (rows + COLS - 1) / COLS; }
 
-// One warp fills `g`.
+// Two steps: the whole block reads the bounds, then (after a block barrier)
+// one warp makes them monotone and counts tiles.
+__device__ __forceinline__ void read_groups(Groups &g, const Params &p) {
+    for (int e = threadIdx.x; e <= p.E; e += kThreads) {
+        long long v;
+        if (!p.offsets) v = e == 0 ? 0 : p.T;
+        else if (p.offsets64) v = static_cast<const long long *>(p.offsets)[e];
+        else v = static_cast<const int *>(p.offsets)[e];
+        g.off[e] = v < 0 ? 0 : v > p.T ? p.T : static_cast<int>(v);
+    }
+}
 template <int COLS>
-__device__ void load_groups(Groups &g, const Params &p, int lane) {
+__device__ __forceinline__ void scan_groups(Groups &g, const Params &p, int lane) {
     int high = 0, tiles = 0;        // last bound and tile count of the chunk before
     for (int base = 0; base <= p.E; base += 32) {
         const int e = base + lane;
-        int o = 0;
-        if (e <= p.E) {
-            if (!p.offsets) {
-                o = e == 0 ? 0 : p.T;
-            } else {
-                const long long v = p.offsets64
-                                        ? static_cast<const long long *>(p.offsets)[e]
-                                        : static_cast<long long>(static_cast<const int *>(p.offsets)[e]);
-                o = v < 0 ? 0 : v > p.T ? p.T : static_cast<int>(v);
-            }
-        }
+        int o = e <= p.E ? g.off[e] : 0;
         if (o < high) o = high;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -324,21 +386,68 @@ struct Walk {
 template <typename T> __device__ __forceinline__ T from_float(float v);
 template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
 template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
+template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b);
+template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
 
-template <int COLS, int STAGES>
+constexpr int kScaleStages = 8;
+
+// The e4m3 kernel with 256 columns holds 128 fp32 sums per epilogue thread.
+// It is launched with 168 registers a thread (3 warpgroups x 168 = 504) and
+// the third warpgroup hands most of its share to the other two: 56 + 2 x 224.
+constexpr int kLaunchRegs = 168, kFewRegs = 56, kManyRegs = 224;
+static_assert(kFewRegs + 2 * kManyRegs == 3 * kLaunchRegs, "");
+template <int KIND, int COLS> constexpr bool kSplitsRegs = KIND == kE4M3 && COLS == 256;
+
+template <int KIND, int COLS, int STAGES>
 struct Smem {
     static constexpr int kA = kLanes * kRowBytes;
     static constexpr int kB = COLS * kRowBytes;
     static constexpr int kStage = kA + kB;
+    static constexpr int kScales = KIND == kE4M3 ? kScaleStages : 1;
     struct Ctl {
         unsigned long long full[STAGES], empty[STAGES], tfull[2], tempty[2], done;
+        unsigned long long sfull[kScaleStages], sempty[kScaleStages];
         uint32_t tmem;
         int fail;
-        float scale[2][COLS];
+        alignas(16) float xs[kScales][COLS];      // e4m3: scales of the tile's rows, and
+        float ws[kScales];                        // of its weight block, one slot per k block
+        alignas(16) unsigned char stage[2][kChunk * kPitch];
         Groups groups;
     };
     static constexpr size_t bytes() { return 1024 + size_t(STAGES) * kStage + sizeof(Ctl); }
 };
+
+// 32 columns of the tile from one half of the epilogue: v[h] holds lanes
+// 16 h.. of this warp's 32.  Packed and transposed into rows of 128 features
+// in shared memory, then one bulk copy for each row that the output has.
+template <typename OUT>
+__device__ __forceinline__ void store_chunk(const float (&v)[2][16], unsigned char *stage, int half,
+                                            int quad, int lane, OUT *out, long ldo, int c0,
+                                            int valid, uint32_t bytes) {
+    if (lane < 8) bulk_wait_read<0>();
+    half_sync(half);
+    const uint32_t base = smem_u32(stage) + (lane & 7) * kPitch + quad * 64 + (lane >> 3) * 16;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        st_transposed(base + j * 8 * kPitch, pack<OUT>(v[0][4 * j], v[0][4 * j + 1]),
+                      pack<OUT>(v[0][4 * j + 2], v[0][4 * j + 3]),
+                      pack<OUT>(v[1][4 * j], v[1][4 * j + 1]),
+                      pack<OUT>(v[1][4 * j + 2], v[1][4 * j + 3]));
+    fence_async();
+    half_sync(half);
+    const int c = quad * 8 + lane;
+    if (lane < 8) {
+        if (c0 + c < valid) bulk_store(out + static_cast<long>(c0 + c) * ldo, smem_u32(stage) + c * kPitch, bytes);
+        bulk_commit();
+    }
+}
 
 // KIND: element type; OUT: output type; WHICH: product; COLS: columns of a
 // tile; STAGES: depth of the shared-memory ring.
@@ -357,7 +466,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     constexpr uint32_t B_STEP = B_MN ? KSLICE * kRowBytes : 32;
     constexpr uint32_t MN_BLOCK = BK * kRowBytes;     // an MN-major block of BK rows
     constexpr uint32_t TMEM_COLS = 2 * COLS < 32 ? 32 : 2 * COLS;
-    using S = Smem<COLS, STAGES>;
+    using S = Smem<KIND, COLS, STAGES>;
     static_assert(!(KIND == kE4M3 && WHICH == kWgrad), "e4m3 has forward and dgrad");
     static_assert(BK % kBoxRows == 0 && COLS % 16 == 0, "");
 
@@ -377,12 +486,18 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             bar_init(smem_u32(&ctl.tempty[i]), kEpiWarps);
         }
         bar_init(smem_u32(&ctl.done), 1);
+        for (int i = 0; i < kScaleStages; ++i) {
+            bar_init(smem_u32(&ctl.sfull[i]), 32);
+            bar_init(smem_u32(&ctl.sempty[i]), kEpiWarps);
+        }
         ctl.fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (blockIdx.x == 0 && p.status) *p.status = 0;   // a failure is a second away
     }
-    if (warp == kEpiWarps + 1) tmem_alloc(smem_u32(&ctl.tmem), TMEM_COLS);
-    if (warp == kEpiWarps) load_groups<COLS>(ctl.groups, p, lane);
+    if (warp == kMmaWarp) tmem_alloc(smem_u32(&ctl.tmem), TMEM_COLS);
+    read_groups(ctl.groups, p);
+    __syncthreads();
+    if (warp == kTmaWarp) scan_groups<COLS>(ctl.groups, p, lane);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -390,202 +505,233 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     Walk<WHICH, COLS> walk(ctl.groups, p);
     Tile t;
 
-    if (warp == kEpiWarps) {
-        // TMA producer
-        if (lane == 0) {
-            uint32_t it = 0;
+    // (a warpgroup sets its registers in one place, and the two sides meet only
+    // at the end: where branches meet, the compiler holds the code to the
+    // smaller share)
+    if (warp >= kEpiWarps) {
+        if constexpr (kSplitsRegs<KIND, COLS>) regs_down<kFewRegs>();
+        if (warp == kTmaWarp) {
+            // TMA producer
+            if (lane == 0) {
+                uint32_t it = 0;
+                bool ok = true;
+                while (ok && walk.next(t)) {
+                    const int nkb = (t.depth + BK - 1) / BK;
+                    const int bboxes = B_MN ? (t.ncols + MNB - 1) / MNB : (t.ncols + kBoxRows - 1) / kBoxRows;
+                    const uint32_t bytes = S::kA + bboxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes);
+                    for (int kb = 0; kb < nkb; ++kb, ++it) {
+                        const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
+                        if (!bar_wait(smem_u32(&ctl.empty[s]), ph ^ 1, fail, p.status)) {
+                            ok = false;
+                            break;
+                        }
+                        if (p.drop && blockIdx.x == 0 && it == 0) continue;
+                        const uint32_t bar = smem_u32(&ctl.full[s]);
+                        const uint32_t a = smem_u32(buf + s * S::kStage), b = a + S::kA;
+                        bar_expect(bar, bytes);
+                        const int kc = t.k0 + kb * BK;
+                        if constexpr (WHICH == kForward) {
+                            tma3(a, &ta, kc, t.lane_tile * kLanes, t.group, bar);
+                        } else if constexpr (WHICH == kDgrad) {
+#pragma unroll
+                            for (int j = 0; j < kLanes / MNB; ++j)
+                                tma3(a + j * MN_BLOCK, &ta, t.lane_tile * kLanes + j * MNB, kc, t.group, bar);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < kLanes / MNB; ++j)
+                                tma2(a + j * MN_BLOCK, &ta, t.lane_tile * kLanes + j * MNB, kc, bar);
+                        }
+                        for (int j = 0; j < bboxes; ++j) {
+                            if constexpr (B_MN)
+                                tma2(b + j * MN_BLOCK, &tb, t.col0 + j * MNB, kc, bar);
+                            else
+                                tma2(b + j * kBoxRows * kRowBytes, &tb, kc, t.col0 + j * kBoxRows, bar);
+                        }
+                    }
+                }
+                if (!ok) {
+                    // copies in flight land before the block ends
+                    volatile int never = 0;
+                    for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
+                        if (!(p.drop && blockIdx.x == 0 && i == 0))
+                            bar_wait(smem_u32(&ctl.full[i % STAGES]), (i / STAGES) & 1, &never, nullptr);
+                }
+            }
+        } else if (warp == kMmaWarp) {
+            // MMA issuer
+            uint32_t it = 0, acc = 0;
             bool ok = true;
             while (ok && walk.next(t)) {
                 const int nkb = (t.depth + BK - 1) / BK;
-                const int bboxes = B_MN ? (t.ncols + MNB - 1) / MNB : (t.ncols + kBoxRows - 1) / kBoxRows;
-                const uint32_t bytes = S::kA + bboxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes);
+                if (nkb == 0) continue;
+                const uint32_t idesc = instr_desc<KIND, A_MN, B_MN>(t.ncols);
                 for (int kb = 0; kb < nkb; ++kb, ++it) {
-                    const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
-                    if (!bar_wait(smem_u32(&ctl.empty[s]), ph ^ 1, fail, p.status)) {
+                    // e4m3: every stage has an accumulator buffer of its own
+                    // (scaled and added in fp32 registers); otherwise every tile
+                    if (KIND == kE4M3 || kb == 0) {
+                        if (!warp_wait(smem_u32(&ctl.tempty[acc & 1]), ((acc >> 1) & 1) ^ 1, fail, p.status)) {
+                            ok = false;
+                            break;
+                        }
+                        tc_fence_after();
+                    }
+                    const uint32_t s = it % STAGES;
+                    if (!warp_wait(smem_u32(&ctl.full[s]), (it / STAGES) & 1, fail, p.status)) {
                         ok = false;
                         break;
                     }
-                    if (p.drop && blockIdx.x == 0 && it == 0) continue;
-                    const uint32_t bar = smem_u32(&ctl.full[s]);
-                    const uint32_t a = smem_u32(buf + s * S::kStage), b = a + S::kA;
-                    bar_expect(bar, bytes);
-                    const int kc = t.k0 + kb * BK;
-                    if constexpr (WHICH == kForward) {
-                        tma3(a, &ta, kc, t.lane_tile * kLanes, t.group, bar);
-                    } else if constexpr (WHICH == kDgrad) {
-#pragma unroll
-                        for (int j = 0; j < kLanes / MNB; ++j)
-                            tma3(a + j * MN_BLOCK, &ta, t.lane_tile * kLanes + j * MNB, kc, t.group, bar);
-                    } else {
-#pragma unroll
-                        for (int j = 0; j < kLanes / MNB; ++j)
-                            tma2(a + j * MN_BLOCK, &ta, t.lane_tile * kLanes + j * MNB, kc, bar);
-                    }
-                    for (int j = 0; j < bboxes; ++j) {
-                        if constexpr (B_MN)
-                            tma2(b + j * MN_BLOCK, &tb, t.col0 + j * MNB, kc, bar);
-                        else
-                            tma2(b + j * kBoxRows * kRowBytes, &tb, kc, t.col0 + j * kBoxRows, bar);
-                    }
-                }
-            }
-            if (!ok) {
-                // copies in flight land before the block ends
-                volatile int never = 0;
-                for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-                    if (!(p.drop && blockIdx.x == 0 && i == 0))
-                        bar_wait(smem_u32(&ctl.full[i % STAGES]), (i / STAGES) & 1, &never, nullptr);
-            }
-        }
-    } else if (warp == kEpiWarps + 1) {
-        // MMA issuer
-        uint32_t it = 0, acc = 0;
-        bool ok = true;
-        while (ok && walk.next(t)) {
-            const int nkb = (t.depth + BK - 1) / BK;
-            if (nkb == 0) continue;
-            const uint32_t idesc = instr_desc<KIND, A_MN, B_MN>(t.ncols);
-            for (int kb = 0; kb < nkb; ++kb, ++it) {
-                // e4m3: every stage has an accumulator buffer of its own
-                // (scaled and added in fp32 registers); otherwise every tile
-                if (KIND == kE4M3 || kb == 0) {
-                    if (!warp_wait(smem_u32(&ctl.tempty[acc & 1]), ((acc >> 1) & 1) ^ 1, fail, p.status)) {
-                        ok = false;
-                        break;
+                    unsigned char *a = buf + s * S::kStage, *b = a + S::kA;
+                    if constexpr (WHICH == kWgrad) {
+                        const int rows = t.depth - kb * BK;
+                        if (rows < BK) {
+                            // rows of the next group (or behind the last one) do not
+                            // count, whatever they hold: both factors become zero
+                            const int cells = (BK - rows) * (kRowBytes / 16);
+                            const int blocks = kLanes / MNB + (t.ncols + MNB - 1) / MNB;
+                            for (int j = 0; j < blocks; ++j) {
+                                uint4 *z = reinterpret_cast<uint4 *>(a + j * MN_BLOCK + rows * kRowBytes);
+                                for (int i = lane; i < cells; i += 32) z[i] = make_uint4(0, 0, 0, 0);
+                            }
+                            fence_async();
+                            __syncwarp();
+                        }
                     }
                     tc_fence_after();
+                    if (lane == 0) {
+                        const uint64_t da = operand_desc(smem_u32(a), MN_BLOCK);
+                        const uint64_t db = operand_desc(smem_u32(b), MN_BLOCK);
+                        const uint32_t d = tmem + (acc & 1) * COLS;
+#pragma unroll
+                        for (int j = 0; j < SLICES; ++j)
+                            mma<KIND>(d, da + ((j * A_STEP) >> 4), db + ((j * B_STEP) >> 4), idesc,
+                                      (KIND == kE4M3 ? j > 0 : (kb | j) > 0) ? 1u : 0u);
+                        mma_commit(smem_u32(&ctl.empty[s]));
+                        if (KIND == kE4M3 || kb == nkb - 1) mma_commit(smem_u32(&ctl.tfull[acc & 1]));
+                    }
+                    __syncwarp();
+                    if (KIND == kE4M3 || kb == nkb - 1) ++acc;
                 }
-                const uint32_t s = it % STAGES;
-                if (!warp_wait(smem_u32(&ctl.full[s]), (it / STAGES) & 1, fail, p.status)) {
-                    ok = false;
-                    break;
-                }
-                unsigned char *a = buf + s * S::kStage, *b = a + S::kA;
-                if constexpr (WHICH == kWgrad) {
-                    const int rows = t.depth - kb * BK;
-                    if (rows < BK) {
-                        // rows of the next group (or behind the last one) do not
-                        // count, whatever they hold: both factors become zero
-                        const int cells = (BK - rows) * (kRowBytes / 16);
-                        const int blocks = kLanes / MNB + (t.ncols + MNB - 1) / MNB;
-                        for (int j = 0; j < blocks; ++j) {
-                            uint4 *z = reinterpret_cast<uint4 *>(a + j * MN_BLOCK + rows * kRowBytes);
-                            for (int i = lane; i < cells; i += 32) z[i] = make_uint4(0, 0, 0, 0);
-                        }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
+            }
+            // every matrix instruction has ended before the block frees its TMEM
+            if (lane == 0) mma_commit(smem_u32(&ctl.done));
+            volatile int never = 0;
+            bar_wait(smem_u32(&ctl.done), 0, &never, nullptr);
+        } else if (warp == kScaleWarp) {
+            // scales of the rows and of the weight block, one slot for each k block
+            if constexpr (KIND == kE4M3) {
+                uint32_t it = 0;
+                bool ok = true;
+                while (ok && walk.next(t)) {
+                    const int nkb = (t.depth + BK - 1) / BK;
+                    const float *xs = p.xs + static_cast<long>(t.col0) * p.xs_row;
+                    const float *ws = p.ws + t.group * p.ws_group + t.lane_tile * p.ws_lane;
+                    for (int kb = 0; kb < nkb; ++kb, ++it) {
+                        const uint32_t s = it % kScaleStages;
+                        ok = warp_wait(smem_u32(&ctl.sempty[s]), ((it / kScaleStages) & 1) ^ 1, fail, p.status);
+                        if (!ok) break;
+                        for (int c = lane; c < ((t.ncols + 31) & ~31); c += 32)
+                            copy4(smem_u32(&ctl.xs[s][c]), c < t.valid ? xs + c * p.xs_row + kb * p.xs_blk : p.xs,
+                                  c < t.valid);
+                        if (lane == 0) copy4(smem_u32(&ctl.ws[s]), ws + kb * p.ws_blk, true);
+                        copy_arrive(smem_u32(&ctl.sfull[s]));
                     }
                 }
-                tc_fence_after();
-                if (lane == 0) {
-                    const uint64_t da = operand_desc(smem_u32(a), MN_BLOCK);
-                    const uint64_t db = operand_desc(smem_u32(b), MN_BLOCK);
-                    const uint32_t d = tmem + (acc & 1) * COLS;
-#pragma unroll
-                    for (int j = 0; j < SLICES; ++j)
-                        mma<KIND>(d, da + ((j * A_STEP) >> 4), db + ((j * B_STEP) >> 4), idesc,
-                                  (KIND == kE4M3 ? j > 0 : (kb | j) > 0) ? 1u : 0u);
-                    mma_commit(smem_u32(&ctl.empty[s]));
-                    if (KIND == kE4M3 || kb == nkb - 1) mma_commit(smem_u32(&ctl.tfull[acc & 1]));
-                }
-                __syncwarp();
-                if (KIND == kE4M3 || kb == nkb - 1) ++acc;
+                asm volatile("cp.async.wait_all;" ::: "memory");
             }
         }
-        // every matrix instruction has ended before the block frees its TMEM
-        if (lane == 0) mma_commit(smem_u32(&ctl.done));
-        volatile int never = 0;
-        bar_wait(smem_u32(&ctl.done), 0, &never, nullptr);
     } else {
-        // epilogue: warp w reads lanes 32 (w % 4).., column chunks of 32 with
-        // index w / 4, w / 4 + 2, ...
-        constexpr int CHUNKS = COLS >= 64 ? COLS / 64 : 1;
+        if constexpr (kSplitsRegs<KIND, COLS>) regs_up<kManyRegs>();
+        // epilogue: warp w has lanes 32 (w % 4).., column chunks w / 4, w / 4 + 2, ...
+        constexpr int CHUNKS = COLS / (2 * kChunk);
+        static_assert(COLS % (2 * kChunk) == 0, "");
         const int quad = warp & 3, half = warp >> 2;
+        const uint32_t lanes_at = static_cast<uint32_t>(quad * 32) << 16;
+        unsigned char *stage = ctl.stage[half];
         uint32_t acc = 0;
         bool ok = true;
         while (walk.next(t)) {
             const int nkb = (t.depth + BK - 1) / BK;
-            const int feature = t.lane_tile * kLanes + quad * 32 + lane;
+            const int lane0 = t.lane_tile * kLanes;
+            const uint32_t bytes = min(kLanes, p.lanes - lane0) * sizeof(OUT);
             OUT *out = static_cast<OUT *>(p.out) + (WHICH == kWgrad ? t.group * p.out_group : 0) +
-                       static_cast<long>(t.col0) * p.ldo + feature;
-            const bool live = feature < p.lanes;
+                       static_cast<long>(t.col0) * p.ldo + lane0;
             if constexpr (KIND == kE4M3) {
-                float sum[CHUNKS * 32];
+                float sum[CHUNKS][2][16];
 #pragma unroll
-                for (int i = 0; i < CHUNKS * 32; ++i) sum[i] = 0.f;
-                const int c = threadIdx.x;
-                const float *xs = p.xs + static_cast<long>(t.col0 + c) * p.xs_row;
-                const float *ws = p.ws + t.group * p.ws_group + t.lane_tile * p.ws_lane;
-                const bool scales = c < t.valid;
-                float next = scales ? xs[0] * ws[0] : 0.f;
+                for (int i = 0; i < CHUNKS; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sum[i][j >> 4][j & 15] = 0.f;
                 for (int kb = 0; kb < nkb; ++kb, ++acc) {
-                    if (c < COLS) ctl.scale[acc & 1][c] = next;
-                    asm volatile("bar.sync 1, 256;" ::: "memory");
-                    if (kb + 1 < nkb)
-                        next = scales ? xs[(kb + 1) * p.xs_blk] * ws[(kb + 1) * p.ws_blk] : 0.f;
+                    const uint32_t s = acc % kScaleStages;
+                    if (ok) ok = warp_wait(smem_u32(&ctl.sfull[s]), (acc / kScaleStages) & 1, fail, p.status);
                     if (ok) ok = warp_wait(smem_u32(&ctl.tfull[acc & 1]), (acc >> 1) & 1, fail, p.status);
                     if (!ok) continue;
-                    __syncwarp();
                     tc_fence_after();
+                    const float ws = ctl.ws[s];
+                    const uint32_t at = tmem + lanes_at + (acc & 1) * COLS;
+                    // the next chunk's load runs under this chunk's sums
+                    float v[2][2][16];
+                    if (half * kChunk < t.ncols) {
+                        tmem_ld(v[0][0], at + half * kChunk);
+                        tmem_ld(v[0][1], at + half * kChunk + (16u << 16));
+                    }
 #pragma unroll
                     for (int i = 0; i < CHUNKS; ++i) {
-                        const int c0 = (half + 2 * i) * 32;
-                        if (c0 < t.ncols) {
+                        const int c0 = (half + 2 * i) * kChunk;
+                        if (c0 >= t.ncols) break;
+                        tmem_wait(v[i & 1][0], v[i & 1][1]);
+                        if (i + 1 < CHUNKS && c0 + 2 * kChunk < t.ncols) {
+                            tmem_ld(v[(i + 1) & 1][0], at + c0 + 2 * kChunk);
+                            tmem_ld(v[(i + 1) & 1][1], at + c0 + 2 * kChunk + (16u << 16));
+                        }
 #pragma unroll
-                            for (int h = 0; h < 2; ++h) {
-                                float v[16];
-                                tmem_ld16(v, tmem + (static_cast<uint32_t>(quad * 32) << 16) +
-                                                 (acc & 1) * COLS + c0 + h * 16);
-                                tmem_wait_ld();
-                                const float4 *sc = reinterpret_cast<const float4 *>(&ctl.scale[acc & 1][c0 + h * 16]);
+                        for (int j = 0; j < 4; ++j) {
+                            float2 f = *reinterpret_cast<const float2 *>(&ctl.xs[s][c0 + 8 * j + 2 * (lane & 3)]);
+                            f = __fmul2_rn(f, make_float2(ws, ws));
 #pragma unroll
-                                for (int q = 0; q < 4; ++q) {
-                                    const float4 f = sc[q];
-                                    float *o = &sum[i * 32 + h * 16 + q * 4];
-                                    o[0] = fmaf(v[4 * q], f.x, o[0]);
-                                    o[1] = fmaf(v[4 * q + 1], f.y, o[1]);
-                                    o[2] = fmaf(v[4 * q + 2], f.z, o[2]);
-                                    o[3] = fmaf(v[4 * q + 3], f.w, o[3]);
+                            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                                for (int q = 0; q < 4; q += 2) {
+                                    const int k = 4 * j + q;
+                                    const float2 r = __ffma2_rn(make_float2(v[i & 1][h][k], v[i & 1][h][k + 1]), f,
+                                                                make_float2(sum[i][h][k], sum[i][h][k + 1]));
+                                    sum[i][h][k] = r.x;
+                                    sum[i][h][k + 1] = r.y;
                                 }
-                            }
                         }
                     }
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(smem_u32(&ctl.tempty[acc & 1]));
+                    if (lane == 0) {
+                        bar_arrive(smem_u32(&ctl.tempty[acc & 1]));
+                        bar_arrive(smem_u32(&ctl.sempty[s]));
+                    }
                 }
-                if (live) {
 #pragma unroll
-                    for (int i = 0; i < CHUNKS; ++i)
+                for (int i = 0; i < CHUNKS; ++i) {
+                    const int c0 = (half + 2 * i) * kChunk;
+                    if (c0 >= t.valid) break;
+                    if (!ok) {
 #pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int col = (half + 2 * i) * 32 + j;
-                            if (col < t.valid)
-                                out[col * p.ldo] = from_float<OUT>(ok ? sum[i * 32 + j] : __int_as_float(0x7fffffff));
-                        }
+                        for (int j = 0; j < 32; ++j) sum[i][j >> 4][j & 15] = __int_as_float(0x7fffffff);
+                    }
+                    store_chunk<OUT>(sum[i], stage, half, quad, lane, out, p.ldo, c0, t.valid, bytes);
                 }
             } else {
                 if (nkb && ok) ok = warp_wait(smem_u32(&ctl.tfull[acc & 1]), (acc >> 1) & 1, fail, p.status);
-                __syncwarp();
                 tc_fence_after();
-                for (int c0 = half * 32; c0 < t.ncols; c0 += 64) {
+                const uint32_t at = tmem + lanes_at + (acc & 1) * COLS;
+                for (int c0 = half * kChunk; c0 < t.valid; c0 += 2 * kChunk) {
+                    float v[2][16];
+                    if (nkb && ok) {
+                        tmem_ld(v[0], at + c0);
+                        tmem_ld(v[1], at + c0 + (16u << 16));
+                        tmem_wait(v[0], v[1]);
+                    } else {
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        float v[16];
-                        if (nkb && ok) {
-                            tmem_ld16(v, tmem + (static_cast<uint32_t>(quad * 32) << 16) +
-                                             (acc & 1) * COLS + c0 + h * 16);
-                            tmem_wait_ld();
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < 16; ++j) v[j] = ok ? 0.f : __int_as_float(0x7fffffff);
-                        }
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const int col = c0 + h * 16 + j;
-                            if (live && col < t.valid) out[col * p.ldo] = from_float<OUT>(v[j]);
-                        }
+                        for (int j = 0; j < 32; ++j) v[j >> 4][j & 15] = ok ? 0.f : __int_as_float(0x7fffffff);
                     }
+                    store_chunk<OUT>(v, stage, half, quad, lane, out, p.ldo, c0, t.valid, bytes);
                 }
                 if (nkb) {
                     tc_fence_before();
@@ -595,6 +741,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 }
             }
         }
+        if (lane < 8) bulk_wait_all();
         if constexpr (WHICH != kWgrad) {
             // rows of no group are zero
             const int lo = ctl.groups.off[0], hi = ctl.groups.off[p.E];
@@ -608,7 +755,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    if (warp == kEpiWarps + 1) tmem_free(tmem, TMEM_COLS);
+    if (warp == kMmaWarp) tmem_free(tmem, TMEM_COLS);
 }
 
 // ---------------------------------------------------------------------------
@@ -659,10 +806,18 @@ cudaError_t launch(const Call &c) {
     if (sms <= 0) return cudaErrorInvalidDevice;
     if (!make_maps<KIND, WHICH>(c, ta, tb)) return cudaErrorInvalidValue;
     auto *k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES>;
-    constexpr size_t bytes = Smem<COLS, STAGES>::bytes();
+    constexpr size_t bytes = Smem<KIND, COLS, STAGES>::bytes();
     static_assert(bytes <= 232448, "shared memory of one block");
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
     if (e != cudaSuccess) return e;
+    if (kSplitsRegs<KIND, COLS>) {
+        // a split of more registers than the block was launched with would wait for good
+        static const int regs = [&] {
+            cudaFuncAttributes f;
+            return cudaFuncGetAttributes(&f, k) == cudaSuccess ? f.numRegs : 0;
+        }();
+        if (regs != kLaunchRegs) return cudaErrorInvalidConfiguration;
+    }
     // no more blocks than there can be tiles
     const long lane_tiles = (c.p.lanes + kLanes - 1) / kLanes;
     const long col_tiles = WHICH == kWgrad ? long(c.p.E) * ((c.p.cols + COLS - 1) / COLS)
