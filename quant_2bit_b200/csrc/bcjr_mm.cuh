@@ -38,14 +38,14 @@ enum { kForward = 0, kDgrad = 1, kWgrad = 2 };    // which product
 constexpr int kLanes = 128;                       // M of the matrix instruction
 constexpr int kRowBytes = 128;                    // one swizzled shared-memory row
 constexpr int kEpiWarps = 8;
-constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10;
-constexpr int kThreads = 384;                     // warp 11 has no role of its own
+constexpr int kTmaWarp = 8, kMmaWarp = 9, kScaleWarp = 10;   // scales: two warps
+constexpr int kThreads = 384;
 constexpr int kChunk = 32;                        // columns that a half of the epilogue stores at once
 constexpr int kPitch = kLanes * 2 + 16;           // bytes of a staged output row: 16-byte pieces of
                                                   // 8 rows fall into different banks
 constexpr int kMaxGroups = 1024;
 constexpr int kBoxRows = 64;                      // rows of one TMA box
-constexpr unsigned long long kWaitLimitNs = 1000000000ull;
+constexpr long long kWaitLimitClocks = 2000000000ll;   // about 1 s
 
 struct Params {
     const void *offsets;      // E + 1 group bounds, or NULL: one group of all rows
@@ -90,30 +90,27 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
 // Bounded wait (about 1 s).  False when it gave up or another warp of the
 // block did; the block then finishes with NaN outputs and the status word
 // says BCJR_ERR_TIMEOUT.
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *fail,
                                          int *status) {
     if (bar_try(bar, parity)) return true;
-    const unsigned long long t0 = now_ns();
+    const long long t0 = clock64();
     while (true) {
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < 32; ++i)
             if (bar_try(bar, parity)) return true;
         if (*fail) return false;
-        if (now_ns() - t0 > kWaitLimitNs) {
+        if (clock64() - t0 > kWaitLimitClocks) {
             *fail = 1;
             if (status) atomicExch(status, 8 /* BCJR_ERR_TIMEOUT */);
             return false;
         }
     }
 }
-// The same for a whole warp: every lane gets the same answer.
+// The same for a whole warp: every lane gets the same answer.  (All lanes
+// test the barrier; one lane that tests and hands its answer around measured
+// 5 % slower.)
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *fail,
                                           int *status) {
     return __all_sync(0xffffffffu, bar_wait(bar, parity, fail, status));
@@ -209,20 +206,6 @@ __device__ __forceinline__ void st_transposed(uint32_t addr, uint32_t a, uint32_
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};"
                  ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
-}
-__device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
-                 ::"l"(dst), "r"(src), "r"(bytes)
-                 : "memory");
-}
-__device__ __forceinline__ void bulk_commit() {
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-}
-template <int LEFT> __device__ __forceinline__ void bulk_wait_read() {
-    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(LEFT) : "memory");
-}
-__device__ __forceinline__ void bulk_wait_all() {
-    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 // 4 bytes global -> shared, or zero.
 __device__ __forceinline__ void copy4(uint32_t dst, const float *src, bool real) {
@@ -426,13 +409,15 @@ struct Smem {
 
 // 32 columns of the tile from one half of the epilogue: v[h] holds lanes
 // 16 h.. of this warp's 32.  Packed and transposed into rows of 128 features
-// in shared memory, then one bulk copy for each row that the output has.
+// in shared memory, and from there to the rows that the output has, 256
+// contiguous bytes for half a warp.  (One bulk copy for each row in place of
+// the vector stores took 22 clocks a row: 268 MB of weight gradients left at
+// 3.2 TB/s.)
 template <typename OUT>
 __device__ __forceinline__ void store_chunk(const float (&v)[2][16], unsigned char *stage, int half,
                                             int quad, int lane, OUT *out, long ldo, int c0,
-                                            int valid, uint32_t bytes) {
-    if (lane < 8) bulk_wait_read<0>();
-    half_sync(half);
+                                            int valid, int features) {
+    half_sync(half);               // the last chunk has been read
     const uint32_t base = smem_u32(stage) + (lane & 7) * kPitch + quad * 64 + (lane >> 3) * 16;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -440,12 +425,16 @@ __device__ __forceinline__ void store_chunk(const float (&v)[2][16], unsigned ch
                       pack<OUT>(v[0][4 * j + 2], v[0][4 * j + 3]),
                       pack<OUT>(v[1][4 * j], v[1][4 * j + 1]),
                       pack<OUT>(v[1][4 * j + 2], v[1][4 * j + 3]));
-    fence_async();
     half_sync(half);
-    const int c = quad * 8 + lane;
-    if (lane < 8) {
-        if (c0 + c < valid) bulk_store(out + static_cast<long>(c0 + c) * ldo, smem_u32(stage) + c * kPitch, bytes);
-        bulk_commit();
+    const int piece = lane & 15;
+    if (piece * 8 < features) {
+#pragma unroll
+        for (int i = 0; i < kChunk / 8; ++i) {
+            const int c = i * 8 + quad * 2 + (lane >> 4);
+            if (c0 + c < valid)
+                *reinterpret_cast<uint4 *>(out + static_cast<long>(c0 + c) * ldo + piece * 8) =
+                    *reinterpret_cast<const uint4 *>(stage + c * kPitch + piece * 16);
+        }
     }
 }
 
@@ -487,7 +476,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         }
         bar_init(smem_u32(&ctl.done), 1);
         for (int i = 0; i < kScaleStages; ++i) {
-            bar_init(smem_u32(&ctl.sfull[i]), 32);
+            bar_init(smem_u32(&ctl.sfull[i]), 64);
             bar_init(smem_u32(&ctl.sempty[i]), kEpiWarps);
         }
         ctl.fail = 0;
@@ -616,28 +605,44 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             if (lane == 0) mma_commit(smem_u32(&ctl.done));
             volatile int never = 0;
             bar_wait(smem_u32(&ctl.done), 0, &never, nullptr);
-        } else if (warp == kScaleWarp) {
-            // scales of the rows and of the weight block, one slot for each k block
-            if constexpr (KIND == kE4M3) {
-                uint32_t it = 0;
-                bool ok = true;
-                while (ok && walk.next(t)) {
-                    const int nkb = (t.depth + BK - 1) / BK;
-                    const float *xs = p.xs + static_cast<long>(t.col0) * p.xs_row;
-                    const float *ws = p.ws + t.group * p.ws_group + t.lane_tile * p.ws_lane;
-                    for (int kb = 0; kb < nkb; ++kb, ++it) {
-                        const uint32_t s = it % kScaleStages;
-                        ok = warp_wait(smem_u32(&ctl.sempty[s]), ((it / kScaleStages) & 1) ^ 1, fail, p.status);
-                        if (!ok) break;
-                        for (int c = lane; c < ((t.ncols + 31) & ~31); c += 32)
-                            copy4(smem_u32(&ctl.xs[s][c]), c < t.valid ? xs + c * p.xs_row + kb * p.xs_blk : p.xs,
-                                  c < t.valid);
-                        if (lane == 0) copy4(smem_u32(&ctl.ws[s]), ws + kb * p.ws_blk, true);
-                        copy_arrive(smem_u32(&ctl.sfull[s]));
-                    }
+        } else if constexpr (KIND == kE4M3) {
+            // Scales of the rows and of the weight block, one slot for each k
+            // block, fetched up to kScaleStages blocks ahead by two warps
+            // (alternate chunks of 32 columns).  Addresses and bounds are set
+            // up once for a tile: with one warp that formed them for each
+            // block, fetching scales took three times as long as the products.
+            constexpr int N = COLS / (2 * 32);
+            const int odd = warp - kScaleWarp;
+            uint32_t it = 0;
+            bool ok = true;
+            while (ok && walk.next(t)) {
+                const int nkb = (t.depth + BK - 1) / BK;
+                const float *ws = p.ws + t.group * p.ws_group + t.lane_tile * p.ws_lane;
+                const float *xs[N];
+                bool real[N];
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    const int c = (2 * i + odd) * 32 + lane;
+                    real[i] = c < t.valid;
+                    xs[i] = real[i] ? p.xs + (t.col0 + c) * p.xs_row : p.xs;
                 }
-                asm volatile("cp.async.wait_all;" ::: "memory");
+                for (int kb = 0; kb < nkb; ++kb, ++it) {
+                    const uint32_t s = it % kScaleStages;
+                    ok = warp_wait(smem_u32(&ctl.sempty[s]), ((it / kScaleStages) & 1) ^ 1, fail, p.status);
+                    if (!ok) break;
+                    const uint32_t dst = smem_u32(&ctl.xs[s][odd * 32 + lane]);
+#pragma unroll
+                    for (int i = 0; i < N; ++i)
+                        if ((2 * i + odd) * 32 < t.ncols) {
+                            copy4(dst + i * 256, xs[i], real[i]);
+                            if (real[i]) xs[i] += p.xs_blk;
+                        }
+                    if (lane == 0 && odd == 0) copy4(smem_u32(&ctl.ws[s]), ws, true);
+                    ws += p.ws_blk;
+                    copy_arrive(smem_u32(&ctl.sfull[s]));
+                }
             }
+            asm volatile("cp.async.wait_all;" ::: "memory");
         }
     } else {
         if constexpr (kSplitsRegs<KIND, COLS>) regs_up<kManyRegs>();
@@ -652,7 +657,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         while (walk.next(t)) {
             const int nkb = (t.depth + BK - 1) / BK;
             const int lane0 = t.lane_tile * kLanes;
-            const uint32_t bytes = min(kLanes, p.lanes - lane0) * sizeof(OUT);
+            const int features = min(kLanes, p.lanes - lane0);
             OUT *out = static_cast<OUT *>(p.out) + (WHICH == kWgrad ? t.group * p.out_group : 0) +
                        static_cast<long>(t.col0) * p.ldo + lane0;
             if constexpr (KIND == kE4M3) {
@@ -715,7 +720,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
 #pragma unroll
                         for (int j = 0; j < 32; ++j) sum[i][j >> 4][j & 15] = __int_as_float(0x7fffffff);
                     }
-                    store_chunk<OUT>(sum[i], stage, half, quad, lane, out, p.ldo, c0, t.valid, bytes);
+                    store_chunk<OUT>(sum[i], stage, half, quad, lane, out, p.ldo, c0, t.valid, features);
                 }
             } else {
                 if (nkb && ok) ok = warp_wait(smem_u32(&ctl.tfull[acc & 1]), (acc >> 1) & 1, fail, p.status);
@@ -731,7 +736,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j >> 4][j & 15] = ok ? 0.f : __int_as_float(0x7fffffff);
                     }
-                    store_chunk<OUT>(v, stage, half, quad, lane, out, p.ldo, c0, t.valid, bytes);
+                    store_chunk<OUT>(v, stage, half, quad, lane, out, p.ldo, c0, t.valid, features);
                 }
                 if (nkb) {
                     tc_fence_before();
@@ -741,7 +746,6 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 }
             }
         }
-        if (lane < 8) bulk_wait_all();
         if constexpr (WHICH != kWgrad) {
             // rows of no group are zero
             const int lo = ctl.groups.off[0], hi = ctl.groups.off[p.E];
