@@ -303,10 +303,10 @@ BCJR_API int bcjr_hyb_codebook(const float *lut, int Q, int L, float *cb_out, bc
  * the quantizers.  w is E x N x K, contiguous; row matrices are row-major with
  * ld elements between rows (a multiple of 16 bytes); bases 16-byte aligned.
  * Sums are fp32 and rounded once to the output type; results do not depend on
- * the run (no atomics).  `status` is one device int: 0, or BCJR_ERR_TIMEOUT if
- * a bounded device-side wait gave up (bcjr_ws_status reads it; the outputs
- * concerned are NaN).  It is written by every call with T > 0, so calls that
- * overlap need one each.
+ * the run (no atomics).  `status` is NULL or one device int that every call
+ * with T > 0 writes: 0, or BCJR_ERR_TIMEOUT if a bounded device-side wait
+ * gave up (bcjr_ws_status reads it; the outputs concerned are NaN, with or
+ * without a status word).
  */
 enum { BCJR_BF16 = 0, BCJR_F16 = 1, BCJR_F32 = 2 };
 
@@ -348,6 +348,17 @@ BCJR_API int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale
                          const void *offsets, int offsets_bytes, long T, int E, int N, int K,
                          int transpose_w, void *out, int out_dtype, int *status,
                          bcjr_stream_t stream);
+
+/* Both steps: the rows of x (T x depth, depth = K or, with transpose_w, N;
+ * BCJR_BF16 or BCJR_F16, the type of `out` too) quantized by rows into the
+ * workspace, and bcjr_fp8_mm.  The workspace (16-byte aligned, of
+ * bcjr_fp8_linear_workspace_bytes(T, depth) bytes, 0 for a bad size) is free
+ * again when the call has run on the stream. */
+BCJR_API size_t bcjr_fp8_linear_workspace_bytes(long T, int depth);
+BCJR_API int bcjr_fp8_linear(const void *x, long ld, int dtype, const void *w,
+                             const float *w_scale, const void *offsets, int offsets_bytes, long T,
+                             int E, int N, int K, int transpose_w, void *out, void *ws,
+                             size_t ws_bytes, int *status, bcjr_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -60,6 +60,8 @@ SIGNATURES = {
     "bcjr_fp8_quantize_rows": ([_P, _L, _L, _I, _I, _P, _P, _L, _L, _P], _I),
     "bcjr_fp8_quantize_blocks": ([_P, _I, _I, _I, _I, _P, _P, _P], _I),
     "bcjr_fp8_mm": ([_P, _L, _P, _L, _L, _P, _P, _P, _I, _L, _I, _I, _I, _I, _P, _I, _P, _P], _I),
+    "bcjr_fp8_linear_workspace_bytes": ([_L, _I], _SZ),
+    "bcjr_fp8_linear": ([_P, _L, _I, _P, _P, _P, _I, _L, _I, _I, _I, _I, _P, _P, _SZ, _P, _P], _I),
     "bcjr_probe_mufu": ([_P, _I, ctypes.POINTER(ctypes.c_double), _P], _I),
 }
 

@@ -169,10 +169,7 @@ cudaError_t run_blocks(const void *w, long blocks, int n, int k, void *q, float 
 
 template <typename OUT>
 cudaError_t run_mm(const Call &c) {
-    const bool small = c.p.T <= 64;
-    if (c.which == kForward)
-        return small ? launch<kE4M3, OUT, kForward, 64, 8>(c) : launch<kE4M3, OUT, kForward, 256, 4>(c);
-    return small ? launch<kE4M3, OUT, kDgrad, 64, 8>(c) : launch<kE4M3, OUT, kDgrad, 256, 4>(c);
+    return c.which == kForward ? launch_rows<kE4M3, OUT, kForward>(c) : launch_rows<kE4M3, OUT, kDgrad>(c);
 }
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
@@ -235,7 +232,7 @@ int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long sc
     if (out_dtype != BCJR_BF16 && out_dtype != BCJR_F16) return BCJR_ERR_UNSUPPORTED;
     if (offsets ? (offsets_bytes != 4 && offsets_bytes != 8) : E != 1) return BCJR_ERR_BAD_SHAPE;
     if (T == 0) return BCJR_OK;
-    if (!rows || !rows_scale || !w || !w_scale || !out || !status) return BCJR_ERR_NULL_POINTER;
+    if (!rows || !rows_scale || !w || !w_scale || !out) return BCJR_ERR_NULL_POINTER;
     const int depth = transpose_w ? N : K, lanes = transpose_w ? K : N;
     if (ld_rows < depth || ld_rows > (1L << 32) || scale_row < 0 || scale_block < 0) return BCJR_ERR_BAD_SHAPE;
     if (!aligned(rows, 16) || ld_rows % 16 || !aligned(w, 16) || !aligned(out, 16) || !aligned(status, 4) ||
@@ -270,6 +267,30 @@ int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long sc
     c.p.status = status;
     c.p.drop = bcjr::test_option(bcjr::kOptDropSends);
     return status_of(out_dtype == BCJR_BF16 ? run_mm<__nv_bfloat16>(c) : run_mm<__half>(c));
+}
+
+// The quantized rows first, then their scales, block by block, so that a tile
+// reads those of its rows side by side.
+size_t bcjr_fp8_linear_workspace_bytes(long T, int depth) {
+    if (T < 0 || T > 0x7fffff00L || depth < 16 || depth % 16 || depth > (1 << 24)) return 0;
+    return size_t(T) * depth + size_t(T) * ((depth + 127) / 128) * 4 + 16;
+}
+
+int bcjr_fp8_linear(const void *x, long ld, int dtype, const void *w, const float *w_scale,
+                    const void *offsets, int offsets_bytes, long T, int E, int N, int K,
+                    int transpose_w, void *out, void *ws, size_t ws_bytes, int *status,
+                    bcjr_stream_t stream) {
+    if (dtype != BCJR_BF16 && dtype != BCJR_F16) return BCJR_ERR_UNSUPPORTED;
+    const int depth = transpose_w ? N : K;
+    const size_t need = bcjr_fp8_linear_workspace_bytes(T, depth);
+    if (!need) return BCJR_ERR_BAD_SHAPE;
+    if (T > 0 && (!ws || ws_bytes < need)) return BCJR_ERR_WORKSPACE;
+    if (!aligned(ws, 16)) return BCJR_ERR_ALIGNMENT;
+    float *scale = reinterpret_cast<float *>(static_cast<char *>(ws) + size_t(T) * depth);
+    const int st = bcjr_fp8_quantize_rows(x, ld, T, depth, dtype, ws, scale, 1, T, stream);
+    if (st) return st;
+    return bcjr_fp8_mm(ws, depth, scale, 1, T, w, w_scale, offsets, offsets_bytes, T, E, N, K,
+                       transpose_w, out, dtype, status, stream);
 }
 
 }  // extern "C"

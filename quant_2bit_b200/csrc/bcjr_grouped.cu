@@ -11,11 +11,8 @@ namespace {
 
 template <int KIND, typename T>
 cudaError_t run(const Call &c) {
-    if (c.which == kWgrad) return launch<KIND, T, kWgrad, 256, 4>(c);
-    const bool small = c.p.T <= 64;
-    if (c.which == kForward)
-        return small ? launch<KIND, T, kForward, 64, 8>(c) : launch<KIND, T, kForward, 256, 4>(c);
-    return small ? launch<KIND, T, kDgrad, 64, 8>(c) : launch<KIND, T, kDgrad, 256, 4>(c);
+    if (c.which == kWgrad) return launch<KIND, T, kWgrad, 256, 4, false>(c);
+    return c.which == kForward ? launch_rows<KIND, T, kForward>(c) : launch_rows<KIND, T, kDgrad>(c);
 }
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
@@ -44,7 +41,7 @@ int bcjr_grouped_mm(const void *rows, long ld_rows, const void *w, const void *o
     const int st = check(offsets, offsets_bytes, T, E, N, K, dtype);
     if (st) return st;
     if (T == 0) return BCJR_OK;
-    if (!rows || !w || !out || !status) return BCJR_ERR_NULL_POINTER;
+    if (!rows || !w || !out) return BCJR_ERR_NULL_POINTER;
     const int depth = transpose_w ? N : K, lanes = transpose_w ? K : N;
     if (ld_rows < depth || ld_rows > (1L << 32)) return BCJR_ERR_BAD_SHAPE;
     if (!aligned(rows, 16) || ld_rows % 8 || !aligned(w, 16) || !aligned(out, 16) || !aligned(status, 4))
@@ -78,7 +75,7 @@ int bcjr_grouped_wgrad(const void *dy, long ld_dy, const void *x, long ld_x, con
                        int *status, bcjr_stream_t stream) {
     const int st = check(offsets, offsets_bytes, T, E, N, K, dtype);
     if (st) return st;
-    if (!dw || !status || (T > 0 && (!dy || !x))) return BCJR_ERR_NULL_POINTER;
+    if (!dw || (T > 0 && (!dy || !x))) return BCJR_ERR_NULL_POINTER;
     if (T > 0 && (ld_dy < N || ld_x < K || ld_dy > (1L << 32) || ld_x > (1L << 32)))
         return BCJR_ERR_BAD_SHAPE;
     if (!aligned(dw, 16) || !aligned(status, 4)) return BCJR_ERR_ALIGNMENT;

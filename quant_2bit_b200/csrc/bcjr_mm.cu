@@ -2,8 +2,6 @@
 // the size of a persistent grid.
 #include "bcjr_mm.cuh"
 
-#include <mutex>
-
 #include "bcjr_kernels.h"
 
 namespace bcjr {
@@ -18,15 +16,16 @@ typedef CUresult (*EncodeFn)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, voi
 // The driver's encoder, found through the runtime (the library does not link
 // libcuda, so it loads on machines without a driver).
 EncodeFn encoder() {
-    static std::mutex mu;
-    static EncodeFn fn = nullptr;
-    std::lock_guard<std::mutex> lk(mu);
+    static std::atomic<EncodeFn> found{nullptr};
+    EncodeFn fn = found.load(std::memory_order_relaxed);
     if (!fn) {
         void *p = nullptr;
         cudaDriverEntryPointQueryResult q;
-        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) == cudaSuccess &&
-            q == cudaDriverEntryPointSuccess)
-            fn = reinterpret_cast<EncodeFn>(p);
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &q) != cudaSuccess ||
+            q != cudaDriverEntryPointSuccess)
+            return nullptr;
+        fn = reinterpret_cast<EncodeFn>(p);
+        found.store(fn, std::memory_order_relaxed);
     }
     return fn;
 }
@@ -51,27 +50,25 @@ bool make_map(CUtensorMap *m, int kind, int rank, const void *base, const unsign
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int grid_sms() {
-    static std::mutex mu;
-    static int sms[64], major[64];
+int grid_sms(int *device) {
+    static std::atomic<int> count[kMaxDevices];       // SMs, -1: not sm_100, 0: not asked yet
     int dev = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= kMaxDevices) return 0;
     // The map encoder wants a current context, which a thread that has made no
     // runtime call on the device yet (autograd's) does not have.
     if (cudaSetDevice(dev) != cudaSuccess) return 0;
-    {
-        std::lock_guard<std::mutex> lk(mu);
-        if (!sms[dev]) {
-            int n = 0, mj = 0;
-            if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-                cudaDeviceGetAttribute(&mj, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
-                return 0;
-            major[dev] = mj;
-            sms[dev] = n;
-        }
-        if (major[dev] != 10) return 0;
+    int n = count[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        int sms = 0, major = 0;
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+            cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess)
+            return 0;
+        n = major == 10 && sms > 0 ? sms : -1;
+        count[dev].store(n, std::memory_order_relaxed);
     }
-    const int n = sms[dev] - reserved_sms();
+    if (n < 0) return 0;
+    *device = dev;
+    n -= reserved_sms();
     return n > 0 ? n : 1;
 }
 

@@ -27,6 +27,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 
 namespace bcjr {
@@ -83,7 +84,7 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar) {
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;"
+        "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;"
         " selp.u32 %0, 1, 0, p; }"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
@@ -217,6 +218,35 @@ __device__ __forceinline__ void copy4(uint32_t dst, const float *src, bool real)
 __device__ __forceinline__ void copy_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
+// Thread block clusters: own rank, size, id; the address of `addr` in rank r.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t cluster_size() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint32_t in_rank(uint32_t addr, uint32_t r) {
+    uint32_t a;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(addr), "r"(r));
+    return a;
+}
+__device__ __forceinline__ void bar_arrive_in(uint32_t bar, uint32_t r) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_rank(bar, r))
+                 : "memory");
+}
+__device__ __forceinline__ float2 load2_in(uint32_t addr, uint32_t r) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_rank(addr, r)) : "memory");
+    return v;
+}
 __device__ __forceinline__ void fence_async() {
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -317,20 +347,26 @@ struct Tile {
     int valid;      // columns to write
     int ncols;      // columns computed, a multiple of 16
     int k0;         // first contraction index (wgrad: row of X)
-    int depth;      // contraction length (0: the output is zero)
+    int depth;      // contraction length from k0 on
+    int nkb;        // its stages (0: the output is zero)
 };
 
 // The tiles of a block, one after the other; every warp walks the same list.
-template <int WHICH, int COLS>
+// SPLIT: the blocks of a cluster share each tile, every one with its part of
+// the contraction.
+template <int WHICH, int COLS, int BK, bool SPLIT>
 struct Walk {
     const Groups &g;
     const Params &p;
-    int lane_tiles, total, tile, group;
+    int lane_tiles, total, tile, step, group, part, parts;
     __device__ Walk(const Groups &g_, const Params &p_) : g(g_), p(p_) {
+        parts = SPLIT ? cluster_size() : 1;
+        part = SPLIT ? cluster_rank() : 0;
+        step = gridDim.x / parts;
         lane_tiles = (p.lanes + kLanes - 1) / kLanes;
         total = WHICH == kWgrad ? p.E * lane_tiles * col_tiles<COLS>(p.cols)
                                 : g.first[p.E] * lane_tiles;
-        tile = blockIdx.x;
+        tile = blockIdx.x / parts;
         group = 0;
     }
     __device__ bool next(Tile &t) {
@@ -345,6 +381,7 @@ struct Walk {
             t.ncols = t.valid;               // cols is a multiple of 16
             t.k0 = g.off[t.group];
             t.depth = g.off[t.group + 1] - t.k0;
+            t.nkb = (t.depth + BK - 1) / BK;
         } else {
             while (tile >= g.first[group + 1] * lane_tiles) ++group;
             const int in = tile - g.first[group] * lane_tiles;
@@ -358,10 +395,13 @@ struct Walk {
             t.col0 = g.off[group] + c * share;
             t.valid = min(share, g.off[group + 1] - t.col0);
             t.ncols = (t.valid + 15) & ~15;
-            t.k0 = 0;
-            t.depth = p.depth;
+            const int nkb = (p.depth + BK - 1) / BK;
+            const int kb0 = SPLIT ? nkb * part / parts : 0;
+            t.nkb = (SPLIT ? nkb * (part + 1) / parts : nkb) - kb0;
+            t.k0 = kb0 * BK;
+            t.depth = p.depth - t.k0;
         }
-        tile += gridDim.x;
+        tile += step;
         return true;
     }
 };
@@ -380,6 +420,7 @@ template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
 }
 
 constexpr int kScaleStages = 8;
+constexpr int kPartPitch = kLanes + 4;            // floats: no bank conflicts either way
 
 // The e4m3 kernel with 256 columns holds 128 fp32 sums per epilogue thread.
 // It is launched with 168 registers a thread (3 warpgroups x 168 = 504) and
@@ -388,7 +429,7 @@ constexpr int kLaunchRegs = 168, kFewRegs = 56, kManyRegs = 224;
 static_assert(kFewRegs + 2 * kManyRegs == 3 * kLaunchRegs, "");
 template <int KIND, int COLS> constexpr bool kSplitsRegs = KIND == kE4M3 && COLS == 256;
 
-template <int KIND, int COLS, int STAGES>
+template <int KIND, int COLS, int STAGES, bool SPLIT>
 struct Smem {
     static constexpr int kA = kLanes * kRowBytes;
     static constexpr int kB = COLS * kRowBytes;
@@ -401,7 +442,9 @@ struct Smem {
         int fail;
         alignas(16) float xs[kScales][COLS];      // e4m3: scales of the tile's rows, and
         float ws[kScales];                        // of its weight block, one slot per k block
-        alignas(16) unsigned char stage[2][kChunk * kPitch];
+        alignas(16) unsigned char stage[2][SPLIT ? 16 : kChunk * kPitch];
+        unsigned long long pfull;                 // a split tile's sums: written by all blocks;
+        alignas(16) float part[SPLIT ? COLS : 1][kPartPitch];     // this block's
         Groups groups;
     };
     static constexpr size_t bytes() { return 1024 + size_t(STAGES) * kStage + sizeof(Ctl); }
@@ -438,9 +481,50 @@ __device__ __forceinline__ void store_chunk(const float (&v)[2][16], unsigned ch
     }
 }
 
+// A tile whose contraction is split over the blocks of a cluster: every block
+// leaves its fp32 sums in its shared memory, and block r adds those of all
+// blocks, in the order of their ranks, for features r * 128 / size .. and
+// writes them.  (A cluster has one tile: the launch gives every tile a cluster
+// of its own, and nobody overwrites the sums.)  A block that failed leaves NaN.
+template <typename OUT>
+__device__ __forceinline__ bool add_parts(const float (&v)[2][16], float (*part)[kPartPitch],
+                                          uint32_t pfull, int half, int quad, int lane,
+                                          OUT *out, long ldo, int valid,
+                                          int features, bool ok, volatile int *fail, int *status) {
+    const uint32_t size = cluster_size(), rank = cluster_rank();
+    const int f0 = quad * 32 + (lane >> 2), c0 = half * kChunk + 2 * (lane & 3);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                if (c0 + 8 * j + (q & 1) < valid)
+                    part[c0 + 8 * j + (q & 1)][f0 + 16 * h + 8 * (q >> 1)] =
+                        ok ? v[h][4 * j + q] : __int_as_float(0x7fffffff);
+    __syncwarp();
+    if (lane < size) bar_arrive_in(pfull, lane);
+    if (ok) ok = warp_wait(pfull, 0, fail, status);
+    const int per = kLanes / 2 / size;              // feature pairs of this block
+    for (int i = threadIdx.x; i < valid * per; i += kEpiWarps * 32) {
+        const int c = i / per, f = (rank * per + i - c * per) * 2;
+        if (f >= features) continue;
+        const uint32_t at = smem_u32(&part[c][f]);
+        float2 s = load2_in(at, 0);
+        for (uint32_t r = 1; r < size; ++r) {
+            const float2 w = load2_in(at, r);
+            s.x += w.x;
+            s.y += w.y;
+        }
+        if (!ok) s.x = s.y = __int_as_float(0x7fffffff);
+        *reinterpret_cast<uint32_t *>(out + c * ldo + f) = pack<OUT>(s.x, s.y);
+    }
+    return ok;
+}
+
 // KIND: element type; OUT: output type; WHICH: product; COLS: columns of a
-// tile; STAGES: depth of the shared-memory ring.
-template <int KIND, typename OUT, int WHICH, int COLS, int STAGES>
+// tile; STAGES: depth of the shared-memory ring; SPLIT: clusters share tiles.
+template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1)
 mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
           const __grid_constant__ Params p) {
@@ -455,7 +539,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     constexpr uint32_t B_STEP = B_MN ? KSLICE * kRowBytes : 32;
     constexpr uint32_t MN_BLOCK = BK * kRowBytes;     // an MN-major block of BK rows
     constexpr uint32_t TMEM_COLS = 2 * COLS < 32 ? 32 : 2 * COLS;
-    using S = Smem<KIND, COLS, STAGES>;
+    using S = Smem<KIND, COLS, STAGES, SPLIT>;
     static_assert(!(KIND == kE4M3 && WHICH == kWgrad), "e4m3 has forward and dgrad");
     static_assert(BK % kBoxRows == 0 && COLS % 16 == 0, "");
 
@@ -475,6 +559,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             bar_init(smem_u32(&ctl.tempty[i]), kEpiWarps);
         }
         bar_init(smem_u32(&ctl.done), 1);
+        if constexpr (SPLIT) bar_init(smem_u32(&ctl.pfull), kEpiWarps * cluster_size());
         for (int i = 0; i < kScaleStages; ++i) {
             bar_init(smem_u32(&ctl.sfull[i]), 64);
             bar_init(smem_u32(&ctl.sempty[i]), kEpiWarps);
@@ -488,10 +573,11 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     __syncthreads();
     if (warp == kTmaWarp) scan_groups<COLS>(ctl.groups, p, lane);
     tc_fence_before();
-    __syncthreads();
+    if constexpr (SPLIT) cluster_sync();
+    else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl.tmem;
-    Walk<WHICH, COLS> walk(ctl.groups, p);
+    Walk<WHICH, COLS, BK, SPLIT> walk(ctl.groups, p);
     Tile t;
 
     // (a warpgroup sets its registers in one place, and the two sides meet only
@@ -505,7 +591,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 uint32_t it = 0;
                 bool ok = true;
                 while (ok && walk.next(t)) {
-                    const int nkb = (t.depth + BK - 1) / BK;
+                    const int nkb = t.nkb;
                     const int bboxes = B_MN ? (t.ncols + MNB - 1) / MNB : (t.ncols + kBoxRows - 1) / kBoxRows;
                     const uint32_t bytes = S::kA + bboxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes);
                     for (int kb = 0; kb < nkb; ++kb, ++it) {
@@ -551,7 +637,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             uint32_t it = 0, acc = 0;
             bool ok = true;
             while (ok && walk.next(t)) {
-                const int nkb = (t.depth + BK - 1) / BK;
+                const int nkb = t.nkb;
                 if (nkb == 0) continue;
                 const uint32_t idesc = instr_desc<KIND, A_MN, B_MN>(t.ncols);
                 for (int kb = 0; kb < nkb; ++kb, ++it) {
@@ -616,15 +702,16 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             uint32_t it = 0;
             bool ok = true;
             while (ok && walk.next(t)) {
-                const int nkb = (t.depth + BK - 1) / BK;
-                const float *ws = p.ws + t.group * p.ws_group + t.lane_tile * p.ws_lane;
+                const int nkb = t.nkb;
+                const long kb0 = t.k0 / BK;
+                const float *ws = p.ws + t.group * p.ws_group + t.lane_tile * p.ws_lane + kb0 * p.ws_blk;
                 const float *xs[N];
                 bool real[N];
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     const int c = (2 * i + odd) * 32 + lane;
                     real[i] = c < t.valid;
-                    xs[i] = real[i] ? p.xs + (t.col0 + c) * p.xs_row : p.xs;
+                    xs[i] = real[i] ? p.xs + (t.col0 + c) * p.xs_row + kb0 * p.xs_blk : p.xs;
                 }
                 for (int kb = 0; kb < nkb; ++kb, ++it) {
                     const uint32_t s = it % kScaleStages;
@@ -652,10 +739,11 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         const int quad = warp & 3, half = warp >> 2;
         const uint32_t lanes_at = static_cast<uint32_t>(quad * 32) << 16;
         unsigned char *stage = ctl.stage[half];
+        static_assert(!SPLIT || CHUNKS == 1, "");
         uint32_t acc = 0;
         bool ok = true;
         while (walk.next(t)) {
-            const int nkb = (t.depth + BK - 1) / BK;
+            const int nkb = t.nkb;
             const int lane0 = t.lane_tile * kLanes;
             const int features = min(kLanes, p.lanes - lane0);
             OUT *out = static_cast<OUT *>(p.out) + (WHICH == kWgrad ? t.group * p.out_group : 0) +
@@ -715,19 +803,22 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
 #pragma unroll
                 for (int i = 0; i < CHUNKS; ++i) {
                     const int c0 = (half + 2 * i) * kChunk;
-                    if (c0 >= t.valid) break;
+                    if (!SPLIT && c0 >= t.valid) break;
                     if (!ok) {
 #pragma unroll
                         for (int j = 0; j < 32; ++j) sum[i][j >> 4][j & 15] = __int_as_float(0x7fffffff);
                     }
-                    store_chunk<OUT>(sum[i], stage, half, quad, lane, out, p.ldo, c0, t.valid, features);
+                    if constexpr (!SPLIT)
+                        store_chunk<OUT>(sum[i], stage, half, quad, lane, out, p.ldo, c0, t.valid, features);
                 }
+                if constexpr (SPLIT)
+                    ok = add_parts<OUT>(sum[0], ctl.part, smem_u32(&ctl.pfull), half, quad, lane, out, p.ldo, t.valid, features, ok, fail, p.status);
             } else {
                 if (nkb && ok) ok = warp_wait(smem_u32(&ctl.tfull[acc & 1]), (acc >> 1) & 1, fail, p.status);
                 tc_fence_after();
                 const uint32_t at = tmem + lanes_at + (acc & 1) * COLS;
-                for (int c0 = half * kChunk; c0 < t.valid; c0 += 2 * kChunk) {
-                    float v[2][16];
+                float v[2][16];
+                for (int c0 = half * kChunk; c0 < (SPLIT ? COLS : t.valid); c0 += 2 * kChunk) {
                     if (nkb && ok) {
                         tmem_ld(v[0], at + c0);
                         tmem_ld(v[1], at + c0 + (16u << 16));
@@ -736,7 +827,8 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
 #pragma unroll
                         for (int j = 0; j < 32; ++j) v[j >> 4][j & 15] = ok ? 0.f : __int_as_float(0x7fffffff);
                     }
-                    store_chunk<OUT>(v, stage, half, quad, lane, out, p.ldo, c0, t.valid, features);
+                    if constexpr (!SPLIT)
+                        store_chunk<OUT>(v, stage, half, quad, lane, out, p.ldo, c0, t.valid, features);
                 }
                 if (nkb) {
                     tc_fence_before();
@@ -744,6 +836,8 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                     if (lane == 0) bar_arrive(smem_u32(&ctl.tempty[acc & 1]));
                     ++acc;
                 }
+                if constexpr (SPLIT)
+                    ok = add_parts<OUT>(v, ctl.part, smem_u32(&ctl.pfull), half, quad, lane, out, p.ldo, t.valid, features, ok, fail, p.status);
             }
         }
         if constexpr (WHICH != kWgrad) {
@@ -756,8 +850,10 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             }
         }
     }
+    __syncwarp();
     tc_fence_before();
-    __syncthreads();
+    if constexpr (SPLIT) cluster_sync();       // nobody reads this block's sums any more
+    else __syncthreads();
     tc_fence_after();
     if (warp == kMmaWarp) tmem_free(tmem, TMEM_COLS);
 }
@@ -770,8 +866,9 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
 bool make_map(CUtensorMap *m, int kind, int rank, const void *base, const unsigned long long *dims,
               const unsigned long long *strides, const unsigned *box);
 // SMs of the current device for a persistent grid (less the reserved ones);
-// 0 when the device is not sm_100.
-int grid_sms();
+// 0 when the device is not sm_100.  Makes the device's context current.
+constexpr int kMaxDevices = 64;
+int grid_sms(int *device);
 
 struct Call {
     int kind, which;          // element type, product
@@ -779,9 +876,11 @@ struct Call {
     long ld_a, ld_b;          // elements between rows of wgrad's X; of the row matrix
     long a_rows, a_inner;     // weight rows (N) and row length (K); wgrad: K in a_inner
     long b_inner;             // row length of the row matrix
+    int split;                // blocks that share a tile
     cudaStream_t stream;
     Params p;
 };
+constexpr int kMaxSplit = 8;
 
 // Both operand maps of a call.
 template <int KIND, int WHICH>
@@ -803,32 +902,65 @@ bool make_maps(const Call &c, CUtensorMap &ta, CUtensorMap &tb) {
     return make_map(&tb, KIND, 2, c.b, dims, st, box);
 }
 
-template <int KIND, typename OUT, int WHICH, int COLS, int STAGES>
+template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, bool SPLIT>
 cudaError_t launch(const Call &c) {
     CUtensorMap ta, tb;
-    const int sms = grid_sms();
+    int dev = 0;
+    const int sms = grid_sms(&dev);
     if (sms <= 0) return cudaErrorInvalidDevice;
     if (!make_maps<KIND, WHICH>(c, ta, tb)) return cudaErrorInvalidValue;
-    auto *k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES>;
-    constexpr size_t bytes = Smem<KIND, COLS, STAGES>::bytes();
+    auto *k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES, SPLIT>;
+    constexpr size_t bytes = Smem<KIND, COLS, STAGES, SPLIT>::bytes();
     static_assert(bytes <= 232448, "shared memory of one block");
-    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-    if (e != cudaSuccess) return e;
-    if (kSplitsRegs<KIND, COLS>) {
-        // a split of more registers than the block was launched with would wait for good
-        static const int regs = [&] {
+    static std::atomic<bool> ready[kMaxDevices];      // this kernel's setting on each device
+    if (!ready[dev].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+        if (e != cudaSuccess) return e;
+        if (kSplitsRegs<KIND, COLS>) {
+            // a split of more registers than the block was launched with would wait for good
             cudaFuncAttributes f;
-            return cudaFuncGetAttributes(&f, k) == cudaSuccess ? f.numRegs : 0;
-        }();
-        if (regs != kLaunchRegs) return cudaErrorInvalidConfiguration;
+            if (cudaFuncGetAttributes(&f, k) != cudaSuccess || f.numRegs != kLaunchRegs)
+                return cudaErrorInvalidConfiguration;
+        }
+        ready[dev].store(true, std::memory_order_release);
     }
     // no more blocks than there can be tiles
     const long lane_tiles = (c.p.lanes + kLanes - 1) / kLanes;
     const long col_tiles = WHICH == kWgrad ? long(c.p.E) * ((c.p.cols + COLS - 1) / COLS)
                                            : c.p.T / COLS + (c.p.E < c.p.T ? c.p.E : c.p.T);
     const long tiles = lane_tiles * (col_tiles > 0 ? col_tiles : 1);
+    if constexpr (SPLIT) {
+        if (tiles * c.split > 0x7fffffffL) return cudaErrorInvalidValue;
+        cudaLaunchAttribute a;
+        a.id = cudaLaunchAttributeClusterDimension;
+        a.val.clusterDim.x = unsigned(c.split);
+        a.val.clusterDim.y = a.val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(unsigned(tiles * c.split));
+        cfg.blockDim = dim3(kThreads);
+        cfg.dynamicSmemBytes = bytes;
+        cfg.stream = c.stream;
+        cfg.attrs = &a;
+        cfg.numAttrs = 1;
+        return cudaLaunchKernelEx(&cfg, k, ta, tb, c.p);
+    }
     k<<<unsigned(tiles < sms ? tiles : sms), kThreads, bytes, c.stream>>>(ta, tb, c.p);
     return cudaGetLastError();
+}
+
+// Forward and dgrad.  Up to 64 rows every group is one tile of at most 64
+// columns, and with few tiles the blocks of a cluster share each one.
+template <int KIND, typename OUT, int WHICH>
+cudaError_t launch_rows(Call c) {
+    if (c.p.T > 64) return launch<KIND, OUT, WHICH, 256, 4, false>(c);
+    int dev = 0;
+    const int sms = grid_sms(&dev);
+    const int nkb = (c.p.depth * (KIND == kE4M3 ? 1 : 2) + kRowBytes - 1) / kRowBytes;
+    const long tiles = (c.p.lanes + kLanes - 1L) / kLanes * (c.p.E < c.p.T ? c.p.E : c.p.T);
+    c.split = 1;
+    while (c.split < kMaxSplit && tiles * c.split * 2 <= sms && nkb >= c.split * 2 * 2) c.split *= 2;
+    if (c.split == 1) return launch<KIND, OUT, WHICH, 64, 8, false>(c);
+    return launch<KIND, OUT, WHICH, 64, 6, true>(c);
 }
 
 }  // namespace mm

@@ -23,8 +23,6 @@ stream, reads ``offsets`` on the device only, and never synchronises.  There is
 no CPU path: CPU tensors raise RuntimeError, wrong shapes AssertionError, wrong
 types ValueError.  Feature counts are multiples of 16 (the quantizers' tile).
 """
-import contextlib
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -38,15 +36,17 @@ _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 
 
 def _need_cuda(**tensors):
-    device = None
+    """All tensors on one GPU; returns its index."""
+    device = -1
     for name, t in tensors.items():
         if t is None:
             continue
         if not (torch.is_tensor(t) and t.is_cuda):
             raise RuntimeError(f"quant_2bit_b200: `{name}` must be a CUDA tensor (the B200 kernels "
                                "have no CPU fallback)")
-        device = device or t.device
-        assert t.device == device, f"`{name}` is on {t.device}, not on {device}"
+        if device < 0:
+            device = t.get_device()
+        assert t.get_device() == device, f"`{name}` is on {t.device}, not on cuda:{device}"
     return device
 
 
@@ -59,14 +59,16 @@ def _need_features(n, name):
     assert n >= _TILE and n % _TILE == 0, f"{name} must be a multiple of {_TILE}, got {n}"
 
 
-def _on(device):
-    if torch.cuda.current_device() == device.index:
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
-
-
-def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+def _call(fn, device, *args):
+    """One C call on `device`'s current stream (appended to the arguments)."""
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if torch._C._cuda_getDevice() == device:
+        st = fn(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            st = fn(*args, stream)
+    if st:
+        _lib.check(st, fn.__name__)
 
 
 def _blocks(n):
@@ -100,10 +102,6 @@ def _need_offsets(offsets, groups):
     return offsets, offsets.data_ptr(), offsets.element_size()
 
 
-def _status(device):
-    return torch.empty(1, dtype=torch.int32, device=device)
-
-
 # --------------------------------------------------------------------------
 # bf16 / fp16, grouped by expert
 
@@ -111,32 +109,26 @@ def _status(device):
 def _grouped_mm(rows, weight, offsets, transpose):
     """rows times weight[e]^T, or times weight[e] when ``transpose``."""
     E, N, K = weight.shape
-    T, dev = rows.shape[0], rows.device
-    out = torch.empty((T, K if transpose else N), dtype=rows.dtype, device=dev)
+    T = rows.shape[0]
+    out = rows.new_empty((T, K if transpose else N))
     if T == 0:
         return out
     rows, ld = _rows(rows)
     weight = _dense(weight)
     offsets, off_ptr, off_size = _need_offsets(offsets, E)
-    with _on(dev):
-        st = _lib.load().bcjr_grouped_mm(rows.data_ptr(), ld, weight.data_ptr(), off_ptr, off_size,
-                                         T, E, N, K, _DTYPES[rows.dtype], int(transpose),
-                                         out.data_ptr(), _status(dev).data_ptr(), _stream(dev))
-    _lib.check(st, "bcjr_grouped_mm")
+    _call(_lib.load().bcjr_grouped_mm, rows.get_device(), rows.data_ptr(), ld, weight.data_ptr(),
+          off_ptr, off_size, T, E, N, K, _DTYPES[rows.dtype], transpose, out.data_ptr(), None)
     return out
 
 
 def _grouped_wgrad(dy, x, offsets, E):
-    (T, N), K, dev = dy.shape, x.shape[1], x.device
-    dw = torch.empty((E, N, K), dtype=x.dtype, device=dev)
+    (T, N), K = dy.shape, x.shape[1]
+    dw = x.new_empty((E, N, K))
     dy, ld_dy = _rows(dy)
     x, ld_x = _rows(x)
     offsets, off_ptr, off_size = _need_offsets(offsets, E)
-    with _on(dev):
-        st = _lib.load().bcjr_grouped_wgrad(dy.data_ptr(), ld_dy, x.data_ptr(), ld_x, off_ptr,
-                                            off_size, T, E, N, K, _DTYPES[x.dtype], dw.data_ptr(),
-                                            _status(dev).data_ptr(), _stream(dev))
-    _lib.check(st, "bcjr_grouped_wgrad")
+    _call(_lib.load().bcjr_grouped_wgrad, x.get_device(), dy.data_ptr(), ld_dy, x.data_ptr(), ld_x,
+          off_ptr, off_size, T, E, N, K, _DTYPES[x.dtype], dw.data_ptr(), None)
     return dw
 
 
@@ -180,21 +172,13 @@ def grouped_linear(x, weight, offsets):
     _need_features(weight.shape[1], "out features")
     _need_features(weight.shape[2], "in features")
     _need_offsets(offsets, weight.shape[0])
-    return _GroupedLinear.apply(x, weight, offsets)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        return _GroupedLinear.apply(x, weight, offsets)
+    return _grouped_mm(x, weight, offsets, False)
 
 
 # --------------------------------------------------------------------------
 # e4m3 with block scales
-
-
-def _quantize_rows_into(x, q_ptr, scale_ptr, scale_row, scale_block):
-    x, ld = _rows(x)
-    dev = x.device
-    with _on(dev):
-        st = _lib.load().bcjr_fp8_quantize_rows(x.data_ptr(), ld, x.shape[0], x.shape[1],
-                                                _DTYPES[x.dtype], q_ptr, scale_ptr, scale_row,
-                                                scale_block, _stream(dev))
-    _lib.check(st, "bcjr_fp8_quantize_rows")
 
 
 def fp8_quantize_rows(x):
@@ -206,10 +190,13 @@ def fp8_quantize_rows(x):
     assert x.dim() >= 1, "x must have at least one axis"
     K = x.shape[-1]
     _need_features(K, "the last axis")
-    q = torch.empty(x.shape, dtype=_F8, device=x.device)
-    scale = torch.empty((*x.shape[:-1], _blocks(K)), dtype=torch.float32, device=x.device)
+    blocks = _blocks(K)
+    q = x.new_empty(x.shape, dtype=_F8)
+    scale = x.new_empty((*x.shape[:-1], blocks), dtype=torch.float32)
     if x.numel():
-        _quantize_rows_into(x.detach().reshape(-1, K), q.data_ptr(), scale.data_ptr(), _blocks(K), 1)
+        rows, ld = _rows(x if x.dim() == 2 else x.detach().reshape(-1, K))
+        _call(_lib.load().bcjr_fp8_quantize_rows, x.get_device(), rows.data_ptr(), ld,
+              rows.shape[0], K, _DTYPES[x.dtype], q.data_ptr(), scale.data_ptr(), blocks, 1)
     return q, scale
 
 
@@ -224,14 +211,11 @@ def fp8_quantize_weight(weight):
     E = weight.shape[0] if weight.dim() == 3 else 1
     assert N >= 1, "weight must have rows"
     _need_features(K, "in features")
-    dev = weight.device
-    w = _dense(weight.detach())
-    q = torch.empty(weight.shape, dtype=_F8, device=dev)
-    scale = torch.empty((*weight.shape[:-2], _blocks(N), _blocks(K)), dtype=torch.float32, device=dev)
-    with _on(dev):
-        st = _lib.load().bcjr_fp8_quantize_blocks(w.data_ptr(), E, N, K, _DTYPES[w.dtype],
-                                                  q.data_ptr(), scale.data_ptr(), _stream(dev))
-    _lib.check(st, "bcjr_fp8_quantize_blocks")
+    w = _dense(weight)
+    q = weight.new_empty(weight.shape, dtype=_F8)
+    scale = weight.new_empty((*weight.shape[:-2], _blocks(N), _blocks(K)), dtype=torch.float32)
+    _call(_lib.load().bcjr_fp8_quantize_blocks, weight.get_device(), w.data_ptr(), E, N, K,
+          _DTYPES[w.dtype], q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
@@ -250,22 +234,6 @@ def _need_fp8_weight(q, scale, offsets):
     assert not scale.requires_grad, "the scales of an e4m3 weight have no gradient"
     _need_offsets(offsets, E)
     return E, N, K
-
-
-def _fp8_mm(rows_ptr, ld, scale_ptr, scale_row, scale_block, q, scale, offsets, T, transpose, dtype):
-    N, K = q.shape[-2:]
-    E = q.shape[0] if q.dim() == 3 else 1
-    dev = q.device
-    q, scale = _dense(q), scale.contiguous()
-    out = torch.empty((T, K if transpose else N), dtype=dtype, device=dev)
-    offsets, off_ptr, off_size = _need_offsets(offsets, E)
-    with _on(dev):
-        st = _lib.load().bcjr_fp8_mm(rows_ptr, ld, scale_ptr, scale_row, scale_block, q.data_ptr(),
-                                     scale.data_ptr(), off_ptr, off_size, T, E, N, K,
-                                     int(transpose), out.data_ptr(), _DTYPES[dtype],
-                                     _status(dev).data_ptr(), _stream(dev))
-    _lib.check(st, "bcjr_fp8_mm")
-    return out
 
 
 def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
@@ -291,25 +259,35 @@ def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
     if T == 0:
         return torch.empty((0, N), dtype=out_dtype, device=xq.device)
     xq, ld = _rows(xq)
-    if min(x_scale.stride()) < 0 or x_scale.stride(0) == 0 and T > 1:
+    if min(x_scale.stride()) < 0:
         x_scale = x_scale.contiguous()
-    return _fp8_mm(xq.data_ptr(), ld, x_scale.data_ptr(), x_scale.stride(0), x_scale.stride(1),
-                   q, scale, offsets, T, False, out_dtype)
+    q, scale = _dense(q), scale.contiguous()
+    out = xq.new_empty((T, N), dtype=out_dtype)
+    offsets, off_ptr, off_size = _need_offsets(offsets, E)
+    _call(_lib.load().bcjr_fp8_mm, xq.get_device(), xq.data_ptr(), ld, x_scale.data_ptr(),
+          x_scale.stride(0), x_scale.stride(1), q.data_ptr(), scale.data_ptr(), off_ptr, off_size,
+          T, E, N, K, False, out.data_ptr(), _DTYPES[out_dtype], None)
+    return out
 
 
 def _quantized_product(x, q, scale, offsets, transpose):
-    """x's rows, quantized, times the e4m3 weight (or its transpose).  The row
-    scales lie block by block, so that a tile reads those of its rows side by
-    side."""
+    """x's rows, quantized, times the e4m3 weight (or its transpose)."""
     T, C = x.shape
+    N, K = q.shape[-2:]
+    E = q.shape[0] if q.dim() == 3 else 1
+    out = x.new_empty((T, K if transpose else N))
     if T == 0:
-        return torch.empty((0, q.shape[-1] if transpose else q.shape[-2]), dtype=x.dtype,
-                           device=x.device)
-    body = -(-T * C // 16) * 16
-    ws = torch.empty(body + 4 * T * _blocks(C), dtype=torch.uint8, device=x.device)
-    rows, scales = ws.data_ptr(), ws.data_ptr() + body
-    _quantize_rows_into(x, rows, scales, 1, T)
-    return _fp8_mm(rows, C, scales, 1, T, q, scale, offsets, T, transpose, x.dtype)
+        return out
+    lib = _lib.load()
+    size = lib.bcjr_fp8_linear_workspace_bytes(T, C)
+    ws = x.new_empty(size, dtype=torch.uint8)
+    x, ld = _rows(x)
+    q, scale = _dense(q), scale.contiguous()
+    offsets, off_ptr, off_size = _need_offsets(offsets, E)
+    _call(lib.bcjr_fp8_linear, x.get_device(), x.data_ptr(), ld, _DTYPES[x.dtype], q.data_ptr(),
+          scale.data_ptr(), off_ptr, off_size, T, E, N, K, transpose, out.data_ptr(),
+          ws.data_ptr(), size, None)
+    return out
 
 
 class _Fp8Linear(torch.autograd.Function):
@@ -342,9 +320,12 @@ def fp8_linear(x, q, scale, offsets=None):
     E, N, K = _need_fp8_weight(q, scale, offsets)
     assert x.dim() >= 1 and x.shape[-1] == K, f"x must be (..., {K}), got {tuple(x.shape)}"
     assert offsets is None or x.dim() == 2, f"x must be (T, K) with offsets, got {tuple(x.shape)}"
-    if x.dim() == 2:
-        return _Fp8Linear.apply(x, q, scale, offsets)
-    return _Fp8Linear.apply(x.reshape(-1, K), q, scale, offsets).view(*x.shape[:-1], N)
+    rows = x if x.dim() == 2 else x.reshape(-1, K)
+    if torch.is_grad_enabled() and x.requires_grad:
+        y = _Fp8Linear.apply(rows, q, scale, offsets)
+    else:
+        y = _quantized_product(rows, q, scale, offsets, False)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 
 __all__ = ["grouped_linear", "fp8_quantize_rows", "fp8_quantize_weight", "fp8_matmul", "fp8_linear"]

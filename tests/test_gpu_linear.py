@@ -93,6 +93,10 @@ GROUPS = [
     ([255, 256, 257, 0, 1], 256, 272),
     ([0, 0, 300, 0, 513, 2], 400, 48),
     ([0, 0, 0], 64, 64),
+    ([3, 0, 5], 144, 1040),                        # few tiles, long contraction: clusters share
+    ([1], 1040, 2064),                             # tiles (forward and rows' gradient)
+    ([33], 16, 8208),
+    ([0, 64, 0], 528, 512),
     ([3, 1, 4, 1, 5, 9, 2, 6, 5, 3, 5, 8, 9, 7, 9, 3] * 5, 32, 96),   # 80 groups
 ]
 
@@ -436,14 +440,16 @@ def _check_fp8(x, q, s, w64, dy, offsets):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,N,K", [(1, 16, 16), (1, 128, 256), (17, 144, 272), (64, 2000, 400),
-                                   (65, 48, 128), (300, 272, 1040), (513, 128, 144)])
+                                   (65, 48, 128), (300, 272, 1040), (513, 128, 144), (37, 48, 4240), (1, 2064, 528),
+                                   (64, 144, 1280)])
 def test_fp8_linear_forward_and_gradient(cuda_ok, T, N, K, dtype):
     x, q, s, w64, dy = _fp8_operands(T, 0, N, K, dtype, seed=T)
     _check_fp8(x, q, s, w64, dy, None)
 
 
 @pytest.mark.parametrize("counts,N,K", [([3, 0, 1, 12], 144, 272), ([130, 0, 300, 70], 272, 144),
-                                        ([0, 0], 128, 128), ([257, 1], 128, 384)])
+                                        ([0, 0], 128, 128), ([257, 1], 128, 384),
+                                        ([9, 0, 1], 144, 2064)])
 def test_fp8_linear_by_expert(cuda_ok, counts, N, K):
     T = sum(counts) + 6
     x, q, s, w64, dy = _fp8_operands(T, len(counts), N, K, torch.bfloat16, seed=T)

@@ -40,7 +40,6 @@ def test_products_refuse_bad_sizes(lib, call):
         assert call(lib, **bad) == SHAPE, bad
     assert call(lib, dtype=2) == UNSUPPORTED
     assert call(lib, dtype=-1) == UNSUPPORTED
-    assert call(lib, status=None) == NULL
 
 
 def test_products_refuse_bad_pointers_and_strides(lib):
@@ -62,6 +61,20 @@ def test_products_refuse_bad_pointers_and_strides(lib):
     assert _fp8(lib, ld=72) == ALIGN
     assert _fp8(lib, s_row=-1) == SHAPE
     assert _fp8(lib, xs=P + 2) == ALIGN
+
+
+def test_fp8_linear_refuses(lib):
+    def call(x=P, ld=64, dtype=0, w=P, s=P, T=8, N=32, K=64, tr=0, out=P, ws=P, size=1 << 20):
+        return lib.bcjr_fp8_linear(x, ld, dtype, w, s, P, 4, T, 2, N, K, tr, out, ws, size, None, None)
+
+    need = lib.bcjr_fp8_linear_workspace_bytes(8, 64)
+    assert need >= 8 * 64 + 8 * 4 and lib.bcjr_fp8_linear_workspace_bytes(8, 40) == 0
+    assert call(size=need - 1) == call(ws=None) == 5
+    assert call(dtype=2) == UNSUPPORTED
+    assert call(K=40) == call(T=-1) == call(ld=32) == SHAPE
+    assert call(x=P + 8) == call(ws=P + 8) == ALIGN
+    assert call(x=None) == NULL
+    assert call(T=0, x=None, ws=None) == OK
 
 
 def test_quantizers_refuse(lib):
