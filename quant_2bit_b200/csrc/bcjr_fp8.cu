@@ -86,6 +86,7 @@ template <typename T>
 __global__ void __launch_bounds__(kQThreads)
 quantize_rows(const T *__restrict__ x, long ld, long rows, int k, uint8_t *__restrict__ q,
               float *__restrict__ scale, long s_row, long s_blk) {
+    let_next_start();              // the product's set-up may overlap (it waits for this kernel's end)
     const int nb = (k + 127) / 128, sub = threadIdx.x & 15;
     const long segs = rows * nb, groups = kQThreads / 16;
     const long first = (blockIdx.x * groups * kUnroll) + (threadIdx.x >> 4);
@@ -222,10 +223,10 @@ int bcjr_fp8_quantize_blocks(const void *w, int E, int N, int K, int dtype, void
     }
 }
 
-int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long scale_row,
-                long scale_block, const void *w, const float *w_scale, const void *offsets,
-                int offsets_bytes, long T, int E, int N, int K, int transpose_w, void *out,
-                int out_dtype, int *status, bcjr_stream_t stream) {
+static int fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long scale_row,
+                  long scale_block, const void *w, const float *w_scale, const void *offsets,
+                  int offsets_bytes, long T, int E, int N, int K, int transpose_w, void *out,
+                  int out_dtype, int *status, bcjr_stream_t stream, int dependent) {
     if (T < 0 || T > 0x7fffff00L || E < 1 || E > kMaxGroups || N < 16 || K < 16 || N % 16 || K % 16 ||
         N > (1 << 24) || K > (1 << 24))
         return BCJR_ERR_BAD_SHAPE;
@@ -266,7 +267,16 @@ int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long sc
     c.p.ws_blk = transpose_w ? kb : 1;
     c.p.status = status;
     c.p.drop = bcjr::test_option(bcjr::kOptDropSends);
+    c.p.dependent = dependent;
     return status_of(out_dtype == BCJR_BF16 ? run_mm<__nv_bfloat16>(c) : run_mm<__half>(c));
+}
+
+int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long scale_row,
+                long scale_block, const void *w, const float *w_scale, const void *offsets,
+                int offsets_bytes, long T, int E, int N, int K, int transpose_w, void *out,
+                int out_dtype, int *status, bcjr_stream_t stream) {
+    return fp8_mm(rows, ld_rows, rows_scale, scale_row, scale_block, w, w_scale, offsets, offsets_bytes, T, E,
+                  N, K, transpose_w, out, out_dtype, status, stream, 0);
 }
 
 // The quantized rows first, then their scales, block by block, so that a tile
@@ -276,6 +286,9 @@ size_t bcjr_fp8_linear_workspace_bytes(long T, int depth) {
     return size_t(T) * depth + size_t(T) * ((depth + 127) / 128) * 4 + 16;
 }
 
+// The product is launched to overlap the end of the quantizer: its set-up and
+// its first weight loads run before it waits for the quantized rows.  The
+// quantizer itself is an ordinary launch, so everything before it has ended.
 int bcjr_fp8_linear(const void *x, long ld, int dtype, const void *w, const float *w_scale,
                     const void *offsets, int offsets_bytes, long T, int E, int N, int K,
                     int transpose_w, void *out, void *ws, size_t ws_bytes, int *status,
@@ -289,8 +302,8 @@ int bcjr_fp8_linear(const void *x, long ld, int dtype, const void *w, const floa
     float *scale = reinterpret_cast<float *>(static_cast<char *>(ws) + size_t(T) * depth);
     const int st = bcjr_fp8_quantize_rows(x, ld, T, depth, dtype, ws, scale, 1, T, stream);
     if (st) return st;
-    return bcjr_fp8_mm(ws, depth, scale, 1, T, w, w_scale, offsets, offsets_bytes, T, E, N, K,
-                       transpose_w, out, dtype, status, stream);
+    return fp8_mm(ws, depth, scale, 1, T, w, w_scale, offsets, offsets_bytes, T, E, N, K, transpose_w, out,
+                  dtype, status, stream, 1);
 }
 
 }  // extern "C"

@@ -45,6 +45,7 @@ constexpr int kChunk = 32;                        // columns that a half of the 
 constexpr int kPitch = kLanes * 2 + 16;           // bytes of a staged output row: 16-byte pieces of
                                                   // 8 rows fall into different banks
 constexpr int kMaxGroups = 1024;
+constexpr int kMaxSplit = 8;                      // blocks of a cluster that share a tile
 constexpr int kBoxRows = 64;                      // rows of one TMA box
 constexpr long long kWaitLimitClocks = 2000000000ll;   // about 1 s
 
@@ -63,6 +64,7 @@ struct Params {
     long ws_group, ws_lane, ws_blk;
     int *status;
     int drop;                 // test option: the first load of block 0 is withheld
+    int dependent;            // launched to overlap the kernel that writes the row matrix
 };
 
 // ---------------------------------------------------------------------------
@@ -208,6 +210,17 @@ __device__ __forceinline__ void st_transposed(uint32_t addr, uint32_t a, uint32_
                  ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
 }
+// Programmatic dependent launch: the next kernel of the stream may start; the
+// one before has ended and its writes are visible.
+__device__ __forceinline__ void let_next_start() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+__device__ __forceinline__ void wait_for_previous() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void prefetch_map(const CUtensorMap *m) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
+}
 // 4 bytes global -> shared, or zero.
 __device__ __forceinline__ void copy4(uint32_t dst, const float *src, bool real) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
@@ -244,7 +257,7 @@ __device__ __forceinline__ void bar_arrive_in(uint32_t bar, uint32_t r) {
 }
 __device__ __forceinline__ float2 load2_in(uint32_t addr, uint32_t r) {
     float2 v;
-    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_rank(addr, r)) : "memory");
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(in_rank(addr, r)));
     return v;
 }
 __device__ __forceinline__ void fence_async() {
@@ -435,8 +448,12 @@ struct Smem {
     static constexpr int kB = COLS * kRowBytes;
     static constexpr int kStage = kA + kB;
     static constexpr int kScales = KIND == kE4M3 ? kScaleStages : 1;
+    // accumulator buffers.  16-bit types use one for a tile, e4m3 one for a k
+    // block: with few columns eight of them fit, and the tensor core runs ahead
+    // of the epilogue (one token, 8192 x 2048: 740 clocks a block with two).
+    static constexpr int kAcc = KIND == kE4M3 && COLS <= 64 ? 8 : 2;
     struct Ctl {
-        unsigned long long full[STAGES], empty[STAGES], tfull[2], tempty[2], done;
+        unsigned long long full[STAGES], empty[STAGES], tfull[kAcc], tempty[kAcc], done;
         unsigned long long sfull[kScaleStages], sempty[kScaleStages];
         uint32_t tmem;
         int fail;
@@ -510,12 +527,17 @@ __device__ __forceinline__ bool add_parts(const float (&v)[2][16], float (*part)
         const int c = i / per, f = (rank * per + i - c * per) * 2;
         if (f >= features) continue;
         const uint32_t at = smem_u32(&part[c][f]);
-        float2 s = load2_in(at, 0);
-        for (uint32_t r = 1; r < size; ++r) {
-            const float2 w = load2_in(at, r);
-            s.x += w.x;
-            s.y += w.y;
-        }
+        float2 w[kMaxSplit];                        // all on their way before the first is added
+#pragma unroll
+        for (uint32_t r = 0; r < kMaxSplit; ++r)
+            if (r < size) w[r] = load2_in(at, r);
+        float2 s = w[0];
+#pragma unroll
+        for (uint32_t r = 1; r < kMaxSplit; ++r)
+            if (r < size) {
+                s.x += w[r].x;
+                s.y += w[r].y;
+            }
         if (!ok) s.x = s.y = __int_as_float(0x7fffffff);
         *reinterpret_cast<uint32_t *>(out + c * ldo + f) = pack<OUT>(s.x, s.y);
     }
@@ -538,8 +560,9 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     constexpr uint32_t A_STEP = A_MN ? KSLICE * kRowBytes : 32;
     constexpr uint32_t B_STEP = B_MN ? KSLICE * kRowBytes : 32;
     constexpr uint32_t MN_BLOCK = BK * kRowBytes;     // an MN-major block of BK rows
-    constexpr uint32_t TMEM_COLS = 2 * COLS < 32 ? 32 : 2 * COLS;
     using S = Smem<KIND, COLS, STAGES, SPLIT>;
+    constexpr uint32_t ACC = S::kAcc, TMEM_COLS = ACC * COLS;
+    static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0 && TMEM_COLS >= 32, "");
     static_assert(!(KIND == kE4M3 && WHICH == kWgrad), "e4m3 has forward and dgrad");
     static_assert(BK % kBoxRows == 0 && COLS % 16 == 0, "");
 
@@ -554,7 +577,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             bar_init(smem_u32(&ctl.full[i]), 1);
             bar_init(smem_u32(&ctl.empty[i]), 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < ACC; ++i) {
             bar_init(smem_u32(&ctl.tfull[i]), 1);
             bar_init(smem_u32(&ctl.tempty[i]), kEpiWarps);
         }
@@ -567,6 +590,10 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         ctl.fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         if (blockIdx.x == 0 && p.status) *p.status = 0;   // a failure is a second away
+    }
+    if (threadIdx.x == 32) {
+        prefetch_map(&ta);
+        prefetch_map(&tb);
     }
     if (warp == kMmaWarp) tmem_alloc(smem_u32(&ctl.tmem), TMEM_COLS);
     read_groups(ctl.groups, p);
@@ -588,38 +615,53 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         if (warp == kTmaWarp) {
             // TMA producer
             if (lane == 0) {
-                uint32_t it = 0;
+                uint32_t it = 0, ahead = 0;
                 bool ok = true;
-                while (ok && walk.next(t)) {
-                    const int nkb = t.nkb;
+                // Arms the stage's barrier for both operands and loads the one
+                // that has the output's lanes.
+                auto load_a = [&](const Tile &t, int kb, uint32_t s) {
+                    const uint32_t bar = smem_u32(&ctl.full[s]), a = smem_u32(buf + s * S::kStage);
                     const int bboxes = B_MN ? (t.ncols + MNB - 1) / MNB : (t.ncols + kBoxRows - 1) / kBoxRows;
-                    const uint32_t bytes = S::kA + bboxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes);
-                    for (int kb = 0; kb < nkb; ++kb, ++it) {
-                        const uint32_t s = it % STAGES, ph = (it / STAGES) & 1;
-                        if (!bar_wait(smem_u32(&ctl.empty[s]), ph ^ 1, fail, p.status)) {
-                            ok = false;
-                            break;
+                    const int kc = t.k0 + kb * BK;
+                    bar_expect(bar, S::kA + bboxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes));
+                    if constexpr (WHICH == kForward) {
+                        tma3(a, &ta, kc, t.lane_tile * kLanes, t.group, bar);
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < kLanes / MNB; ++j) {
+                            const int x = t.lane_tile * kLanes + j * MNB;
+                            if constexpr (WHICH == kDgrad) tma3(a + j * MN_BLOCK, &ta, x, kc, t.group, bar);
+                            else tma2(a + j * MN_BLOCK, &ta, x, kc, bar);
                         }
-                        if (p.drop && blockIdx.x == 0 && it == 0) continue;
-                        const uint32_t bar = smem_u32(&ctl.full[s]);
-                        const uint32_t a = smem_u32(buf + s * S::kStage), b = a + S::kA;
-                        bar_expect(bar, bytes);
+                    }
+                };
+                const bool drop = p.drop && blockIdx.x == 0;      // test option: the first load is withheld
+                if (p.dependent) {
+                    // the weights do not come from the kernel before this one
+                    Walk<WHICH, COLS, BK, SPLIT> first = walk;
+                    if (first.next(t))
+                        for (; ahead < STAGES && ahead < t.nkb; ++ahead)
+                            if (!drop || ahead) load_a(t, ahead, ahead);
+                    wait_for_previous();
+                }
+                while (ok && walk.next(t)) {
+                    for (int kb = 0; kb < t.nkb; ++kb, ++it) {
+                        const uint32_t s = it % STAGES;
+                        if (it >= ahead) {
+                            if (!bar_wait(smem_u32(&ctl.empty[s]), ((it / STAGES) & 1) ^ 1, fail, p.status)) {
+                                ok = false;
+                                break;
+                            }
+                            if (!drop || it) load_a(t, kb, s);
+                        }
+                        if (drop && it == 0) continue;
+                        const uint32_t bar = smem_u32(&ctl.full[s]), b = smem_u32(buf + s * S::kStage) + S::kA;
                         const int kc = t.k0 + kb * BK;
-                        if constexpr (WHICH == kForward) {
-                            tma3(a, &ta, kc, t.lane_tile * kLanes, t.group, bar);
-                        } else if constexpr (WHICH == kDgrad) {
-#pragma unroll
-                            for (int j = 0; j < kLanes / MNB; ++j)
-                                tma3(a + j * MN_BLOCK, &ta, t.lane_tile * kLanes + j * MNB, kc, t.group, bar);
-                        } else {
-#pragma unroll
-                            for (int j = 0; j < kLanes / MNB; ++j)
-                                tma2(a + j * MN_BLOCK, &ta, t.lane_tile * kLanes + j * MNB, kc, bar);
-                        }
-                        for (int j = 0; j < bboxes; ++j) {
-                            if constexpr (B_MN)
+                        if constexpr (B_MN) {
+                            for (int j = 0; j * MNB < t.ncols; ++j)
                                 tma2(b + j * MN_BLOCK, &tb, t.col0 + j * MNB, kc, bar);
-                            else
+                        } else {
+                            for (int j = 0; j * kBoxRows < t.ncols; ++j)
                                 tma2(b + j * kBoxRows * kRowBytes, &tb, kc, t.col0 + j * kBoxRows, bar);
                         }
                     }
@@ -628,7 +670,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                     // copies in flight land before the block ends
                     volatile int never = 0;
                     for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-                        if (!(p.drop && blockIdx.x == 0 && i == 0))
+                        if (!(drop && i == 0))
                             bar_wait(smem_u32(&ctl.full[i % STAGES]), (i / STAGES) & 1, &never, nullptr);
                 }
             }
@@ -644,7 +686,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                     // e4m3: every stage has an accumulator buffer of its own
                     // (scaled and added in fp32 registers); otherwise every tile
                     if (KIND == kE4M3 || kb == 0) {
-                        if (!warp_wait(smem_u32(&ctl.tempty[acc & 1]), ((acc >> 1) & 1) ^ 1, fail, p.status)) {
+                        if (!warp_wait(smem_u32(&ctl.tempty[acc % ACC]), ((acc / ACC) & 1) ^ 1, fail, p.status)) {
                             ok = false;
                             break;
                         }
@@ -675,13 +717,13 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                     if (lane == 0) {
                         const uint64_t da = operand_desc(smem_u32(a), MN_BLOCK);
                         const uint64_t db = operand_desc(smem_u32(b), MN_BLOCK);
-                        const uint32_t d = tmem + (acc & 1) * COLS;
+                        const uint32_t d = tmem + (acc % ACC) * COLS;
 #pragma unroll
                         for (int j = 0; j < SLICES; ++j)
                             mma<KIND>(d, da + ((j * A_STEP) >> 4), db + ((j * B_STEP) >> 4), idesc,
                                       (KIND == kE4M3 ? j > 0 : (kb | j) > 0) ? 1u : 0u);
                         mma_commit(smem_u32(&ctl.empty[s]));
-                        if (KIND == kE4M3 || kb == nkb - 1) mma_commit(smem_u32(&ctl.tfull[acc & 1]));
+                        if (KIND == kE4M3 || kb == nkb - 1) mma_commit(smem_u32(&ctl.tfull[acc % ACC]));
                     }
                     __syncwarp();
                     if (KIND == kE4M3 || kb == nkb - 1) ++acc;
@@ -699,6 +741,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             // block, fetching scales took three times as long as the products.
             constexpr int N = COLS / (2 * 32);
             const int odd = warp - kScaleWarp;
+            if (p.dependent) wait_for_previous();
             uint32_t it = 0;
             bool ok = true;
             while (ok && walk.next(t)) {
@@ -757,11 +800,11 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 for (int kb = 0; kb < nkb; ++kb, ++acc) {
                     const uint32_t s = acc % kScaleStages;
                     if (ok) ok = warp_wait(smem_u32(&ctl.sfull[s]), (acc / kScaleStages) & 1, fail, p.status);
-                    if (ok) ok = warp_wait(smem_u32(&ctl.tfull[acc & 1]), (acc >> 1) & 1, fail, p.status);
+                    if (ok) ok = warp_wait(smem_u32(&ctl.tfull[acc % ACC]), (acc / ACC) & 1, fail, p.status);
                     if (!ok) continue;
                     tc_fence_after();
                     const float ws = ctl.ws[s];
-                    const uint32_t at = tmem + lanes_at + (acc & 1) * COLS;
+                    const uint32_t at = tmem + lanes_at + (acc % ACC) * COLS;
                     // the next chunk's load runs under this chunk's sums
                     float v[2][2][16];
                     if (half * kChunk < t.ncols) {
@@ -796,7 +839,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
-                        bar_arrive(smem_u32(&ctl.tempty[acc & 1]));
+                        bar_arrive(smem_u32(&ctl.tempty[acc % ACC]));
                         bar_arrive(smem_u32(&ctl.sempty[s]));
                     }
                 }
@@ -814,9 +857,9 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 if constexpr (SPLIT)
                     ok = add_parts<OUT>(sum[0], ctl.part, smem_u32(&ctl.pfull), half, quad, lane, out, p.ldo, t.valid, features, ok, fail, p.status);
             } else {
-                if (nkb && ok) ok = warp_wait(smem_u32(&ctl.tfull[acc & 1]), (acc >> 1) & 1, fail, p.status);
+                if (nkb && ok) ok = warp_wait(smem_u32(&ctl.tfull[acc % ACC]), (acc / ACC) & 1, fail, p.status);
                 tc_fence_after();
-                const uint32_t at = tmem + lanes_at + (acc & 1) * COLS;
+                const uint32_t at = tmem + lanes_at + (acc % ACC) * COLS;
                 float v[2][16];
                 for (int c0 = half * kChunk; c0 < (SPLIT ? COLS : t.valid); c0 += 2 * kChunk) {
                     if (nkb && ok) {
@@ -833,7 +876,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 if (nkb) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(smem_u32(&ctl.tempty[acc & 1]));
+                    if (lane == 0) bar_arrive(smem_u32(&ctl.tempty[acc % ACC]));
                     ++acc;
                 }
                 if constexpr (SPLIT)
@@ -880,7 +923,7 @@ struct Call {
     cudaStream_t stream;
     Params p;
 };
-constexpr int kMaxSplit = 8;
+
 
 // Both operand maps of a call.
 template <int KIND, int WHICH>
@@ -929,23 +972,26 @@ cudaError_t launch(const Call &c) {
     const long col_tiles = WHICH == kWgrad ? long(c.p.E) * ((c.p.cols + COLS - 1) / COLS)
                                            : c.p.T / COLS + (c.p.E < c.p.T ? c.p.E : c.p.T);
     const long tiles = lane_tiles * (col_tiles > 0 ? col_tiles : 1);
-    if constexpr (SPLIT) {
-        if (tiles * c.split > 0x7fffffffL) return cudaErrorInvalidValue;
-        cudaLaunchAttribute a;
-        a.id = cudaLaunchAttributeClusterDimension;
-        a.val.clusterDim.x = unsigned(c.split);
-        a.val.clusterDim.y = a.val.clusterDim.z = 1;
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3(unsigned(tiles * c.split));
-        cfg.blockDim = dim3(kThreads);
-        cfg.dynamicSmemBytes = bytes;
-        cfg.stream = c.stream;
-        cfg.attrs = &a;
-        cfg.numAttrs = 1;
-        return cudaLaunchKernelEx(&cfg, k, ta, tb, c.p);
+    const long blocks = SPLIT ? tiles * c.split : tiles < sms ? tiles : sms;
+    if (blocks > 0x7fffffffL) return cudaErrorInvalidValue;
+    cudaLaunchAttribute a[2];
+    cudaLaunchConfig_t cfg = {};
+    if (c.p.dependent) {
+        a[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        a[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
-    k<<<unsigned(tiles < sms ? tiles : sms), kThreads, bytes, c.stream>>>(ta, tb, c.p);
-    return cudaGetLastError();
+    if (SPLIT) {
+        a[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+        a[cfg.numAttrs].val.clusterDim.x = unsigned(c.split);
+        a[cfg.numAttrs].val.clusterDim.y = a[cfg.numAttrs].val.clusterDim.z = 1;
+        ++cfg.numAttrs;
+    }
+    cfg.gridDim = dim3(unsigned(blocks));
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = c.stream;
+    cfg.attrs = a;
+    return cudaLaunchKernelEx(&cfg, k, ta, tb, c.p);
 }
 
 // Forward and dgrad.  Up to 64 rows every group is one tile of at most 64

@@ -71,6 +71,14 @@ def _call(fn, device, *args):
         _lib.check(st, fn.__name__)
 
 
+def _differentiate(backward, ctx, dy):
+    """A backward without a second derivative (asking for one raises); the
+    bookkeeping for that is left out when no graph of the backward is made."""
+    if torch.is_grad_enabled():
+        backward = once_differentiable(backward)
+    return backward(ctx, dy)
+
+
 def _blocks(n):
     return -(-n // _BLOCK)
 
@@ -93,13 +101,18 @@ def _dense(t):
 
 
 def _need_offsets(offsets, groups):
+    """Checked and contiguous."""
     if offsets is None:
-        return None, 0, 0
+        return None
     _need_dtype(offsets, "offsets", (torch.int32, torch.int64))
     assert offsets.dim() == 1 and offsets.shape[0] == groups + 1, \
         f"offsets must have one more element than there are experts ({groups}), got {tuple(offsets.shape)}"
-    offsets = offsets.contiguous()
-    return offsets, offsets.data_ptr(), offsets.element_size()
+    return offsets.contiguous()
+
+
+def _bounds(offsets):
+    """(pointer, bytes of an element)"""
+    return (0, 0) if offsets is None else (offsets.data_ptr(), offsets.element_size())
 
 
 # --------------------------------------------------------------------------
@@ -115,7 +128,7 @@ def _grouped_mm(rows, weight, offsets, transpose):
         return out
     rows, ld = _rows(rows)
     weight = _dense(weight)
-    offsets, off_ptr, off_size = _need_offsets(offsets, E)
+    off_ptr, off_size = _bounds(offsets)
     _call(_lib.load().bcjr_grouped_mm, rows.get_device(), rows.data_ptr(), ld, weight.data_ptr(),
           off_ptr, off_size, T, E, N, K, _DTYPES[rows.dtype], transpose, out.data_ptr(), None)
     return out
@@ -126,10 +139,20 @@ def _grouped_wgrad(dy, x, offsets, E):
     dw = x.new_empty((E, N, K))
     dy, ld_dy = _rows(dy)
     x, ld_x = _rows(x)
-    offsets, off_ptr, off_size = _need_offsets(offsets, E)
+    off_ptr, off_size = _bounds(offsets)
     _call(_lib.load().bcjr_grouped_wgrad, x.get_device(), dy.data_ptr(), ld_dy, x.data_ptr(), ld_x,
           off_ptr, off_size, T, E, N, K, _DTYPES[x.dtype], dw.data_ptr(), None)
     return dw
+
+
+def _grouped_backward(ctx, dy):
+    x, weight, offsets = ctx.saved_tensors
+    dx = dw = None
+    if ctx.needs_input_grad[0]:
+        dx = _grouped_mm(dy, weight, offsets, True)
+    if ctx.needs_input_grad[1]:
+        dw = _grouped_wgrad(dy, x, offsets, weight.shape[0])
+    return dx, dw, None
 
 
 class _GroupedLinear(torch.autograd.Function):
@@ -139,15 +162,8 @@ class _GroupedLinear(torch.autograd.Function):
         return _grouped_mm(x, weight, offsets, False)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x, weight, offsets = ctx.saved_tensors
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            dx = _grouped_mm(dy, weight, offsets, True)
-        if ctx.needs_input_grad[1]:
-            dw = _grouped_wgrad(dy, x, offsets, weight.shape[0])
-        return dx, dw, None
+        return _differentiate(_grouped_backward, ctx, dy)
 
 
 def grouped_linear(x, weight, offsets):
@@ -171,7 +187,7 @@ def grouped_linear(x, weight, offsets):
     assert 1 <= weight.shape[0] <= _MAX_GROUPS, f"1 to {_MAX_GROUPS} experts, got {weight.shape[0]}"
     _need_features(weight.shape[1], "out features")
     _need_features(weight.shape[2], "in features")
-    _need_offsets(offsets, weight.shape[0])
+    offsets = _need_offsets(offsets, weight.shape[0])
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _GroupedLinear.apply(x, weight, offsets)
     return _grouped_mm(x, weight, offsets, False)
@@ -232,8 +248,7 @@ def _need_fp8_weight(q, scale, offsets):
     assert scale.shape == (*q.shape[:-2], _blocks(N), _blocks(K)), \
         f"scale must be {(*q.shape[:-2], _blocks(N), _blocks(K))}, got {tuple(scale.shape)}"
     assert not scale.requires_grad, "the scales of an e4m3 weight have no gradient"
-    _need_offsets(offsets, E)
-    return E, N, K
+    return E, N, K, _need_offsets(offsets, E)
 
 
 def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
@@ -251,7 +266,7 @@ def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
     _need_dtype(x_scale, "x_scale", (torch.float32,))
     if out_dtype not in (torch.bfloat16, torch.float16):
         raise ValueError(f"out_dtype must be torch.bfloat16 or torch.float16, got {out_dtype}")
-    E, N, K = _need_fp8_weight(q, scale, offsets)
+    E, N, K, offsets = _need_fp8_weight(q, scale, offsets)
     assert xq.dim() == 2 and xq.shape[1] == K, f"xq must be (T, {K}), got {tuple(xq.shape)}"
     assert x_scale.shape == (xq.shape[0], _blocks(K)), \
         f"x_scale must be {(xq.shape[0], _blocks(K))}, got {tuple(x_scale.shape)}"
@@ -263,7 +278,7 @@ def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
         x_scale = x_scale.contiguous()
     q, scale = _dense(q), scale.contiguous()
     out = xq.new_empty((T, N), dtype=out_dtype)
-    offsets, off_ptr, off_size = _need_offsets(offsets, E)
+    off_ptr, off_size = _bounds(offsets)
     _call(_lib.load().bcjr_fp8_mm, xq.get_device(), xq.data_ptr(), ld, x_scale.data_ptr(),
           x_scale.stride(0), x_scale.stride(1), q.data_ptr(), scale.data_ptr(), off_ptr, off_size,
           T, E, N, K, False, out.data_ptr(), _DTYPES[out_dtype], None)
@@ -283,11 +298,17 @@ def _quantized_product(x, q, scale, offsets, transpose):
     ws = x.new_empty(size, dtype=torch.uint8)
     x, ld = _rows(x)
     q, scale = _dense(q), scale.contiguous()
-    offsets, off_ptr, off_size = _need_offsets(offsets, E)
+    off_ptr, off_size = _bounds(offsets)
     _call(lib.bcjr_fp8_linear, x.get_device(), x.data_ptr(), ld, _DTYPES[x.dtype], q.data_ptr(),
           scale.data_ptr(), off_ptr, off_size, T, E, N, K, transpose, out.data_ptr(),
           ws.data_ptr(), size, None)
     return out
+
+
+def _fp8_backward(ctx, dy):
+    q, scale, offsets = ctx.saved_tensors
+    dx = _quantized_product(dy, q, scale, offsets, True) if ctx.needs_input_grad[0] else None
+    return dx, None, None, None
 
 
 class _Fp8Linear(torch.autograd.Function):
@@ -297,11 +318,8 @@ class _Fp8Linear(torch.autograd.Function):
         return _quantized_product(x, q, scale, offsets, False)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        q, scale, offsets = ctx.saved_tensors
-        dx = _quantized_product(dy, q, scale, offsets, True) if ctx.needs_input_grad[0] else None
-        return dx, None, None, None
+        return _differentiate(_fp8_backward, ctx, dy)
 
 
 def fp8_linear(x, q, scale, offsets=None):
@@ -317,7 +335,7 @@ def fp8_linear(x, q, scale, offsets=None):
     is constant."""
     _need_cuda(x=x, q=q, scale=scale, offsets=offsets)
     _need_dtype(x, "x", (torch.bfloat16, torch.float16))
-    E, N, K = _need_fp8_weight(q, scale, offsets)
+    E, N, K, offsets = _need_fp8_weight(q, scale, offsets)
     assert x.dim() >= 1 and x.shape[-1] == K, f"x must be (..., {K}), got {tuple(x.shape)}"
     assert offsets is None or x.dim() == 2, f"x must be (T, K) with offsets, got {tuple(x.shape)}"
     rows = x if x.dim() == 2 else x.reshape(-1, K)
