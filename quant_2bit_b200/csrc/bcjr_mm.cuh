@@ -45,7 +45,7 @@ constexpr int kChunk = 32;                        // columns that a half of the 
 constexpr int kPitch = kLanes * 2 + 16;           // bytes of a staged output row: 16-byte pieces of
                                                   // 8 rows fall into different banks
 constexpr int kMaxGroups = 1024;
-constexpr int kMaxSplit = 8;                      // blocks of a cluster that share a tile
+constexpr int kMaxSplit = 4;                      // blocks of a cluster that share a tile
 constexpr int kBoxRows = 64;                      // rows of one TMA box
 constexpr long long kWaitLimitClocks = 2000000000ll;   // about 1 s
 
@@ -72,6 +72,15 @@ struct Params {
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+// True for one lane of a converged warp.  (Tensor-core and TMA instructions
+// take their operands from uniform registers; under a branch that this
+// instruction made the compiler knows that one lane runs them, under
+// `lane == 0` it does not, and four matrix instructions took 770 clocks.)
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(one));
+    return one != 0;
 }
 __device__ __forceinline__ void bar_init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
@@ -614,7 +623,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         if constexpr (kSplitsRegs<KIND, COLS>) regs_down<kFewRegs>();
         if (warp == kTmaWarp) {
             // TMA producer
-            if (lane == 0) {
+            if (elect_one()) {
                 uint32_t it = 0, ahead = 0;
                 bool ok = true;
                 // Arms the stage's barrier for both operands and loads the one
@@ -714,7 +723,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                         }
                     }
                     tc_fence_after();
-                    if (lane == 0) {
+                    if (elect_one()) {
                         const uint64_t da = operand_desc(smem_u32(a), MN_BLOCK);
                         const uint64_t db = operand_desc(smem_u32(b), MN_BLOCK);
                         const uint32_t d = tmem + (acc % ACC) * COLS;
@@ -730,7 +739,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 }
             }
             // every matrix instruction has ended before the block frees its TMEM
-            if (lane == 0) mma_commit(smem_u32(&ctl.done));
+            if (elect_one()) mma_commit(smem_u32(&ctl.done));
             volatile int never = 0;
             bar_wait(smem_u32(&ctl.done), 0, &never, nullptr);
         } else if constexpr (KIND == kE4M3) {
