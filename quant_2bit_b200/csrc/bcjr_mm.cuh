@@ -95,6 +95,17 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar) {
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
+        "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;"
+        " selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// The same for a barrier that other blocks of the cluster arrive on.
+__device__ __forceinline__ bool bar_try_cluster(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
         "{ .reg .pred p; mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;"
         " selp.u32 %0, 1, 0, p; }"
         : "=r"(ok)
@@ -105,13 +116,15 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
 // Bounded wait (about 1 s).  False when it gave up or another warp of the
 // block did; the block then finishes with NaN outputs and the status word
 // says BCJR_ERR_TIMEOUT.
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *fail,
                                          int *status) {
-    if (bar_try(bar, parity)) return true;
+    auto test = [&] { return CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity); };
+    if (test()) return true;
     const long long t0 = clock64();
     while (true) {
         for (int i = 0; i < 32; ++i)
-            if (bar_try(bar, parity)) return true;
+            if (test()) return true;
         if (*fail) return false;
         if (clock64() - t0 > kWaitLimitClocks) {
             *fail = 1;
@@ -123,9 +136,10 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 // The same for a whole warp: every lane gets the same answer.  (All lanes
 // test the barrier; one lane that tests and hands its answer around measured
 // 5 % slower.)
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *fail,
                                           int *status) {
-    return __all_sync(0xffffffffu, bar_wait(bar, parity, fail, status));
+    return __all_sync(0xffffffffu, bar_wait<CLUSTER>(bar, parity, fail, status));
 }
 __device__ __forceinline__ void tma2(uint32_t dst, const CUtensorMap *map, int x, int y,
                                      uint32_t bar) {
@@ -462,7 +476,7 @@ struct Smem {
     // of the epilogue (one token, 8192 x 2048: 740 clocks a block with two).
     static constexpr int kAcc = KIND == kE4M3 && COLS <= 64 ? 8 : 2;
     struct Ctl {
-        unsigned long long full[STAGES], empty[STAGES], tfull[kAcc], tempty[kAcc], done;
+        unsigned long long full[STAGES], empty[STAGES], checked[STAGES], tfull[kAcc], tempty[kAcc], done;
         unsigned long long sfull[kScaleStages], sempty[kScaleStages];
         uint32_t tmem;
         int fail;
@@ -530,7 +544,7 @@ __device__ __forceinline__ bool add_parts(const float (&v)[2][16], float (*part)
                         ok ? v[h][4 * j + q] : __int_as_float(0x7fffffff);
     __syncwarp();
     if (lane < size) bar_arrive_in(pfull, lane);
-    if (ok) ok = warp_wait(pfull, 0, fail, status);
+    if (ok) ok = warp_wait<true>(pfull, 0, fail, status);
     const int per = kLanes / 2 / size;              // feature pairs of this block
     for (int i = threadIdx.x; i < valid * per; i += kEpiWarps * 32) {
         const int c = i / per, f = (rank * per + i - c * per) * 2;
@@ -585,6 +599,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         for (int i = 0; i < STAGES; ++i) {
             bar_init(smem_u32(&ctl.full[i]), 1);
             bar_init(smem_u32(&ctl.empty[i]), 1);
+            bar_init(smem_u32(&ctl.checked[i]), 1);
         }
         for (int i = 0; i < ACC; ++i) {
             bar_init(smem_u32(&ctl.tfull[i]), 1);
@@ -684,64 +699,68 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 }
             }
         } else if (warp == kMmaWarp) {
-            // MMA issuer
-            uint32_t it = 0, acc = 0;
-            bool ok = true;
-            while (ok && walk.next(t)) {
-                const int nkb = t.nkb;
-                if (nkb == 0) continue;
-                const uint32_t idesc = instr_desc<KIND, A_MN, B_MN>(t.ncols);
-                for (int kb = 0; kb < nkb; ++kb, ++it) {
-                    // e4m3: every stage has an accumulator buffer of its own
-                    // (scaled and added in fp32 registers); otherwise every tile
-                    if (KIND == kE4M3 || kb == 0) {
-                        if (!warp_wait(smem_u32(&ctl.tempty[acc % ACC]), ((acc / ACC) & 1) ^ 1, fail, p.status)) {
-                            ok = false;
-                            break;
-                        }
+            // MMA issuer: one thread runs the whole loop (a warp that elected a
+            // thread and met again for every stage took 220 clocks more for it)
+            if (elect_one()) {
+                uint32_t it = 0, acc = 0;
+                bool ok = true;
+                while (ok && walk.next(t)) {
+                    if (t.nkb == 0) continue;
+                    const uint32_t idesc = instr_desc<KIND, A_MN, B_MN>(t.ncols);
+                    for (int kb = 0; kb < t.nkb; ++kb, ++it) {
+                        const uint32_t s = it % STAGES;
+                        // e4m3: every stage has an accumulator buffer of its own
+                        // (scaled and added in fp32 registers); otherwise every tile
+                        if (KIND == kE4M3 || kb == 0)
+                            ok = bar_wait(smem_u32(&ctl.tempty[acc % ACC]), ((acc / ACC) & 1) ^ 1, fail, p.status);
+                        if (ok)
+                            ok = bar_wait(smem_u32(WHICH == kWgrad ? &ctl.checked[s] : &ctl.full[s]),
+                                          (it / STAGES) & 1, fail, p.status);
+                        if (!ok) break;
                         tc_fence_after();
-                    }
-                    const uint32_t s = it % STAGES;
-                    if (!warp_wait(smem_u32(&ctl.full[s]), (it / STAGES) & 1, fail, p.status)) {
-                        ok = false;
-                        break;
-                    }
-                    unsigned char *a = buf + s * S::kStage, *b = a + S::kA;
-                    if constexpr (WHICH == kWgrad) {
-                        const int rows = t.depth - kb * BK;
-                        if (rows < BK) {
-                            // rows of the next group (or behind the last one) do not
-                            // count, whatever they hold: both factors become zero
-                            const int cells = (BK - rows) * (kRowBytes / 16);
-                            const int blocks = kLanes / MNB + (t.ncols + MNB - 1) / MNB;
-                            for (int j = 0; j < blocks; ++j) {
-                                uint4 *z = reinterpret_cast<uint4 *>(a + j * MN_BLOCK + rows * kRowBytes);
-                                for (int i = lane; i < cells; i += 32) z[i] = make_uint4(0, 0, 0, 0);
-                            }
-                            fence_async();
-                            __syncwarp();
-                        }
-                    }
-                    tc_fence_after();
-                    if (elect_one()) {
-                        const uint64_t da = operand_desc(smem_u32(a), MN_BLOCK);
-                        const uint64_t db = operand_desc(smem_u32(b), MN_BLOCK);
+                        const uint32_t a = smem_u32(buf + s * S::kStage);
+                        const uint64_t da = operand_desc(a, MN_BLOCK), db = operand_desc(a + S::kA, MN_BLOCK);
                         const uint32_t d = tmem + (acc % ACC) * COLS;
 #pragma unroll
                         for (int j = 0; j < SLICES; ++j)
                             mma<KIND>(d, da + ((j * A_STEP) >> 4), db + ((j * B_STEP) >> 4), idesc,
                                       (KIND == kE4M3 ? j > 0 : (kb | j) > 0) ? 1u : 0u);
+                        if (KIND == kE4M3 || kb == t.nkb - 1) mma_commit(smem_u32(&ctl.tfull[acc++ % ACC]));
                         mma_commit(smem_u32(&ctl.empty[s]));
-                        if (KIND == kE4M3 || kb == nkb - 1) mma_commit(smem_u32(&ctl.tfull[acc % ACC]));
                     }
-                    __syncwarp();
-                    if (KIND == kE4M3 || kb == nkb - 1) ++acc;
+                }
+                // every matrix instruction has ended before the block frees its TMEM
+                mma_commit(smem_u32(&ctl.done));
+                volatile int never = 0;
+                bar_wait(smem_u32(&ctl.done), 0, &never, nullptr);
+            }
+        } else if constexpr (WHICH == kWgrad) {
+            // Between the loads and the products one warp sees every stage: the
+            // rows of a group's last one that belong to the next group (or lie
+            // behind the last group) do not count, whatever they hold, and
+            // become zero in both factors.
+            uint32_t it = 0;
+            bool ok = warp == kScaleWarp;
+            while (ok && walk.next(t)) {
+                for (int kb = 0; kb < t.nkb; ++kb, ++it) {
+                    const uint32_t s = it % STAGES;
+                    ok = warp_wait(smem_u32(&ctl.full[s]), (it / STAGES) & 1, fail, p.status);
+                    if (!ok) break;
+                    const int rows = t.depth - kb * BK;
+                    if (rows < BK) {
+                        unsigned char *a = buf + s * S::kStage;
+                        const int cells = (BK - rows) * (kRowBytes / 16);
+                        const int blocks = kLanes / MNB + (t.ncols + MNB - 1) / MNB;
+                        for (int j = 0; j < blocks; ++j) {
+                            uint4 *z = reinterpret_cast<uint4 *>(a + j * MN_BLOCK + rows * kRowBytes);
+                            for (int i = lane; i < cells; i += 32) z[i] = make_uint4(0, 0, 0, 0);
+                        }
+                        fence_async();
+                        __syncwarp();
+                    }
+                    if (lane == 0) bar_arrive(smem_u32(&ctl.checked[s]));
                 }
             }
-            // every matrix instruction has ended before the block frees its TMEM
-            if (elect_one()) mma_commit(smem_u32(&ctl.done));
-            volatile int never = 0;
-            bar_wait(smem_u32(&ctl.done), 0, &never, nullptr);
         } else if constexpr (KIND == kE4M3) {
             // Scales of the rows and of the weight block, one slot for each k
             // block, fetched up to kScaleStages blocks ahead by two warps

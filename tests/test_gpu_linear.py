@@ -97,6 +97,7 @@ GROUPS = [
     ([1], 1040, 2064),                             # tiles (forward and rows' gradient)
     ([33], 16, 8208),
     ([0, 64, 0], 528, 512),
+    ([7, 33, 0, 64, 12, 1] * 40, 144, 272),        # several tiles and short groups for each block
     ([3, 1, 4, 1, 5, 9, 2, 6, 5, 3, 5, 8, 9, 7, 9, 3] * 5, 32, 96),   # 80 groups
 ]
 
