@@ -168,9 +168,341 @@ cudaError_t run_blocks(const void *w, long blocks, int n, int k, void *q, float 
     return cudaGetLastError();
 }
 
+// ---------------------------------------------------------------------------
+// The product of more than 64 rows.
+//
+// Every k block of 128 is scaled on its own, so the tensor core's sums leave
+// TMEM once for each of them, and that traffic and the fp32 additions, not the
+// products, bound the kernel.  Here the rows of x lie on the lanes and the
+// features on the columns (the other way round from mm_kernel): a thread has
+// one row, a half of the epilogue one block of 128 features, and the two
+// scales become one factor per thread and block, against one for each column.
+// Each half has accumulator buffers and an issuing warp of its own, so that
+// they run out of step: one half's sums run under the other's products.
+constexpr int kRowTile = 128, kFeatTile = 256, kRowStages = 4;
+constexpr int kStoreCols = 32, kStorePitch = kStoreCols * 2 + 16;
+constexpr uint32_t kBlockBytes = 128 * kRowBytes;
+// Registers: 3 warpgroups x 168 at launch; the two of the epilogue hold 128
+// sums a thread and take over most of the third one's share.
+constexpr int kLaunchRegs = 168, kFewRegs = 56, kManyRegs = 224;
+static_assert(kFewRegs + 2 * kManyRegs == 3 * kLaunchRegs, "");
+
+struct RowsCtl {
+    unsigned long long full[kRowStages], empty[kRowStages];
+    unsigned long long tfull[2][2], tempty[2][2], done[2];     // [half][buffer]
+    uint32_t tmem;
+    int fail;
+    alignas(16) unsigned char stage[kEpiWarps][32 * kStorePitch];
+    Groups groups;
+};
+constexpr size_t kRowsBytes = 1024 + size_t(kRowStages) * 3 * kBlockBytes + sizeof(RowsCtl);
+static_assert(kRowsBytes <= 232448, "shared memory of one block");
+
+struct RowTile {
+    int group, row0, rows, feat0;
+};
+
+// Feature tiles of a row tile follow one another: they share the rows, and the
+// weights of a layer stay in L2.
+struct RowWalk {
+    const Groups &g;
+    const Params &p;
+    int feat_tiles, total, tile, group;
+    __device__ RowWalk(const Groups &g_, const Params &p_) : g(g_), p(p_) {
+        feat_tiles = (p.lanes + kFeatTile - 1) / kFeatTile;
+        total = g.first[p.E] * feat_tiles;
+        tile = blockIdx.x;
+        group = 0;
+    }
+    __device__ bool next(RowTile &t) {
+        if (tile >= total) return false;
+        while (tile >= g.first[group + 1] * feat_tiles) ++group;
+        const int in = tile - g.first[group] * feat_tiles, r = in / feat_tiles;
+        t.group = group;
+        t.row0 = g.off[group] + r * kRowTile;
+        t.rows = min(kRowTile, g.off[group + 1] - t.row0);
+        t.feat0 = (in - r * feat_tiles) * kFeatTile;
+        tile += gridDim.x;
+        return true;
+    }
+};
+
+template <typename OUT, int WHICH>
+__global__ void __launch_bounds__(kThreads, 1)
+fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
+                const __grid_constant__ Params p) {
+    constexpr bool W_MN = WHICH == kDgrad;
+    constexpr int BK = kRowBytes, SLICES = 4;
+    constexpr uint32_t W_STEP = W_MN ? BK / SLICES * kRowBytes : 32;
+
+    extern __shared__ unsigned char raw[];
+    unsigned char *buf = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    RowsCtl &ctl = *reinterpret_cast<RowsCtl *>(buf + size_t(kRowStages) * 3 * kBlockBytes);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    volatile int *fail = &ctl.fail;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kRowStages; ++i) {
+            bar_init(smem_u32(&ctl.full[i]), 1);
+            bar_init(smem_u32(&ctl.empty[i]), 2);
+        }
+        for (int i = 0; i < 4; ++i) {
+            bar_init(smem_u32(&ctl.tfull[i >> 1][i & 1]), 1);
+            bar_init(smem_u32(&ctl.tempty[i >> 1][i & 1]), kEpiWarps / 2);
+        }
+        bar_init(smem_u32(&ctl.done[0]), 1);
+        bar_init(smem_u32(&ctl.done[1]), 1);
+        ctl.fail = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        if (blockIdx.x == 0 && p.status) *p.status = 0;   // a failure is a second away
+    }
+    if (threadIdx.x == 32) {
+        prefetch_map(&tw);
+        prefetch_map(&tx);
+    }
+    if (warp == kMmaWarp) tmem_alloc(smem_u32(&ctl.tmem), 512);
+    read_groups(ctl.groups, p);
+    __syncthreads();
+    if (warp == kTmaWarp) scan_groups<kRowTile>(ctl.groups, p, lane);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = ctl.tmem;
+    const int nkb = (p.depth + BK - 1) / BK;
+    RowWalk walk(ctl.groups, p);
+    RowTile t;
+
+    // (a warpgroup sets its registers in one place, and the two sides meet only
+    // at the end: where branches meet, the compiler holds the code to the
+    // smaller share)
+    if (warp >= kEpiWarps) {
+        regs_down<kFewRegs>();
+        if (warp == kTmaWarp) {
+            if (elect_one()) {
+                uint32_t it = 0, ahead = 0;
+                bool ok = true;
+                auto load_w = [&](const RowTile &t, int kb, uint32_t s) {
+                    const uint32_t bar = smem_u32(&ctl.full[s]), w = smem_u32(buf + s * 3 * kBlockBytes) + kBlockBytes;
+                    const bool two = t.feat0 + 128 < p.lanes;
+                    bar_expect(bar, (two ? 3 : 2) * kBlockBytes);
+                    for (int h = 0; h < (two ? 2 : 1); ++h) {
+                        if constexpr (W_MN) tma3(w + h * kBlockBytes, &tw, t.feat0 + h * 128, kb * BK, t.group, bar);
+                        else tma3(w + h * kBlockBytes, &tw, kb * BK, t.feat0 + h * 128, t.group, bar);
+                    }
+                };
+                const bool drop = p.drop && blockIdx.x == 0;      // test option: the first load is withheld
+                if (p.dependent) {
+                    // the weights do not come from the kernel before this one
+                    RowWalk first = walk;
+                    if (first.next(t))
+                        for (; ahead < kRowStages && int(ahead) < nkb; ++ahead)
+                            if (!drop || ahead) load_w(t, ahead, ahead);
+                    wait_for_previous();
+                }
+                while (ok && walk.next(t)) {
+                    for (int kb = 0; kb < nkb; ++kb, ++it) {
+                        const uint32_t s = it % kRowStages;
+                        if (it >= ahead) {
+                            if (!bar_wait(smem_u32(&ctl.empty[s]), ((it / kRowStages) & 1) ^ 1, fail, p.status)) {
+                                ok = false;
+                                break;
+                            }
+                            if (!drop || it) load_w(t, kb, s);
+                        }
+                        if (drop && it == 0) continue;
+                        tma2(smem_u32(buf + s * 3 * kBlockBytes), &tx, kb * BK, t.row0, smem_u32(&ctl.full[s]));
+                    }
+                }
+                if (!ok) {
+                    // copies in flight land before the block ends
+                    volatile int never = 0;
+                    for (uint32_t i = it > kRowStages ? it - kRowStages : 0; i < it; ++i)
+                        if (!(drop && i == 0))
+                            bar_wait(smem_u32(&ctl.full[i % kRowStages]), (i / kRowStages) & 1, &never, nullptr);
+                }
+            }
+        } else if (warp <= kMmaWarp + 1) {
+            // one issuing thread for each half of the features
+            if (elect_one()) {
+                const int half = warp - kMmaWarp;
+                uint32_t it = 0, acc = 0;
+                bool ok = true;
+                while (ok && walk.next(t)) {
+                    const int n = min(128, p.lanes - t.feat0 - half * 128);
+                    const uint32_t idesc = instr_desc<kE4M3, false, W_MN>(n > 0 ? n : 16);
+                    for (int kb = 0; kb < nkb; ++kb, ++it) {
+                        const uint32_t s = it % kRowStages;
+                        if (n > 0)
+                            ok = bar_wait(smem_u32(&ctl.tempty[half][acc & 1]), ((acc >> 1) & 1) ^ 1, fail, p.status);
+                        if (ok) ok = bar_wait(smem_u32(&ctl.full[s]), (it / kRowStages) & 1, fail, p.status);
+                        if (!ok) break;
+                        if (n > 0) {
+                            tc_fence_after();
+                            const uint32_t x = smem_u32(buf + s * 3 * kBlockBytes);
+                            const uint64_t dx = operand_desc(x, 0), dw = operand_desc(x + (1 + half) * kBlockBytes, 0);
+                            const uint32_t d = tmem + (half * 2 + (acc & 1)) * 128;
+#pragma unroll
+                            for (int j = 0; j < SLICES; ++j)
+                                mma<kE4M3>(d, dx + ((j * 32) >> 4), dw + ((j * W_STEP) >> 4), idesc, j > 0 ? 1u : 0u);
+                            mma_commit(smem_u32(&ctl.tfull[half][acc++ & 1]));
+                            mma_commit(smem_u32(&ctl.empty[s]));
+                        } else {
+                            bar_arrive(smem_u32(&ctl.empty[s]));
+                        }
+                    }
+                }
+                // every matrix instruction has ended before the block frees its TMEM
+                mma_commit(smem_u32(&ctl.done[half]));
+                volatile int never = 0;
+                bar_wait(smem_u32(&ctl.done[half]), 0, &never, nullptr);
+            }
+        }
+    } else {
+        regs_up<kManyRegs>();
+        const int quad = warp & 3, half = warp >> 2;
+        const uint32_t lanes_at = static_cast<uint32_t>(quad * 32) << 16;
+        unsigned char *stage = ctl.stage[warp];
+        uint32_t acc = 0;
+        bool ok = true;
+        if (p.dependent) wait_for_previous();
+        bool more = walk.next(t);
+        // scales of this thread's row and of the half's weight block, two k
+        // blocks ahead; those of the next tile are on their way while this one
+        // is stored
+        const float *xs = p.xs, *ws = p.ws;
+        long xs_step = 0, ws_step = 0;
+        float x0 = 0.f, x1 = 0.f, w0 = 0.f, w1 = 0.f;
+        auto begin = [&] {
+            const int r = quad * 32 + lane, f = t.feat0 + half * 128;
+            const bool real = r < t.rows && f < p.lanes;
+            xs = p.xs + (real ? (t.row0 + r) * p.xs_row : 0);
+            ws = p.ws + (real ? t.group * p.ws_group + (f >> 7) * p.ws_lane : 0);
+            xs_step = real ? p.xs_blk : 0;
+            ws_step = real ? p.ws_blk : 0;
+            x0 = *xs;
+            w0 = *ws;
+            if (nkb > 1) {
+                x1 = *(xs += xs_step);
+                w1 = *(ws += ws_step);
+            }
+        };
+        if (more) begin();
+        while (more) {
+            const int feats = min(128, p.lanes - t.feat0 - half * 128);
+            const RowTile now = t;
+            if (feats > 0) {
+                float sum[4][32];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) sum[i][j] = 0.f;
+                for (int kb = 0; kb < nkb; ++kb, ++acc) {
+                    const float f = x0 * w0;
+                    x0 = x1;
+                    w0 = w1;
+                    if (kb + 2 < nkb) {
+                        x1 = *(xs += xs_step);
+                        w1 = *(ws += ws_step);
+                    }
+                    if (ok) ok = warp_wait(smem_u32(&ctl.tfull[half][acc & 1]), (acc >> 1) & 1, fail, p.status);
+                    if (!ok) continue;
+                    tc_fence_after();
+                    const uint32_t at = tmem + lanes_at + (half * 2 + (acc & 1)) * 128;
+                    const float2 ff = make_float2(f, f);
+                    float v[2][32];
+                    tmem_ld_row(v[0], at);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        tmem_wait_row(v[i & 1]);
+                        if (i < 3) tmem_ld_row(v[(i + 1) & 1], at + (i + 1) * 32);
+                        else {
+                            tc_fence_before();
+                            __syncwarp();
+                            if (lane == 0) bar_arrive(smem_u32(&ctl.tempty[half][acc & 1]));
+                        }
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            const float2 r = __ffma2_rn(make_float2(v[i & 1][j], v[i & 1][j + 1]), ff,
+                                                        make_float2(sum[i][j], sum[i][j + 1]));
+                            sum[i][j] = r.x;
+                            sum[i][j + 1] = r.y;
+                        }
+                    }
+                }
+                more = walk.next(t);
+                if (more) begin();
+                // 32 rows x 32 features at a time: each thread's row into shared
+                // memory, then 64 contiguous bytes for 4 threads
+                OUT *out = static_cast<OUT *>(p.out) + static_cast<long>(now.row0 + quad * 32) * p.ldo + now.feat0 + half * 128;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    if (i * kStoreCols < feats) {
+                        if (!ok) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) sum[i][j] = __int_as_float(0x7fffffff);
+                        }
+                        __syncwarp();
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const float *v = &sum[i][8 * q];
+                            *reinterpret_cast<uint4 *>(stage + lane * kStorePitch + q * 16) =
+                                make_uint4(pack<OUT>(v[0], v[1]), pack<OUT>(v[2], v[3]), pack<OUT>(v[4], v[5]), pack<OUT>(v[6], v[7]));
+                        }
+                        __syncwarp();
+                        const int c = i * kStoreCols + (lane & 3) * 8;
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            const int r = q * 8 + (lane >> 2);
+                            if (quad * 32 + r < now.rows && c < feats)
+                                *reinterpret_cast<uint4 *>(out + r * p.ldo + c) =
+                                    *reinterpret_cast<const uint4 *>(stage + r * kStorePitch + (lane & 3) * 16);
+                        }
+                    }
+                }
+            } else {
+                more = walk.next(t);
+                if (more) begin();
+            }
+        }
+        // rows of no group are zero
+        const int lo = ctl.groups.off[0], hi = ctl.groups.off[p.E];
+        const long rows = static_cast<long>(lo) + (p.T - hi);
+        for (long r = blockIdx.x; r < rows; r += gridDim.x) {
+            OUT *o = static_cast<OUT *>(p.out) + (r < lo ? r : r - lo + hi) * p.ldo;
+            for (int f = threadIdx.x; f < p.lanes; f += kEpiWarps * 32) o[f] = from_float<OUT>(0.f);
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == kMmaWarp) tmem_free(tmem, 512);
+}
+
+template <typename OUT, int WHICH>
+cudaError_t launch_many(const Call &c) {
+    using U = unsigned long long;
+    CUtensorMap tw, tx;
+    int dev = 0;
+    const int sms = grid_sms(&dev);
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    const U wd[3] = {U(c.a_inner), U(c.a_rows), U(c.p.E)}, wst[2] = {U(c.a_inner), U(c.a_inner) * U(c.a_rows)};
+    const U xd[2] = {U(c.b_inner), U(c.p.T)}, xst[1] = {U(c.ld_b)};
+    const unsigned wb[3] = {128, 128, 1}, xb[2] = {128, unsigned(kRowTile)};
+    if (!make_map(&tw, kE4M3, 3, c.a, wd, wst, wb) || !make_map(&tx, kE4M3, 2, c.b, xd, xst, xb)) return cudaErrorInvalidValue;
+    const Kernel k = &fp8_rows_kernel<OUT, WHICH>;
+    static std::atomic<bool> ready[kMaxDevices];
+    const cudaError_t e = set_up(k, kRowsBytes, kLaunchRegs, ready[dev]);
+    if (e != cudaSuccess) return e;
+    const long row_tiles = c.p.T / kRowTile + (c.p.E < c.p.T ? c.p.E : c.p.T);
+    const long tiles = row_tiles * ((c.p.lanes + kFeatTile - 1) / kFeatTile);
+    return launch_on(k, tiles < sms ? tiles : sms, 1, kRowsBytes, c, tw, tx);
+}
+
 template <typename OUT>
 cudaError_t run_mm(const Call &c) {
-    return c.which == kForward ? launch_rows<kE4M3, OUT, kForward>(c) : launch_rows<kE4M3, OUT, kDgrad>(c);
+    if (c.p.T <= 64) return c.which == kForward ? launch_few<kE4M3, OUT, kForward>(c) : launch_few<kE4M3, OUT, kDgrad>(c);
+    return c.which == kForward ? launch_many<OUT, kForward>(c) : launch_many<OUT, kDgrad>(c);
 }
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }

@@ -12,7 +12,8 @@ namespace {
 template <int KIND, typename T>
 cudaError_t run(const Call &c) {
     if (c.which == kWgrad) return launch<KIND, T, kWgrad, 256, 4, false>(c);
-    return c.which == kForward ? launch_rows<KIND, T, kForward>(c) : launch_rows<KIND, T, kDgrad>(c);
+    if (c.p.T <= 64) return c.which == kForward ? launch_few<KIND, T, kForward>(c) : launch_few<KIND, T, kDgrad>(c);
+    return c.which == kForward ? launch<KIND, T, kForward, 256, 4, false>(c) : launch<KIND, T, kDgrad, 256, 4, false>(c);
 }
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }

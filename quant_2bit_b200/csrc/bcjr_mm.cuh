@@ -224,6 +224,27 @@ __device__ __forceinline__ void tmem_wait(float (&a)[16], float (&b)[16]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(b[i]));
 }
+// One lane and 32 columns per thread.
+__device__ __forceinline__ void tmem_ld_row(float (&v)[32], uint32_t addr) {
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+}
+__device__ __forceinline__ void tmem_wait_row(float (&v)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
+}
 // Four 8 x 8 blocks of 16-bit values, transposed on the way: thread t gives
 // row t / 4, columns 2 (t % 4).. of each; the address of thread 8 m + c
 // receives column c of block m.
@@ -458,12 +479,6 @@ template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
 constexpr int kScaleStages = 8;
 constexpr int kPartPitch = kLanes + 4;            // floats: no bank conflicts either way
 
-// The e4m3 kernel with 256 columns holds 128 fp32 sums per epilogue thread.
-// It is launched with 168 registers a thread (3 warpgroups x 168 = 504) and
-// the third warpgroup hands most of its share to the other two: 56 + 2 x 224.
-constexpr int kLaunchRegs = 168, kFewRegs = 56, kManyRegs = 224;
-static_assert(kFewRegs + 2 * kManyRegs == 3 * kLaunchRegs, "");
-template <int KIND, int COLS> constexpr bool kSplitsRegs = KIND == kE4M3 && COLS == 256;
 
 template <int KIND, int COLS, int STAGES, bool SPLIT>
 struct Smem {
@@ -631,11 +646,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     Walk<WHICH, COLS, BK, SPLIT> walk(ctl.groups, p);
     Tile t;
 
-    // (a warpgroup sets its registers in one place, and the two sides meet only
-    // at the end: where branches meet, the compiler holds the code to the
-    // smaller share)
     if (warp >= kEpiWarps) {
-        if constexpr (kSplitsRegs<KIND, COLS>) regs_down<kFewRegs>();
         if (warp == kTmaWarp) {
             // TMA producer
             if (elect_one()) {
@@ -803,7 +814,6 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             asm volatile("cp.async.wait_all;" ::: "memory");
         }
     } else {
-        if constexpr (kSplitsRegs<KIND, COLS>) regs_up<kManyRegs>();
         // epilogue: warp w has lanes 32 (w % 4).., column chunks w / 4, w / 4 + 2, ...
         constexpr int CHUNKS = COLS / (2 * kChunk);
         static_assert(COLS % (2 * kChunk) == 0, "");
@@ -973,34 +983,9 @@ bool make_maps(const Call &c, CUtensorMap &ta, CUtensorMap &tb) {
     return make_map(&tb, KIND, 2, c.b, dims, st, box);
 }
 
-template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, bool SPLIT>
-cudaError_t launch(const Call &c) {
-    CUtensorMap ta, tb;
-    int dev = 0;
-    const int sms = grid_sms(&dev);
-    if (sms <= 0) return cudaErrorInvalidDevice;
-    if (!make_maps<KIND, WHICH>(c, ta, tb)) return cudaErrorInvalidValue;
-    auto *k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES, SPLIT>;
-    constexpr size_t bytes = Smem<KIND, COLS, STAGES, SPLIT>::bytes();
-    static_assert(bytes <= 232448, "shared memory of one block");
-    static std::atomic<bool> ready[kMaxDevices];      // this kernel's setting on each device
-    if (!ready[dev].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-        if (e != cudaSuccess) return e;
-        if (kSplitsRegs<KIND, COLS>) {
-            // a split of more registers than the block was launched with would wait for good
-            cudaFuncAttributes f;
-            if (cudaFuncGetAttributes(&f, k) != cudaSuccess || f.numRegs != kLaunchRegs)
-                return cudaErrorInvalidConfiguration;
-        }
-        ready[dev].store(true, std::memory_order_release);
-    }
-    // no more blocks than there can be tiles
-    const long lane_tiles = (c.p.lanes + kLanes - 1) / kLanes;
-    const long col_tiles = WHICH == kWgrad ? long(c.p.E) * ((c.p.cols + COLS - 1) / COLS)
-                                           : c.p.T / COLS + (c.p.E < c.p.T ? c.p.E : c.p.T);
-    const long tiles = lane_tiles * (col_tiles > 0 ? col_tiles : 1);
-    const long blocks = SPLIT ? tiles * c.split : tiles < sms ? tiles : sms;
+using Kernel = void (*)(CUtensorMap, CUtensorMap, Params);
+inline cudaError_t launch_on(Kernel k, long blocks, int cluster, size_t bytes, const Call &c,
+                             const CUtensorMap &ta, const CUtensorMap &tb) {
     if (blocks > 0x7fffffffL) return cudaErrorInvalidValue;
     cudaLaunchAttribute a[2];
     cudaLaunchConfig_t cfg = {};
@@ -1008,9 +993,9 @@ cudaError_t launch(const Call &c) {
         a[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
         a[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
     }
-    if (SPLIT) {
+    if (cluster > 1) {
         a[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
-        a[cfg.numAttrs].val.clusterDim.x = unsigned(c.split);
+        a[cfg.numAttrs].val.clusterDim.x = unsigned(cluster);
         a[cfg.numAttrs].val.clusterDim.y = a[cfg.numAttrs].val.clusterDim.z = 1;
         ++cfg.numAttrs;
     }
@@ -1022,11 +1007,44 @@ cudaError_t launch(const Call &c) {
     return cudaLaunchKernelEx(&cfg, k, ta, tb, c.p);
 }
 
-// Forward and dgrad.  Up to 64 rows every group is one tile of at most 64
+// A kernel's settings on the current device, once: its shared memory, and for
+// one that splits registers that it was compiled for the expected number (a
+// split of more registers than a block is launched with would wait for good).
+inline cudaError_t set_up(Kernel k, size_t bytes, int regs, std::atomic<bool> &ready) {
+    if (ready.load(std::memory_order_acquire)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (e != cudaSuccess) return e;
+    cudaFuncAttributes f;
+    if (regs && (cudaFuncGetAttributes(&f, k) != cudaSuccess || f.numRegs != regs)) return cudaErrorInvalidConfiguration;
+    ready.store(true, std::memory_order_release);
+    return cudaSuccess;
+}
+
+template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, bool SPLIT>
+cudaError_t launch(const Call &c) {
+    CUtensorMap ta, tb;
+    int dev = 0;
+    const int sms = grid_sms(&dev);
+    if (sms <= 0) return cudaErrorInvalidDevice;
+    if (!make_maps<KIND, WHICH>(c, ta, tb)) return cudaErrorInvalidValue;
+    const Kernel k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES, SPLIT>;
+    constexpr size_t bytes = Smem<KIND, COLS, STAGES, SPLIT>::bytes();
+    static_assert(bytes <= 232448, "shared memory of one block");
+    static std::atomic<bool> ready[kMaxDevices];
+    const cudaError_t e = set_up(k, bytes, 0, ready[dev]);
+    if (e != cudaSuccess) return e;
+    // no more blocks than there can be tiles
+    const long lane_tiles = (c.p.lanes + kLanes - 1) / kLanes;
+    const long col_tiles = WHICH == kWgrad ? long(c.p.E) * ((c.p.cols + COLS - 1) / COLS)
+                                           : c.p.T / COLS + (c.p.E < c.p.T ? c.p.E : c.p.T);
+    const long tiles = lane_tiles * (col_tiles > 0 ? col_tiles : 1);
+    return launch_on(k, SPLIT ? tiles * c.split : tiles < sms ? tiles : sms, SPLIT ? c.split : 1, bytes, c, ta, tb);
+}
+
+// Forward and dgrad of at most 64 rows: every group is one tile of at most 64
 // columns, and with few tiles the blocks of a cluster share each one.
 template <int KIND, typename OUT, int WHICH>
-cudaError_t launch_rows(Call c) {
-    if (c.p.T > 64) return launch<KIND, OUT, WHICH, 256, 4, false>(c);
+cudaError_t launch_few(Call c) {
     int dev = 0;
     const int sms = grid_sms(&dev);
     const int nkb = (c.p.depth * (KIND == kE4M3 ? 1 : 2) + kRowBytes - 1) / kRowBytes;

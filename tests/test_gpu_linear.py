@@ -442,7 +442,7 @@ def _check_fp8(x, q, s, w64, dy, offsets):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,N,K", [(1, 16, 16), (1, 128, 256), (17, 144, 272), (64, 2000, 400),
                                    (65, 48, 128), (300, 272, 1040), (513, 128, 144), (37, 48, 4240), (1, 2064, 528),
-                                   (64, 144, 1280)])
+                                   (64, 144, 1280), (200, 656, 304), (129, 16, 16)])
 def test_fp8_linear_forward_and_gradient(cuda_ok, T, N, K, dtype):
     x, q, s, w64, dy = _fp8_operands(T, 0, N, K, dtype, seed=T)
     _check_fp8(x, q, s, w64, dy, None)
@@ -584,7 +584,18 @@ def test_a_wait_that_runs_out_is_reported(cuda_ok):
         return lib.bcjr_grouped_wgrad(dy.data_ptr(), 32, x.data_ptr(), 64, None, 0, 20, 1, 32, 64,
                                       0, dw.data_ptr(), status.data_ptr(), stream)
 
-    for call, out in ((forward, y), (wgrad, dw)):
+    from quant_2bit_b200 import fp8_quantize_weight
+    q, s = fp8_quantize_weight(torch.randn(32, 64, device="cuda"))
+    x8 = torch.randn(70, 64, device="cuda").to(torch.bfloat16)
+    y8 = torch.zeros(70, 32, dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(lib.bcjr_fp8_linear_workspace_bytes(70, 64), dtype=torch.uint8, device="cuda")
+
+    def fp8(rows):
+        return lib.bcjr_fp8_linear(x8.data_ptr(), 64, 0, q.data_ptr(), s.data_ptr(), None, 0, rows, 1,
+                                   32, 64, 0, y8.data_ptr(), ws.data_ptr(), ws.numel(),
+                                   status.data_ptr(), stream)
+
+    for call, out in ((forward, y), (wgrad, dw), (lambda: fp8(20), y8[:20]), (lambda: fp8(70), y8)):
         with _lib.test_option(_lib.OPT_TEST_DROP_SENDS, 1):
             assert call() == 0
             assert lib.bcjr_ws_status(ctypes.c_void_p(status.data_ptr()), stream) == _lib.BCJR_ERR_TIMEOUT
