@@ -310,19 +310,21 @@ BCJR_API int bcjr_hyb_codebook(const float *lut, int Q, int L, float *cb_out, bc
  */
 enum { BCJR_BF16 = 0, BCJR_F16 = 1, BCJR_F32 = 2 };
 
-/* transpose_w 0: out (T x N) = rows (T x K) times w[e]^T; 1: out (T x K) =
- * rows (T x N) times w[e], the gradient of the first with respect to its
- * rows.  Rows of no group are zero in `out`, which is contiguous.  dtype
- * BCJR_BF16 or BCJR_F16 for rows, w and out. */
-BCJR_API int bcjr_grouped_mm(const void *rows, long ld_rows, const void *w, const void *offsets,
-                             int offsets_bytes, long T, int E, int N, int K, int dtype,
-                             int transpose_w, void *out, int *status, bcjr_stream_t stream);
+/* y (T x N) = x (T x K) times w[e]^T for the rows of each group e.  Rows of no
+ * group are zero in y, which is contiguous (as all outputs are).  dtype
+ * BCJR_BF16 or BCJR_F16 for x, w and y. */
+BCJR_API int bcjr_grouped_mm(const void *x, long ld_x, const void *w, const void *offsets,
+                             int offsets_bytes, long T, int E, int N, int K, int dtype, void *y,
+                             int *status, bcjr_stream_t stream);
 
-/* dw[e] (N x K) = dy[group e]^T (N x T_e) times x[group e] (T_e x K); zero for
- * an empty group. */
-BCJR_API int bcjr_grouped_wgrad(const void *dy, long ld_dy, const void *x, long ld_x,
-                                const void *offsets, int offsets_bytes, long T, int E, int N,
-                                int K, int dtype, void *dw, int *status, bcjr_stream_t stream);
+/* The gradients of that product: dx (T x K) = dy (T x N) times w[e], zero for
+ * rows of no group, and dw[e] (N x K) = dy[group e]^T times x[group e], zero
+ * for an empty group.  Either output may be NULL and is then not computed (and
+ * w, or x, not read). */
+BCJR_API int bcjr_grouped_backward(const void *dy, long ld_dy, const void *x, long ld_x,
+                                   const void *w, const void *offsets, int offsets_bytes, long T,
+                                   int E, int N, int K, int dtype, void *dx, void *dw,
+                                   int *status, bcjr_stream_t stream);
 
 /* e4m3 quantizers (dtype of the input: BCJR_BF16, BCJR_F16 or BCJR_F32).
  * With amax = max(max |x|, 2^-100) over a block: scale = amax * (1/448), q =
@@ -340,8 +342,10 @@ BCJR_API int bcjr_fp8_quantize_rows(const void *x, long ld, long rows, int k, in
 BCJR_API int bcjr_fp8_quantize_blocks(const void *w, int E, int N, int K, int dtype, void *q,
                                       float *scale, bcjr_stream_t stream);
 
-/* bcjr_grouped_mm over such operands: rows quantized by rows along the
- * contraction, w by blocks; out_dtype BCJR_BF16 or BCJR_F16.  The product of
+/* transpose_w 0: out (T x N) = rows (T x K) times w[e]^T, over such operands;
+ * 1: out (T x K) = rows (T x N) times w[e], the gradient of the first with
+ * respect to its rows.  The rows are quantized by rows along the contraction,
+ * w by blocks; out_dtype BCJR_BF16 or BCJR_F16.  The product of
  * a row scale and a weight scale is formed in fp32 (it must not underflow). */
 BCJR_API int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long scale_row,
                          long scale_block, const void *w, const float *w_scale,

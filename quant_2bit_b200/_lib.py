@@ -55,8 +55,8 @@ SIGNATURES = {
     "bcjr_viterbi_launches": ([_I, _I, _I, _I, _I], _I),
     "bcjr_viterbi": ([_P, _P, _I, _I, _I, _I, _I, _P, _P, _P, _P, _P, _SZ, _P], _I),
     "bcjr_hyb_codebook": ([_P, _I, _I, _P, _P], _I),
-    "bcjr_grouped_mm": ([_P, _L, _P, _P, _I, _L, _I, _I, _I, _I, _I, _P, _P, _P], _I),
-    "bcjr_grouped_wgrad": ([_P, _L, _P, _L, _P, _I, _L, _I, _I, _I, _I, _P, _P, _P], _I),
+    "bcjr_grouped_mm": ([_P, _L, _P, _P, _I, _L, _I, _I, _I, _I, _P, _P, _P], _I),
+    "bcjr_grouped_backward": ([_P, _L, _P, _L, _P, _P, _I, _L, _I, _I, _I, _I, _P, _P, _P, _P], _I),
     "bcjr_fp8_quantize_rows": ([_P, _L, _L, _I, _I, _P, _P, _L, _L, _P], _I),
     "bcjr_fp8_quantize_blocks": ([_P, _I, _I, _I, _I, _P, _P, _P], _I),
     "bcjr_fp8_mm": ([_P, _L, _P, _L, _L, _P, _P, _P, _I, _L, _I, _I, _I, _I, _P, _I, _P, _P], _I),

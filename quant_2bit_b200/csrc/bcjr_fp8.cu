@@ -88,19 +88,22 @@ quantize_rows(const T *__restrict__ x, long ld, long rows, int k, uint8_t *__res
               float *__restrict__ scale, long s_row, long s_blk) {
     let_next_start();              // the product's set-up may overlap (it waits for this kernel's end)
     const int nb = (k + 127) / 128, sub = threadIdx.x & 15;
-    const long segs = rows * nb, groups = kQThreads / 16;
-    const long first = (blockIdx.x * groups * kUnroll) + (threadIdx.x >> 4);
+    constexpr int groups = kQThreads / 16;
     float v[kUnroll][8];
     long row[kUnroll];
     int blk[kUnroll];
+    // segments threadIdx / 16, + groups, ..  of the block's: one 64-bit division
+    // for the block, 32-bit ones for its threads
+    const long base = long(blockIdx.x) * (groups * kUnroll), row0 = base / nb;
+    const unsigned blk0 = unsigned(base - row0 * nb);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-        const long s = first + u * groups;
-        row[u] = s / nb;
-        blk[u] = int(s - row[u] * nb);
+        const unsigned s = blk0 + u * groups + (threadIdx.x >> 4), r = s / unsigned(nb);
+        row[u] = row0 + r;
+        blk[u] = int(s - r * nb);
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
-        if (s < segs && blk[u] * 128 + sub * 8 < k) load8(x + row[u] * ld + blk[u] * 128 + sub * 8, v[u]);
+        if (row[u] < rows && blk[u] * 128 + sub * 8 < k) load8(x + row[u] * ld + blk[u] * 128 + sub * 8, v[u]);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -108,8 +111,7 @@ quantize_rows(const T *__restrict__ x, long ld, long rows, int k, uint8_t *__res
 #pragma unroll
         for (int d = 8; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
         m = block_amax(m);
-        const long s = first + u * groups;
-        if (s >= segs) continue;
+        if (row[u] >= rows) continue;
         const int c = blk[u] * 128 + sub * 8;
         if (c < k) *reinterpret_cast<uint2 *>(q + row[u] * k + c) = to_e4m3(v[u], block_inv(m));
         if (sub == 0) scale[row[u] * s_row + blk[u] * s_blk] = block_scale(m);
@@ -169,7 +171,7 @@ cudaError_t run_blocks(const void *w, long blocks, int n, int k, void *q, float 
 }
 
 // ---------------------------------------------------------------------------
-// The product of more than 64 rows.
+// The product with more than a few rows to a group.
 //
 // Every k block of 128 is scaled on its own, so the tensor core's sums leave
 // TMEM once for each of them, and that traffic and the fp32 additions, not the
@@ -179,8 +181,8 @@ cudaError_t run_blocks(const void *w, long blocks, int n, int k, void *q, float 
 // scales become one factor per thread and block, against one for each column.
 // Each half has accumulator buffers and an issuing warp of its own, so that
 // they run out of step: one half's sums run under the other's products.
-constexpr int kRowTile = 128, kFeatTile = 256, kRowStages = 4;
-constexpr int kStoreCols = 32, kStorePitch = kStoreCols * 2 + 16;
+constexpr int kRowTile = 128, kFeatTile = 256, kRowStages = 3;
+constexpr int kStorePitch = 256 + 16;             // a row of 128 features; no bank conflicts
 constexpr uint32_t kBlockBytes = 128 * kRowBytes;
 // Registers: 3 warpgroups x 168 at launch; the two of the epilogue hold 128
 // sums a thread and take over most of the third one's share.
@@ -261,7 +263,7 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ 
         prefetch_map(&tx);
     }
     if (warp == kMmaWarp) tmem_alloc(smem_u32(&ctl.tmem), 512);
-    read_groups(ctl.groups, p);
+    read_groups<kThreads>(ctl.groups, p);
     __syncthreads();
     if (warp == kTmaWarp) scan_groups<kRowTile>(ctl.groups, p, lane);
     tc_fence_before();
@@ -409,61 +411,55 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ 
                     tc_fence_after();
                     const uint32_t at = tmem + lanes_at + (half * 2 + (acc & 1)) * 128;
                     const float2 ff = make_float2(f, f);
-                    float v[2][32];
-                    tmem_ld_row(v[0], at);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        tmem_wait_row(v[i & 1]);
-                        if (i < 3) tmem_ld_row(v[(i + 1) & 1], at + (i + 1) * 32);
-                        else {
+                    for (int i = 0; i < 8; ++i) {
+                        float v[16];
+                        tmem_ld_row(v, at + i * 16);
+                        tmem_wait_row(v);
+                        if (i == 7) {
                             tc_fence_before();
                             __syncwarp();
-                            if (lane == 0) bar_arrive(smem_u32(&ctl.tempty[half][acc & 1]));
+                            if (lane == 0) bar_arrive_tmem(smem_u32(&ctl.tempty[half][acc & 1]));
                         }
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            const float2 r = __ffma2_rn(make_float2(v[i & 1][j], v[i & 1][j + 1]), ff,
-                                                        make_float2(sum[i][j], sum[i][j + 1]));
-                            sum[i][j] = r.x;
-                            sum[i][j + 1] = r.y;
+                        for (int j = 0; j < 16; j += 2) {
+                            float *s = &sum[i >> 1][(i & 1) * 16 + j];
+                            const float2 r = __ffma2_rn(make_float2(v[j], v[j + 1]), ff, make_float2(s[0], s[1]));
+                            s[0] = r.x;
+                            s[1] = r.y;
                         }
                     }
                 }
                 more = walk.next(t);
                 if (more) begin();
-                // 32 rows x 32 features at a time: each thread's row into shared
-                // memory, then 64 contiguous bytes for 4 threads
-                OUT *out = static_cast<OUT *>(p.out) + static_cast<long>(now.row0 + quad * 32) * p.ldo + now.feat0 + half * 128;
+                // Each thread's row into shared memory, and from there as one
+                // asynchronous copy: a tile's 64 KB leave under the next tile's
+                // sums.  (All blocks store at about the same time, and vector
+                // stores held the epilogue up for 5600 clocks a tile.)
+                const int r = quad * 32 + lane;
+                unsigned char *row = stage + lane * kStorePitch;
+                bulk_wait_read();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    if (i * kStoreCols < feats) {
-                        if (!ok) {
+                for (int i = 0; i < 16; ++i) {
+                    float *v = &sum[i >> 2][(i & 3) * 8];
+                    if (!ok) {
 #pragma unroll
-                            for (int j = 0; j < 32; ++j) sum[i][j] = __int_as_float(0x7fffffff);
-                        }
-                        __syncwarp();
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const float *v = &sum[i][8 * q];
-                            *reinterpret_cast<uint4 *>(stage + lane * kStorePitch + q * 16) =
-                                make_uint4(pack<OUT>(v[0], v[1]), pack<OUT>(v[2], v[3]), pack<OUT>(v[4], v[5]), pack<OUT>(v[6], v[7]));
-                        }
-                        __syncwarp();
-                        const int c = i * kStoreCols + (lane & 3) * 8;
-#pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            const int r = q * 8 + (lane >> 2);
-                            if (quad * 32 + r < now.rows && c < feats)
-                                *reinterpret_cast<uint4 *>(out + r * p.ldo + c) =
-                                    *reinterpret_cast<const uint4 *>(stage + r * kStorePitch + (lane & 3) * 16);
-                        }
+                        for (int j = 0; j < 8; ++j) v[j] = __int_as_float(0x7fffffff);
                     }
+                    *reinterpret_cast<uint4 *>(row + i * 16) =
+                        make_uint4(pack<OUT>(v[0], v[1]), pack<OUT>(v[2], v[3]), pack<OUT>(v[4], v[5]), pack<OUT>(v[6], v[7]));
                 }
+                fence_async();
+                if (r < now.rows)
+                    bulk_store(static_cast<OUT *>(p.out) + (now.row0 + r) * p.ldo + now.feat0 + half * 128,
+                               smem_u32(row), feats * sizeof(OUT));
+                bulk_commit();
             } else {
                 more = walk.next(t);
                 if (more) begin();
             }
         }
+        bulk_wait_all();
         // rows of no group are zero
         const int lo = ctl.groups.off[0], hi = ctl.groups.off[p.E];
         const long rows = static_cast<long>(lo) + (p.T - hi);
@@ -494,14 +490,13 @@ cudaError_t launch_many(const Call &c) {
     static std::atomic<bool> ready[kMaxDevices];
     const cudaError_t e = set_up(k, kRowsBytes, kLaunchRegs, ready[dev]);
     if (e != cudaSuccess) return e;
-    const long row_tiles = c.p.T / kRowTile + (c.p.E < c.p.T ? c.p.E : c.p.T);
-    const long tiles = row_tiles * ((c.p.lanes + kFeatTile - 1) / kFeatTile);
-    return launch_on(k, tiles < sms ? tiles : sms, 1, kRowsBytes, c, tw, tx);
+    const long tiles = max_col_tiles<kRowTile>(c) * ((c.p.lanes + kFeatTile - 1) / kFeatTile);
+    return launch_on(k, tiles < sms ? tiles : sms, kThreads, 1, kRowsBytes, c, tw, tx);
 }
 
 template <typename OUT>
 cudaError_t run_mm(const Call &c) {
-    if (c.p.T <= 64) return c.which == kForward ? launch_few<kE4M3, OUT, kForward>(c) : launch_few<kE4M3, OUT, kDgrad>(c);
+    if (few_rows(c)) return c.which == kForward ? launch_few<kE4M3, OUT, kForward>(c) : launch_few<kE4M3, OUT, kDgrad>(c);
     return c.which == kForward ? launch_many<OUT, kForward>(c) : launch_many<OUT, kDgrad>(c);
 }
 

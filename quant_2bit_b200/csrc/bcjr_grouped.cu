@@ -1,6 +1,6 @@
 // Products grouped by expert with ragged sizes, bf16 and fp16 (the kernel and
-// its mathematics: bcjr_mm.cuh).  C entry points bcjr_grouped_mm (forward and
-// the gradient of the rows) and bcjr_grouped_wgrad (gradient of the weights).
+// its mathematics: bcjr_mm.cuh).  C entry points bcjr_grouped_mm and
+// bcjr_grouped_backward (gradients of the rows and of the weights).
 #include "../../include/bcjr_b200.h"
 #include "bcjr_kernels.h"
 #include "bcjr_mm.cuh"
@@ -10,9 +10,9 @@ namespace mm {
 namespace {
 
 template <int KIND, typename T>
-cudaError_t run(const Call &c) {
+cudaError_t launch_which(const Call &c) {
     if (c.which == kWgrad) return launch<KIND, T, kWgrad, 256, 4, false>(c);
-    if (c.p.T <= 64) return c.which == kForward ? launch_few<KIND, T, kForward>(c) : launch_few<KIND, T, kDgrad>(c);
+    if (few_rows(c)) return c.which == kForward ? launch_few<KIND, T, kForward>(c) : launch_few<KIND, T, kDgrad>(c);
     return c.which == kForward ? launch<KIND, T, kForward, 256, 4, false>(c) : launch<KIND, T, kDgrad, 256, 4, false>(c);
 }
 
@@ -28,6 +28,25 @@ int check(const void *offsets, int offsets_bytes, long T, int E, int N, int K, i
     return BCJR_OK;
 }
 
+Call call(const void *offsets, int offsets_bytes, long T, int E, int dtype, int *status,
+          bcjr_stream_t stream) {
+    Call c = {};
+    c.kind = dtype == BCJR_BF16 ? kBF16 : kF16;
+    c.stream = reinterpret_cast<cudaStream_t>(stream);
+    c.p.offsets = offsets;
+    c.p.offsets64 = offsets_bytes == 8;
+    c.p.T = int(T);
+    c.p.E = E;
+    c.p.status = status;
+    c.p.drop = test_option(kOptDropSends);
+    return c;
+}
+
+int run(const Call &c) {
+    const cudaError_t e = c.kind == kBF16 ? launch_which<kBF16, __nv_bfloat16>(c) : launch_which<kF16, __half>(c);
+    return e == cudaSuccess ? BCJR_OK : e == cudaErrorInvalidDevice ? BCJR_ERR_DEVICE : BCJR_ERR_LAUNCH;
+}
+
 }  // namespace
 }  // namespace mm
 }  // namespace bcjr
@@ -36,77 +55,69 @@ using namespace bcjr::mm;
 
 extern "C" {
 
-int bcjr_grouped_mm(const void *rows, long ld_rows, const void *w, const void *offsets,
-                    int offsets_bytes, long T, int E, int N, int K, int dtype, int transpose_w,
-                    void *out, int *status, bcjr_stream_t stream) {
+int bcjr_grouped_mm(const void *x, long ld_x, const void *w, const void *offsets,
+                    int offsets_bytes, long T, int E, int N, int K, int dtype, void *y,
+                    int *status, bcjr_stream_t stream) {
     const int st = check(offsets, offsets_bytes, T, E, N, K, dtype);
     if (st) return st;
     if (T == 0) return BCJR_OK;
-    if (!rows || !w || !out) return BCJR_ERR_NULL_POINTER;
-    const int depth = transpose_w ? N : K, lanes = transpose_w ? K : N;
-    if (ld_rows < depth || ld_rows > (1L << 32)) return BCJR_ERR_BAD_SHAPE;
-    if (!aligned(rows, 16) || ld_rows % 8 || !aligned(w, 16) || !aligned(out, 16) || !aligned(status, 4))
+    if (!x || !w || !y) return BCJR_ERR_NULL_POINTER;
+    if (ld_x < K || ld_x > (1L << 32)) return BCJR_ERR_BAD_SHAPE;
+    if (!aligned(x, 16) || ld_x % 8 || !aligned(w, 16) || !aligned(y, 16) || !aligned(status, 4))
         return BCJR_ERR_ALIGNMENT;
-    Call c = {};
-    c.kind = dtype == BCJR_BF16 ? kBF16 : kF16;
-    c.which = transpose_w ? kDgrad : kForward;
+    Call c = call(offsets, offsets_bytes, T, E, dtype, status, stream);
+    c.which = kForward;
     c.a = w;
     c.a_rows = N;
     c.a_inner = K;
-    c.b = rows;
-    c.ld_b = ld_rows;
-    c.b_inner = depth;
-    c.stream = reinterpret_cast<cudaStream_t>(stream);
-    c.p.offsets = offsets;
-    c.p.offsets64 = offsets_bytes == 8;
-    c.p.T = int(T);
-    c.p.E = E;
-    c.p.lanes = lanes;
-    c.p.depth = depth;
-    c.p.out = out;
-    c.p.ldo = lanes;
-    c.p.status = status;
-    c.p.drop = bcjr::test_option(bcjr::kOptDropSends);
-    const cudaError_t e = c.kind == kBF16 ? run<kBF16, __nv_bfloat16>(c) : run<kF16, __half>(c);
-    return e == cudaSuccess ? BCJR_OK : e == cudaErrorInvalidDevice ? BCJR_ERR_DEVICE : BCJR_ERR_LAUNCH;
+    c.b = x;
+    c.ld_b = ld_x;
+    c.b_inner = c.p.depth = K;
+    c.p.out = y;
+    c.p.ldo = c.p.lanes = N;
+    return run(c);
 }
 
-int bcjr_grouped_wgrad(const void *dy, long ld_dy, const void *x, long ld_x, const void *offsets,
-                       int offsets_bytes, long T, int E, int N, int K, int dtype, void *dw,
-                       int *status, bcjr_stream_t stream) {
-    const int st = check(offsets, offsets_bytes, T, E, N, K, dtype);
+int bcjr_grouped_backward(const void *dy, long ld_dy, const void *x, long ld_x, const void *w,
+                          const void *offsets, int offsets_bytes, long T, int E, int N, int K,
+                          int dtype, void *dx, void *dw, int *status, bcjr_stream_t stream) {
+    int st = check(offsets, offsets_bytes, T, E, N, K, dtype);
     if (st) return st;
-    if (!dw || (T > 0 && (!dy || !x))) return BCJR_ERR_NULL_POINTER;
-    if (T > 0 && (ld_dy < N || ld_x < K || ld_dy > (1L << 32) || ld_x > (1L << 32)))
-        return BCJR_ERR_BAD_SHAPE;
-    if (!aligned(dw, 16) || !aligned(status, 4)) return BCJR_ERR_ALIGNMENT;
-    if (T > 0 && (!aligned(dy, 16) || !aligned(x, 16) || ld_dy % 8 || ld_x % 8)) return BCJR_ERR_ALIGNMENT;
-    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-    if (T == 0)
-        return cudaMemsetAsync(dw, 0, size_t(E) * N * K * 2, s) == cudaSuccess ? BCJR_OK : BCJR_ERR_LAUNCH;
-    Call c = {};
-    c.kind = dtype == BCJR_BF16 ? kBF16 : kF16;
-    c.which = kWgrad;
-    c.a = x;
-    c.ld_a = ld_x;
-    c.a_inner = K;
+    if (T == 0) {
+        cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+        if (dw && cudaMemsetAsync(dw, 0, size_t(E) * N * K * 2, s) != cudaSuccess) return BCJR_ERR_LAUNCH;
+        return BCJR_OK;
+    }
+    if (!dy || (dx && !w) || (dw && !x)) return BCJR_ERR_NULL_POINTER;
+    if (ld_dy < N || ld_dy > (1L << 32) || (dw && (ld_x < K || ld_x > (1L << 32)))) return BCJR_ERR_BAD_SHAPE;
+    if (!aligned(dy, 16) || ld_dy % 8 || !aligned(dx, 16) || !aligned(dw, 16) || !aligned(status, 4) ||
+        (dx && !aligned(w, 16)) || (dw && (!aligned(x, 16) || ld_x % 8)))
+        return BCJR_ERR_ALIGNMENT;
+    Call c = call(offsets, offsets_bytes, T, E, dtype, status, stream);
     c.b = dy;
     c.ld_b = ld_dy;
     c.b_inner = N;
-    c.stream = s;
-    c.p.offsets = offsets;
-    c.p.offsets64 = offsets_bytes == 8;
-    c.p.T = int(T);
-    c.p.E = E;
-    c.p.lanes = K;
-    c.p.cols = N;
-    c.p.out = dw;
-    c.p.ldo = K;
-    c.p.out_group = long(N) * K;
-    c.p.status = status;
-    c.p.drop = bcjr::test_option(bcjr::kOptDropSends);
-    const cudaError_t e = c.kind == kBF16 ? run<kBF16, __nv_bfloat16>(c) : run<kF16, __half>(c);
-    return e == cudaSuccess ? BCJR_OK : e == cudaErrorInvalidDevice ? BCJR_ERR_DEVICE : BCJR_ERR_LAUNCH;
+    c.a_inner = K;
+    c.p.ldo = c.p.lanes = K;
+    if (dx) {
+        c.which = kDgrad;
+        c.a = w;
+        c.a_rows = N;
+        c.p.depth = N;
+        c.p.out = dx;
+        if ((st = run(c))) return st;
+    }
+    if (dw) {
+        c.which = kWgrad;
+        c.a = x;
+        c.ld_a = ld_x;
+        c.p.cols = N;
+        c.p.out = dw;
+        c.p.out_group = long(N) * K;
+        c.p.keep_status = dx != nullptr;       // a failure of the first kernel stays
+        if ((st = run(c))) return st;
+    }
+    return BCJR_OK;
 }
 
 }  // extern "C"

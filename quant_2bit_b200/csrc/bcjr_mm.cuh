@@ -63,6 +63,7 @@ struct Params {
     const float *ws;          // e4m3: weight scales, (group, lane block, contraction block)
     long ws_group, ws_lane, ws_blk;
     int *status;
+    int keep_status;          // a later kernel of one call: the word is not reset
     int drop;                 // test option: the first load of block 0 is withheld
     int dependent;            // launched to overlap the kernel that writes the row matrix
 };
@@ -92,10 +93,26 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 __device__ __forceinline__ void bar_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// For accumulators that have been read (after tcgen05.fence::before_thread_sync,
+// which orders the TMEM loads): nothing else has to be visible.
+__device__ __forceinline__ void bar_arrive_tmem(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
         "{ .reg .pred p; mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;"
+        " selp.u32 %0, 1, 0, p; }"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+// Without waiting for it (try_wait may suspend the thread).
+__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;"
         " selp.u32 %0, 1, 0, p; }"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
@@ -224,26 +241,23 @@ __device__ __forceinline__ void tmem_wait(float (&a)[16], float (&b)[16]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(b[i]));
 }
-// One lane and 32 columns per thread.
-__device__ __forceinline__ void tmem_ld_row(float (&v)[32], uint32_t addr) {
-    uint32_t r[32];
+// One lane and 16 columns per thread.
+__device__ __forceinline__ void tmem_ld_row(float (&v)[16], uint32_t addr) {
+    uint32_t r[16];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
-          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
-          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[14]), "=r"(r[15])
         : "r"(addr));
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
-__device__ __forceinline__ void tmem_wait_row(float (&v)[32]) {
+__device__ __forceinline__ void tmem_wait_row(float (&v)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 32; ++i) asm volatile("" : "+f"(v[i]));
+    for (int i = 0; i < 16; ++i) asm volatile("" : "+f"(v[i]));
 }
 // Four 8 x 8 blocks of 16-bit values, transposed on the way: thread t gives
 // row t / 4, columns 2 (t % 4).. of each; the address of thread 8 m + c
@@ -253,6 +267,22 @@ __device__ __forceinline__ void st_transposed(uint32_t addr, uint32_t a, uint32_
     asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};"
                  ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
+}
+// Asynchronous copy of shared memory to global memory, in a group of this thread.
+__device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t bytes) {
+    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
+                 ::"l"(dst), "r"(src), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void bulk_commit() {
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// This thread's copies have read their source; have been written.
+__device__ __forceinline__ void bulk_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+__device__ __forceinline__ void bulk_wait_all() {
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 // Programmatic dependent launch: the next kernel of the stream may start; the
 // one before has ended and its writes are visible.
@@ -271,9 +301,72 @@ __device__ __forceinline__ void copy4(uint32_t dst, const float *src, bool real)
                  ::"r"(dst), "l"(src), "r"(real ? 4 : 0)
                  : "memory");
 }
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the LEFT youngest groups of this thread's copies have landed.
+template <int LEFT> __device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
 // One arrival of this thread on `bar` when its copies so far have landed.
 __device__ __forceinline__ void copy_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+// Pairs of blocks whose tensor cores work on one tile (cta_group::2): rank 0
+// issues the matrix instructions, each block holds half of either operand and
+// the sums of its half of the lanes.  A load of either block completes on a
+// barrier of rank 0 (its address in the cluster is given); a commit arrives on
+// the same barrier of both.
+__device__ __forceinline__ void pair_expect(uint32_t bar0, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;"
+                 ::"r"(bar0), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void pair_tma2(uint32_t dst, const CUtensorMap *map, int x, int y,
+                                          uint32_t bar0) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3}], [%4];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar0)
+        : "memory");
+}
+__device__ __forceinline__ void pair_tma3(uint32_t dst, const CUtensorMap *map, int x, int y, int z,
+                                          uint32_t bar0) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%2, %3, %4}], [%5];"
+        ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar0)
+        : "memory");
+}
+template <int KIND>
+__device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
+                                         uint32_t accumulate) {
+    if constexpr (KIND == kE4M3)
+        asm volatile(
+            "{ .reg .pred p; setp.ne.b32 p, %4, 0;"
+            " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p; }"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+    else
+        asm volatile(
+            "{ .reg .pred p; setp.ne.b32 p, %4, 0;"
+            " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }"
+            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+            : "memory");
+}
+__device__ __forceinline__ void pair_commit(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
+        ::"r"(bar), "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+__device__ __forceinline__ void pair_tmem_alloc(uint32_t dst, uint32_t cols) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
+                 ::"r"(dst), "r"(cols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void pair_tmem_free(uint32_t addr, uint32_t cols) {
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols)
+                 : "memory");
 }
 // Thread block clusters: own rank, size, id; the address of `addr` in rank r.
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -297,6 +390,10 @@ __device__ __forceinline__ uint32_t in_rank(uint32_t addr, uint32_t r) {
 }
 __device__ __forceinline__ void bar_arrive_in(uint32_t bar, uint32_t r) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_rank(bar, r))
+                 : "memory");
+}
+__device__ __forceinline__ void bar_arrive_tmem_in(uint32_t bar, uint32_t r) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_rank(bar, r))
                  : "memory");
 }
 __device__ __forceinline__ float2 load2_in(uint32_t addr, uint32_t r) {
@@ -334,12 +431,12 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t mn_stri
     return d;
 }
 
-template <int KIND, bool A_MN, bool B_MN>
+template <int KIND, bool A_MN, bool B_MN, int M = kLanes>
 __device__ __forceinline__ uint32_t instr_desc(int n) {
     const uint32_t fmt = KIND == kBF16 ? 1u : 0u;   // f16 0, bf16 1; e4m3 0
     return (1u << 4) | (fmt << 7) | (fmt << 10) | (A_MN ? 1u << 15 : 0u) |
            (B_MN ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) |
-           (static_cast<uint32_t>(kLanes >> 4) << 24);
+           (static_cast<uint32_t>(M >> 4) << 24);
 }
 
 // ---------------------------------------------------------------------------
@@ -358,8 +455,9 @@ __device__ __forceinline__ int col_tiles(int rows) { return (rows + COLS - 1) / 
 
 // Two steps: the whole block reads the bounds, then (after a block barrier)
 // one warp makes them monotone and counts tiles.
+template <int THREADS>
 __device__ __forceinline__ void read_groups(Groups &g, const Params &p) {
-    for (int e = threadIdx.x; e <= p.E; e += kThreads) {
+    for (int e = threadIdx.x; e <= p.E; e += THREADS) {
         long long v;
         if (!p.offsets) v = e == 0 ? 0 : p.T;
         else if (p.offsets64) v = static_cast<const long long *>(p.offsets)[e];
@@ -491,7 +589,7 @@ struct Smem {
     // of the epilogue (one token, 8192 x 2048: 740 clocks a block with two).
     static constexpr int kAcc = KIND == kE4M3 && COLS <= 64 ? 8 : 2;
     struct Ctl {
-        unsigned long long full[STAGES], empty[STAGES], checked[STAGES], tfull[kAcc], tempty[kAcc], done;
+        unsigned long long full[STAGES], empty[STAGES], zeroed[STAGES], tfull[kAcc], tempty[kAcc], done;
         unsigned long long sfull[kScaleStages], sempty[kScaleStages];
         uint32_t tmem;
         int fail;
@@ -613,8 +711,8 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             bar_init(smem_u32(&ctl.full[i]), 1);
-            bar_init(smem_u32(&ctl.empty[i]), 1);
-            bar_init(smem_u32(&ctl.checked[i]), 1);
+            bar_init(smem_u32(&ctl.empty[i]), WHICH == kWgrad ? 2 : 1);
+            bar_init(smem_u32(&ctl.zeroed[i]), 1);
         }
         for (int i = 0; i < ACC; ++i) {
             bar_init(smem_u32(&ctl.tfull[i]), 1);
@@ -628,14 +726,14 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         }
         ctl.fail = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-        if (blockIdx.x == 0 && p.status) *p.status = 0;   // a failure is a second away
+        if (blockIdx.x == 0 && p.status && !p.keep_status) *p.status = 0;   // a failure is a second away
     }
     if (threadIdx.x == 32) {
         prefetch_map(&ta);
         prefetch_map(&tb);
     }
     if (warp == kMmaWarp) tmem_alloc(smem_u32(&ctl.tmem), TMEM_COLS);
-    read_groups(ctl.groups, p);
+    read_groups<kThreads>(ctl.groups, p);
     __syncthreads();
     if (warp == kTmaWarp) scan_groups<COLS>(ctl.groups, p, lane);
     tc_fence_before();
@@ -725,7 +823,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                         if (KIND == kE4M3 || kb == 0)
                             ok = bar_wait(smem_u32(&ctl.tempty[acc % ACC]), ((acc / ACC) & 1) ^ 1, fail, p.status);
                         if (ok)
-                            ok = bar_wait(smem_u32(WHICH == kWgrad ? &ctl.checked[s] : &ctl.full[s]),
+                            ok = bar_wait(smem_u32(WHICH == kWgrad && t.depth - kb * BK < BK ? &ctl.zeroed[s] : &ctl.full[s]),
                                           (it / STAGES) & 1, fail, p.status);
                         if (!ok) break;
                         tc_fence_after();
@@ -746,10 +844,11 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 bar_wait(smem_u32(&ctl.done), 0, &never, nullptr);
             }
         } else if constexpr (WHICH == kWgrad) {
-            // Between the loads and the products one warp sees every stage: the
-            // rows of a group's last one that belong to the next group (or lie
-            // behind the last group) do not count, whatever they hold, and
-            // become zero in both factors.
+            // The rows of a group's last stage that belong to the next group (or
+            // lie behind the last one) do not count, whatever they hold: one
+            // warp makes them zero in both factors before they are multiplied.
+            // It follows every stage, and a stage is loaded again only after it,
+            // so that nobody mistakes a barrier's phase.
             uint32_t it = 0;
             bool ok = warp == kScaleWarp;
             while (ok && walk.next(t)) {
@@ -769,7 +868,10 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                         fence_async();
                         __syncwarp();
                     }
-                    if (lane == 0) bar_arrive(smem_u32(&ctl.checked[s]));
+                    if (lane == 0) {
+                        bar_arrive(smem_u32(&ctl.zeroed[s]));
+                        bar_arrive(smem_u32(&ctl.empty[s]));
+                    }
                 }
             }
         } else if constexpr (KIND == kE4M3) {
@@ -877,7 +979,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
-                        bar_arrive(smem_u32(&ctl.tempty[acc % ACC]));
+                        bar_arrive_tmem(smem_u32(&ctl.tempty[acc % ACC]));
                         bar_arrive(smem_u32(&ctl.sempty[s]));
                     }
                 }
@@ -914,7 +1016,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 if (nkb) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) bar_arrive(smem_u32(&ctl.tempty[acc % ACC]));
+                    if (lane == 0) bar_arrive_tmem(smem_u32(&ctl.tempty[acc % ACC]));
                     ++acc;
                 }
                 if constexpr (SPLIT)
@@ -983,8 +1085,15 @@ bool make_maps(const Call &c, CUtensorMap &ta, CUtensorMap &tb) {
     return make_map(&tb, KIND, 2, c.b, dims, st, box);
 }
 
+// No more column tiles than this can T rows in E groups make.
+template <int COLS>
+long max_col_tiles(const Call &c) {
+    if (c.p.E == 1) return (c.p.T + COLS - 1) / COLS;
+    return c.p.T / COLS + (c.p.E < c.p.T ? c.p.E : c.p.T);
+}
+
 using Kernel = void (*)(CUtensorMap, CUtensorMap, Params);
-inline cudaError_t launch_on(Kernel k, long blocks, int cluster, size_t bytes, const Call &c,
+inline cudaError_t launch_on(Kernel k, long blocks, int threads, int cluster, size_t bytes, const Call &c,
                              const CUtensorMap &ta, const CUtensorMap &tb) {
     if (blocks > 0x7fffffffL) return cudaErrorInvalidValue;
     cudaLaunchAttribute a[2];
@@ -1000,7 +1109,7 @@ inline cudaError_t launch_on(Kernel k, long blocks, int cluster, size_t bytes, c
         ++cfg.numAttrs;
     }
     cfg.gridDim = dim3(unsigned(blocks));
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(unsigned(threads));
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = c.stream;
     cfg.attrs = a;
@@ -1034,21 +1143,21 @@ cudaError_t launch(const Call &c) {
     const cudaError_t e = set_up(k, bytes, 0, ready[dev]);
     if (e != cudaSuccess) return e;
     // no more blocks than there can be tiles
-    const long lane_tiles = (c.p.lanes + kLanes - 1) / kLanes;
-    const long col_tiles = WHICH == kWgrad ? long(c.p.E) * ((c.p.cols + COLS - 1) / COLS)
-                                           : c.p.T / COLS + (c.p.E < c.p.T ? c.p.E : c.p.T);
-    const long tiles = lane_tiles * (col_tiles > 0 ? col_tiles : 1);
-    return launch_on(k, SPLIT ? tiles * c.split : tiles < sms ? tiles : sms, SPLIT ? c.split : 1, bytes, c, ta, tb);
+    const long col_tiles = WHICH == kWgrad ? long(c.p.E) * ((c.p.cols + COLS - 1) / COLS) : max_col_tiles<COLS>(c);
+    const long tiles = (c.p.lanes + kLanes - 1L) / kLanes * col_tiles;
+    return launch_on(k, SPLIT ? tiles * c.split : tiles < sms ? tiles : sms, kThreads, SPLIT ? c.split : 1, bytes, c, ta, tb);
 }
 
-// Forward and dgrad of at most 64 rows: every group is one tile of at most 64
-// columns, and with few tiles the blocks of a cluster share each one.
+// Forward and dgrad with few rows to a group: tiles of 64 columns and eight
+// stages (16 KB of weights each, against 64 KB in all with 256 columns).  With
+// few tiles the blocks of a cluster share each one.
+inline bool few_rows(const Call &c) { return c.p.T <= 64 || c.p.T / 32 <= c.p.E; }
 template <int KIND, typename OUT, int WHICH>
 cudaError_t launch_few(Call c) {
     int dev = 0;
     const int sms = grid_sms(&dev);
     const int nkb = (c.p.depth * (KIND == kE4M3 ? 1 : 2) + kRowBytes - 1) / kRowBytes;
-    const long tiles = (c.p.lanes + kLanes - 1L) / kLanes * (c.p.E < c.p.T ? c.p.E : c.p.T);
+    const long tiles = (c.p.lanes + kLanes - 1L) / kLanes * max_col_tiles<64>(c);
     c.split = 1;
     while (c.split < kMaxSplit && tiles * c.split * 2 <= sms && nkb >= c.split * 2 * 2) c.split *= 2;
     if (c.split == 1) return launch<KIND, OUT, WHICH, 64, 8, false>(c);

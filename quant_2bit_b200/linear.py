@@ -119,39 +119,34 @@ def _bounds(offsets):
 # bf16 / fp16, grouped by expert
 
 
-def _grouped_mm(rows, weight, offsets, transpose):
-    """rows times weight[e]^T, or times weight[e] when ``transpose``."""
+def _grouped_forward(x, weight, offsets):
     E, N, K = weight.shape
-    T = rows.shape[0]
-    out = rows.new_empty((T, K if transpose else N))
+    T = x.shape[0]
+    y = x.new_empty((T, N))
     if T == 0:
-        return out
-    rows, ld = _rows(rows)
+        return y
+    x, ld = _rows(x)
     weight = _dense(weight)
     off_ptr, off_size = _bounds(offsets)
-    _call(_lib.load().bcjr_grouped_mm, rows.get_device(), rows.data_ptr(), ld, weight.data_ptr(),
-          off_ptr, off_size, T, E, N, K, _DTYPES[rows.dtype], transpose, out.data_ptr(), None)
-    return out
-
-
-def _grouped_wgrad(dy, x, offsets, E):
-    (T, N), K = dy.shape, x.shape[1]
-    dw = x.new_empty((E, N, K))
-    dy, ld_dy = _rows(dy)
-    x, ld_x = _rows(x)
-    off_ptr, off_size = _bounds(offsets)
-    _call(_lib.load().bcjr_grouped_wgrad, x.get_device(), dy.data_ptr(), ld_dy, x.data_ptr(), ld_x,
-          off_ptr, off_size, T, E, N, K, _DTYPES[x.dtype], dw.data_ptr(), None)
-    return dw
+    _call(_lib.load().bcjr_grouped_mm, x.get_device(), x.data_ptr(), ld, weight.data_ptr(), off_ptr,
+          off_size, T, E, N, K, _DTYPES[x.dtype], y.data_ptr(), None)
+    return y
 
 
 def _grouped_backward(ctx, dy):
     x, weight, offsets = ctx.saved_tensors
-    dx = dw = None
-    if ctx.needs_input_grad[0]:
-        dx = _grouped_mm(dy, weight, offsets, True)
-    if ctx.needs_input_grad[1]:
-        dw = _grouped_wgrad(dy, x, offsets, weight.shape[0])
+    need_x, need_w, _ = ctx.needs_input_grad
+    E, N, K = weight.shape
+    T = x.shape[0]
+    dx = x.new_empty((T, K)) if need_x else None
+    dw = x.new_empty((E, N, K)) if need_w else None
+    dy, ld_dy = _rows(dy)
+    x, ld_x = _rows(x)
+    weight = _dense(weight)
+    off_ptr, off_size = _bounds(offsets)
+    _call(_lib.load().bcjr_grouped_backward, x.get_device(), dy.data_ptr(), ld_dy, x.data_ptr(), ld_x,
+          weight.data_ptr(), off_ptr, off_size, T, E, N, K, _DTYPES[x.dtype],
+          dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None, None)
     return dx, dw, None
 
 
@@ -159,7 +154,7 @@ class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets):
         ctx.save_for_backward(x, weight, offsets)
-        return _grouped_mm(x, weight, offsets, False)
+        return _grouped_forward(x, weight, offsets)
 
     @staticmethod
     def backward(ctx, dy):
@@ -190,7 +185,7 @@ def grouped_linear(x, weight, offsets):
     offsets = _need_offsets(offsets, weight.shape[0])
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _GroupedLinear.apply(x, weight, offsets)
-    return _grouped_mm(x, weight, offsets, False)
+    return _grouped_forward(x, weight, offsets)
 
 
 # --------------------------------------------------------------------------

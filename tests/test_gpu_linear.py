@@ -98,6 +98,7 @@ GROUPS = [
     ([33], 16, 8208),
     ([0, 64, 0], 528, 512),
     ([7, 33, 0, 64, 12, 1] * 40, 144, 272),        # several tiles and short groups for each block
+    ([90, 0, 3, 1, 20, 0, 0, 0, 2], 80, 208),      # more than 64 rows, few to a group
     ([3, 1, 4, 1, 5, 9, 2, 6, 5, 3, 5, 8, 9, 7, 9, 3] * 5, 32, 96),   # 80 groups
 ]
 
@@ -450,7 +451,8 @@ def test_fp8_linear_forward_and_gradient(cuda_ok, T, N, K, dtype):
 
 @pytest.mark.parametrize("counts,N,K", [([3, 0, 1, 12], 144, 272), ([130, 0, 300, 70], 272, 144),
                                         ([0, 0], 128, 128), ([257, 1], 128, 384),
-                                        ([9, 0, 1], 144, 2064)])
+                                        ([9, 0, 1], 144, 2064),
+                                        ([90, 0, 3, 1, 20, 0, 0, 0, 2], 208, 272)])
 def test_fp8_linear_by_expert(cuda_ok, counts, N, K):
     T = sum(counts) + 6
     x, q, s, w64, dy = _fp8_operands(T, len(counts), N, K, torch.bfloat16, seed=T)
@@ -576,13 +578,16 @@ def test_a_wait_that_runs_out_is_reported(cuda_ok):
     dw = torch.zeros(1, 32, 64, dtype=torch.bfloat16, device="cuda")
     stream = torch.cuda.current_stream().cuda_stream
 
+    dx = torch.zeros(20, 64, dtype=torch.bfloat16, device="cuda")
+
     def forward():
-        return lib.bcjr_grouped_mm(x.data_ptr(), 64, w.data_ptr(), None, 0, 20, 1, 32, 64, 0, 0,
+        return lib.bcjr_grouped_mm(x.data_ptr(), 64, w.data_ptr(), None, 0, 20, 1, 32, 64, 0,
                                    y.data_ptr(), status.data_ptr(), stream)
 
-    def wgrad():
-        return lib.bcjr_grouped_wgrad(dy.data_ptr(), 32, x.data_ptr(), 64, None, 0, 20, 1, 32, 64,
-                                      0, dw.data_ptr(), status.data_ptr(), stream)
+    def backward(rows, weights):
+        return lib.bcjr_grouped_backward(dy.data_ptr(), 32, x.data_ptr(), 64, w.data_ptr(), None, 0, 20,
+                                         1, 32, 64, 0, dx.data_ptr() if rows else None,
+                                         dw.data_ptr() if weights else None, status.data_ptr(), stream)
 
     from quant_2bit_b200 import fp8_quantize_weight
     q, s = fp8_quantize_weight(torch.randn(32, 64, device="cuda"))
@@ -595,7 +600,8 @@ def test_a_wait_that_runs_out_is_reported(cuda_ok):
                                    32, 64, 0, y8.data_ptr(), ws.data_ptr(), ws.numel(),
                                    status.data_ptr(), stream)
 
-    for call, out in ((forward, y), (wgrad, dw), (lambda: fp8(20), y8[:20]), (lambda: fp8(70), y8)):
+    for call, out in ((forward, y), (lambda: backward(1, 0), dx), (lambda: backward(0, 1), dw),
+                      (lambda: backward(1, 1), dw), (lambda: fp8(20), y8[:20]), (lambda: fp8(70), y8)):
         with _lib.test_option(_lib.OPT_TEST_DROP_SENDS, 1):
             assert call() == 0
             assert lib.bcjr_ws_status(ctypes.c_void_p(status.data_ptr()), stream) == _lib.BCJR_ERR_TIMEOUT

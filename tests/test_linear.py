@@ -16,15 +16,14 @@ def lib():
     return _lib.load()
 
 
-def _mm(lib, rows=P, ld=64, w=P, off=P, off_size=4, T=8, E=2, N=32, K=64, dtype=0, tr=0, out=P,
-        status=P):
-    return lib.bcjr_grouped_mm(rows, ld, w, off, off_size, T, E, N, K, dtype, tr, out, status, None)
+def _mm(lib, x=P, ld=64, w=P, off=P, off_size=4, T=8, E=2, N=32, K=64, dtype=0, y=P, status=P):
+    return lib.bcjr_grouped_mm(x, ld, w, off, off_size, T, E, N, K, dtype, y, status, None)
 
 
-def _wgrad(lib, dy=P, ld_dy=32, x=P, ld_x=64, off=P, off_size=4, T=8, E=2, N=32, K=64, dtype=0,
-           dw=P, status=P):
-    return lib.bcjr_grouped_wgrad(dy, ld_dy, x, ld_x, off, off_size, T, E, N, K, dtype, dw, status,
-                                  None)
+def _backward(lib, dy=P, ld_dy=32, x=P, ld_x=64, w=P, off=P, off_size=4, T=8, E=2, N=32, K=64, dtype=0,
+              dx=P, dw=P, status=P):
+    return lib.bcjr_grouped_backward(dy, ld_dy, x, ld_x, w, off, off_size, T, E, N, K, dtype, dx, dw,
+                                     status, None)
 
 
 def _fp8(lib, rows=P, ld=64, xs=P, s_row=1, s_blk=8, w=P, ws=P, off=P, off_size=4, T=8, E=2, N=32,
@@ -33,7 +32,7 @@ def _fp8(lib, rows=P, ld=64, xs=P, s_row=1, s_blk=8, w=P, ws=P, off=P, off_size=
                            dtype, status, None)
 
 
-@pytest.mark.parametrize("call", [_mm, _wgrad, _fp8])
+@pytest.mark.parametrize("call", [_mm, _backward, _fp8])
 def test_products_refuse_bad_sizes(lib, call):
     for bad in (dict(T=-1), dict(T=1 << 31), dict(E=0), dict(E=1025), dict(N=0), dict(N=24),
                 dict(K=8), dict(K=72), dict(off_size=2), dict(off=None), dict(N=1 << 25)):
@@ -43,21 +42,24 @@ def test_products_refuse_bad_sizes(lib, call):
 
 
 def test_products_refuse_bad_pointers_and_strides(lib):
-    assert _mm(lib, T=0, rows=None, out=None, status=None) == OK         # nothing to do
+    assert _mm(lib, T=0, x=None, y=None, status=None) == OK              # nothing to do
+    assert _backward(lib, T=0, dy=None, x=None, dw=None) == OK
     assert _fp8(lib, T=0, rows=None, xs=None, out=None, status=None) == OK
-    for call, names in ((_mm, ("rows", "w", "out")), (_wgrad, ("dy", "x", "dw")),
+    for call, names in ((_mm, ("x", "w", "y")), (_backward, ("dy", "x", "w")),
                         (_fp8, ("rows", "xs", "w", "ws", "out"))):
         for n in names:
             assert call(lib, **{n: None}) == NULL, n
     assert _mm(lib, ld=56) == SHAPE
     assert _mm(lib, ld=68) == ALIGN
-    assert _mm(lib, tr=1, ld=24) == SHAPE
-    assert _mm(lib, rows=P + 8) == ALIGN
+    assert _mm(lib, x=P + 8) == ALIGN
     assert _mm(lib, w=P + 2) == ALIGN
+    assert _mm(lib, y=P + 8) == ALIGN
     assert _mm(lib, off=P + 4, off_size=8) == ALIGN
-    assert _wgrad(lib, ld_dy=16) == SHAPE
-    assert _wgrad(lib, ld_x=68) == ALIGN
-    assert _wgrad(lib, x=P + 8) == ALIGN
+    assert _backward(lib, ld_dy=16) == SHAPE
+    assert _backward(lib, ld_x=48) == SHAPE
+    assert _backward(lib, ld_x=68) == ALIGN
+    assert _backward(lib, dx=P + 8) == _backward(lib, dw=P + 8) == ALIGN
+    assert _backward(lib, w=P + 8) == ALIGN
     assert _fp8(lib, ld=72) == ALIGN
     assert _fp8(lib, s_row=-1) == SHAPE
     assert _fp8(lib, xs=P + 2) == ALIGN
