@@ -78,32 +78,27 @@ __device__ __forceinline__ uint2 to_e4m3(const float (&v)[8], float inv) {
     return make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
 }
 
-constexpr int kQThreads = 256, kUnroll = 4;
+constexpr int kQThreads = 256, kUnroll = 4, kQRows = kQThreads / 16;
 
-// 16 lanes per segment, 8 elements per lane (the width is a multiple of 16);
-// kUnroll segments of a thread are loaded before the first is used.
+// 16 lanes per segment, 8 elements per lane (the width is a multiple of 16).
+// A block has 16 rows and kUnroll neighbouring segments of each, all loaded
+// before the first is used; the scales of a column of segments, side by side
+// when they are stored block by block, leave together.
 template <typename T>
 __global__ void __launch_bounds__(kQThreads)
 quantize_rows(const T *__restrict__ x, long ld, long rows, int k, uint8_t *__restrict__ q,
               float *__restrict__ scale, long s_row, long s_blk) {
     let_next_start();              // the product's set-up may overlap (it waits for this kernel's end)
-    const int nb = (k + 127) / 128, sub = threadIdx.x & 15;
-    constexpr int groups = kQThreads / 16;
+    const int sub = threadIdx.x & 15, blk0 = blockIdx.y * kUnroll;
+    const long row = long(blockIdx.x) * kQRows + (threadIdx.x >> 4);
+    const bool live = row < rows;
     float v[kUnroll][8];
-    long row[kUnroll];
-    int blk[kUnroll];
-    // segments threadIdx / 16, + groups, ..  of the block's: one 64-bit division
-    // for the block, 32-bit ones for its threads
-    const long base = long(blockIdx.x) * (groups * kUnroll), row0 = base / nb;
-    const unsigned blk0 = unsigned(base - row0 * nb);
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-        const unsigned s = blk0 + u * groups + (threadIdx.x >> 4), r = s / unsigned(nb);
-        row[u] = row0 + r;
-        blk[u] = int(s - r * nb);
+        const int c = (blk0 + u) * 128 + sub * 8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[u][i] = 0.f;
-        if (row[u] < rows && blk[u] * 128 + sub * 8 < k) load8(x + row[u] * ld + blk[u] * 128 + sub * 8, v[u]);
+        if (live && c < k) load8(x + row * ld + c, v[u]);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
@@ -111,10 +106,9 @@ quantize_rows(const T *__restrict__ x, long ld, long rows, int k, uint8_t *__res
 #pragma unroll
         for (int d = 8; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
         m = block_amax(m);
-        if (row[u] >= rows) continue;
-        const int c = blk[u] * 128 + sub * 8;
-        if (c < k) *reinterpret_cast<uint2 *>(q + row[u] * k + c) = to_e4m3(v[u], block_inv(m));
-        if (sub == 0) scale[row[u] * s_row + blk[u] * s_blk] = block_scale(m);
+        const int c = (blk0 + u) * 128 + sub * 8;
+        if (live && c < k) *reinterpret_cast<uint2 *>(q + row * k + c) = to_e4m3(v[u], block_inv(m));
+        if (live && sub == 0 && c < k) scale[row * s_row + (blk0 + u) * s_blk] = block_scale(m);
     }
 }
 
@@ -157,8 +151,8 @@ quantize_blocks(const T *__restrict__ w, int n, int k, uint8_t *__restrict__ q,
 template <typename T>
 cudaError_t run_rows(const void *x, long ld, long rows, int k, void *q, float *scale, long s_row,
                      long s_blk, cudaStream_t st) {
-    const long per = long(kQThreads / 16) * kUnroll, segs = rows * ((k + 127) / 128);
-    quantize_rows<T><<<unsigned((segs + per - 1) / per), kQThreads, 0, st>>>(
+    const dim3 grid(unsigned((rows + kQRows - 1) / kQRows), unsigned(((k + 127) / 128 + kUnroll - 1) / kUnroll));
+    quantize_rows<T><<<grid, kQThreads, 0, st>>>(
         static_cast<const T *>(x), ld, rows, k, static_cast<uint8_t *>(q), scale, s_row, s_blk);
     return cudaGetLastError();
 }
@@ -460,13 +454,7 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ 
             }
         }
         bulk_wait_all();
-        // rows of no group are zero
-        const int lo = ctl.groups.off[0], hi = ctl.groups.off[p.E];
-        const long rows = static_cast<long>(lo) + (p.T - hi);
-        for (long r = blockIdx.x; r < rows; r += gridDim.x) {
-            OUT *o = static_cast<OUT *>(p.out) + (r < lo ? r : r - lo + hi) * p.ldo;
-            for (int f = threadIdx.x; f < p.lanes; f += kEpiWarps * 32) o[f] = from_float<OUT>(0.f);
-        }
+        zero_other_rows<OUT>(ctl.groups, p);
     }
     __syncwarp();
     tc_fence_before();
@@ -524,7 +512,6 @@ int bcjr_fp8_quantize_rows(const void *x, long ld, long rows, int k, int dtype, 
     if (!x || !q || !scale) return BCJR_ERR_NULL_POINTER;
     if (!aligned(x, 16) || ld % (dtype == BCJR_F32 ? 4 : 8) || !aligned(q, 8) || !aligned(scale, 4))
         return BCJR_ERR_ALIGNMENT;
-    if (rows * ((k + 127L) / 128) > (1L << 36)) return BCJR_ERR_BAD_SHAPE;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     switch (dtype) {
         case BCJR_BF16: return status_of(run_rows<__nv_bfloat16>(x, ld, rows, k, q, scale, scale_row, scale_block, st));

@@ -9,11 +9,22 @@ namespace bcjr {
 namespace mm {
 namespace {
 
+// Many features: two blocks to a tile of 256 lanes; else one block to 128.  (64
+// experts, 32768 rows, 1024 and 2048 features: 113 us forward, 115 and 139 us
+// gradients in pairs, 125, 125 and 157 us alone.  4 experts, 3000 rows, 1040
+// features: the same.  96 experts, 3079 rows, 272 features, weights' gradient:
+// 27 us in pairs, 20 alone: 272 lanes are two tiles of 256 but three of 128.)
+template <int KIND, typename T, int WHICH>
+cudaError_t launch_many(const Call &c) {
+    if (c.p.lanes >= 1024) return launch<KIND, T, WHICH, 256, 6, kPair>(c);
+    return launch<KIND, T, WHICH, 256, 4, kAlone>(c);
+}
+
 template <int KIND, typename T>
 cudaError_t launch_which(const Call &c) {
-    if (c.which == kWgrad) return launch<KIND, T, kWgrad, 256, 4, false>(c);
+    if (c.which == kWgrad) return launch_many<KIND, T, kWgrad>(c);
     if (few_rows(c)) return c.which == kForward ? launch_few<KIND, T, kForward>(c) : launch_few<KIND, T, kDgrad>(c);
-    return c.which == kForward ? launch<KIND, T, kForward, 256, 4, false>(c) : launch<KIND, T, kDgrad, 256, 4, false>(c);
+    return c.which == kForward ? launch_many<KIND, T, kForward>(c) : launch_many<KIND, T, kDgrad>(c);
 }
 
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }

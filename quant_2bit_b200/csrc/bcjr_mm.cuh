@@ -35,6 +35,9 @@ namespace mm {
 
 enum { kBF16 = 0, kF16 = 1, kE4M3 = 2 };          // element type of A and B
 enum { kForward = 0, kDgrad = 1, kWgrad = 2 };    // which product
+// Blocks to a tile: one; several that share its contraction (few rows); two
+// that share its products (many rows).
+enum { kAlone = 0, kSplit = 1, kPair = 2 };
 
 constexpr int kLanes = 128;                       // M of the matrix instruction
 constexpr int kRowBytes = 128;                    // one swizzled shared-memory row
@@ -133,9 +136,10 @@ __device__ __forceinline__ bool bar_try_cluster(uint32_t bar, uint32_t parity) {
 // Bounded wait (about 1 s).  False when it gave up or another warp of the
 // block did; the block then finishes with NaN outputs and the status word
 // says BCJR_ERR_TIMEOUT.
+// `stages` of products, at well under 4096 clocks each, are waited for.
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int *fail,
-                                         int *status) {
+                                         int *status, int stages = 0) {
     auto test = [&] { return CLUSTER ? bar_try_cluster(bar, parity) : bar_try(bar, parity); };
     if (test()) return true;
     const long long t0 = clock64();
@@ -143,7 +147,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
         for (int i = 0; i < 32; ++i)
             if (test()) return true;
         if (*fail) return false;
-        if (clock64() - t0 > kWaitLimitClocks) {
+        if (clock64() - t0 > kWaitLimitClocks + 4096ll * stages) {
             *fail = 1;
             if (status) atomicExch(status, 8 /* BCJR_ERR_TIMEOUT */);
             return false;
@@ -155,8 +159,8 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
 // 5 % slower.)
 template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int *fail,
-                                          int *status) {
-    return __all_sync(0xffffffffu, bar_wait<CLUSTER>(bar, parity, fail, status));
+                                          int *status, int stages = 0) {
+    return __all_sync(0xffffffffu, bar_wait<CLUSTER>(bar, parity, fail, status, stages));
 }
 __device__ __forceinline__ void tma2(uint32_t dst, const CUtensorMap *map, int x, int y,
                                      uint32_t bar) {
@@ -315,8 +319,10 @@ __device__ __forceinline__ void copy_arrive(uint32_t bar) {
 // the sums of its half of the lanes.  A load of either block completes on a
 // barrier of rank 0 (its address in the cluster is given); a commit arrives on
 // the same barrier of both.
+// (Relaxed: the thread has written nothing that others read, and a release at
+// cluster scope for every stage took longer than the stage's products.)
 __device__ __forceinline__ void pair_expect(uint32_t bar0, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.release.cluster.shared::cluster.b64 _, [%0], %1;"
+    asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;"
                  ::"r"(bar0), "r"(bytes)
                  : "memory");
 }
@@ -358,6 +364,10 @@ __device__ __forceinline__ void pair_commit(uint32_t bar) {
         ::"r"(bar), "h"(static_cast<uint16_t>(3))
         : "memory");
 }
+template <bool PAIR> __device__ __forceinline__ void commit(uint32_t bar) {
+    if constexpr (PAIR) pair_commit(bar);
+    else mma_commit(bar);
+}
 __device__ __forceinline__ void pair_tmem_alloc(uint32_t dst, uint32_t cols) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                  ::"r"(dst), "r"(cols)
@@ -392,7 +402,7 @@ __device__ __forceinline__ void bar_arrive_in(uint32_t bar, uint32_t r) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_rank(bar, r))
                  : "memory");
 }
-__device__ __forceinline__ void bar_arrive_tmem_in(uint32_t bar, uint32_t r) {
+__device__ __forceinline__ void bar_arrive_relaxed_in(uint32_t bar, uint32_t r) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_rank(bar, r))
                  : "memory");
 }
@@ -465,34 +475,35 @@ __device__ __forceinline__ void read_groups(Groups &g, const Params &p) {
         g.off[e] = v < 0 ? 0 : v > p.T ? p.T : static_cast<int>(v);
     }
 }
+// Every lane has a run of neighbouring bounds, so one pass over the warp joins
+// them (lane by lane, a layer of 64 experts took three).
 template <int COLS>
 __device__ __forceinline__ void scan_groups(Groups &g, const Params &p, int lane) {
-    int high = 0, tiles = 0;        // last bound and tile count of the chunk before
-    for (int base = 0; base <= p.E; base += 32) {
-        const int e = base + lane;
-        int o = e <= p.E ? g.off[e] : 0;
-        if (o < high) o = high;
+    const int run = (p.E + 32) / 32, lo = lane * run, hi = min(lo + run, p.E + 1);
+    int top = 0;
+    for (int e = lo; e < hi; ++e) top = max(top, g.off[e]);
 #pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, o, d);
-            if (lane >= d && u > o) o = u;
-        }
-        int prev = __shfl_up_sync(0xffffffffu, o, 1);
-        if (lane == 0) prev = high;
-        // tiles of group e - 1, which ends at this bound
-        int n = (e >= 1 && e <= p.E) ? col_tiles<COLS>(o - prev) : 0;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, n, d);
-            if (lane >= d) n += u;
-        }
-        if (e <= p.E) {
-            g.off[e] = o;
-            g.first[e] = tiles + n;
-        }
-        high = __shfl_sync(0xffffffffu, o, 31);
-        tiles += __shfl_sync(0xffffffffu, n, 31);
+    for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, top, d);
+        if (lane >= d) top = max(top, u);
     }
+    int before = __shfl_up_sync(0xffffffffu, top, 1);     // the largest bound of the lanes before
+    if (lane == 0) before = 0;
+    int o = before, tiles = 0;
+    for (int e = lo; e < hi; ++e) {
+        const int next = max(o, g.off[e]);
+        // tiles of group e - 1, which ends at this bound
+        if (e > 0) tiles += col_tiles<COLS>(next - o);
+        g.off[e] = o = next;
+        g.first[e] = tiles;
+    }
+    int sum = tiles;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += u;
+    }
+    for (int e = lo; e < hi; ++e) g.first[e] += sum - tiles;
 }
 
 struct Tile {
@@ -500,28 +511,32 @@ struct Tile {
     int lane_tile;
     int col0;       // first output row (forward, dgrad: row of X; wgrad: n)
     int valid;      // columns to write
-    int ncols;      // columns computed, a multiple of 16
+    int ncols;      // columns computed, a multiple of 16 (of 32 by a pair)
     int k0;         // first contraction index (wgrad: row of X)
     int depth;      // contraction length from k0 on
     int nkb;        // its stages (0: the output is zero)
 };
 
 // The tiles of a block, one after the other; every warp walks the same list.
-// SPLIT: the blocks of a cluster share each tile, every one with its part of
-// the contraction.
-template <int WHICH, int COLS, int BK, bool SPLIT>
+// kSplit: the blocks of a cluster share each tile, every one with its part of
+// the contraction.  kPair: two blocks have the halves of 256 lanes.
+template <int WHICH, int COLS, int BK, int MODE>
 struct Walk {
+    static constexpr bool SPLIT = MODE == kSplit;
+    static constexpr int LANES = MODE == kPair ? 2 * kLanes : kLanes;
+    static constexpr int STEP = MODE == kPair ? 32 : 16;     // of the columns' number
     const Groups &g;
     const Params &p;
     int lane_tiles, total, tile, step, group, part, parts;
     __device__ Walk(const Groups &g_, const Params &p_) : g(g_), p(p_) {
         parts = SPLIT ? cluster_size() : 1;
         part = SPLIT ? cluster_rank() : 0;
-        step = gridDim.x / parts;
-        lane_tiles = (p.lanes + kLanes - 1) / kLanes;
+        const int blocks = MODE == kPair ? 2 : parts;
+        step = gridDim.x / blocks;
+        lane_tiles = (p.lanes + LANES - 1) / LANES;
         total = WHICH == kWgrad ? p.E * lane_tiles * col_tiles<COLS>(p.cols)
                                 : g.first[p.E] * lane_tiles;
-        tile = blockIdx.x / parts;
+        tile = blockIdx.x / blocks;
         group = 0;
     }
     __device__ bool next(Tile &t) {
@@ -533,7 +548,7 @@ struct Walk {
             t.lane_tile = in / ct;
             t.col0 = (in - t.lane_tile * ct) * COLS;
             t.valid = min(COLS, p.cols - t.col0);
-            t.ncols = t.valid;               // cols is a multiple of 16
+            t.ncols = (t.valid + STEP - 1) & ~(STEP - 1);
             t.k0 = g.off[t.group];
             t.depth = g.off[t.group + 1] - t.k0;
             t.nkb = (t.depth + BK - 1) / BK;
@@ -546,10 +561,10 @@ struct Walk {
             const int c = in - t.lane_tile * ct;
             const int rows = g.off[group + 1] - g.off[group];
             // equal shares: no small tile at the end of a group
-            const int share = ((rows + ct - 1) / ct + 15) & ~15;
+            const int share = ((rows + ct - 1) / ct + STEP - 1) & ~(STEP - 1);
             t.col0 = g.off[group] + c * share;
             t.valid = min(share, g.off[group + 1] - t.col0);
-            t.ncols = (t.valid + 15) & ~15;
+            t.ncols = (t.valid + STEP - 1) & ~(STEP - 1);
             const int nkb = (p.depth + BK - 1) / BK;
             const int kb0 = SPLIT ? nkb * part / parts : 0;
             t.nkb = (SPLIT ? nkb * (part + 1) / parts : nkb) - kb0;
@@ -561,9 +576,6 @@ struct Walk {
     }
 };
 
-template <typename T> __device__ __forceinline__ T from_float(float v);
-template <> __device__ __forceinline__ __nv_bfloat16 from_float(float v) { return __float2bfloat16_rn(v); }
-template <> __device__ __forceinline__ __half from_float(float v) { return __float2half_rn(v); }
 template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b);
 template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
@@ -574,14 +586,27 @@ template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
+// Rows of no group (before the first, behind the last) are zero: all threads
+// of all epilogues.
+template <typename OUT>
+__device__ __forceinline__ void zero_other_rows(const Groups &g, const Params &p) {
+    const int lo = g.off[0], hi = g.off[p.E];
+    const long rows = static_cast<long>(lo) + (p.T - hi);
+    for (long r = blockIdx.x; r < rows; r += gridDim.x) {
+        uint4 *o = reinterpret_cast<uint4 *>(static_cast<OUT *>(p.out) + (r < lo ? r : r - lo + hi) * p.ldo);
+        for (int f = threadIdx.x; f < p.lanes / 8; f += kEpiWarps * 32) o[f] = make_uint4(0, 0, 0, 0);
+    }
+}
+
 constexpr int kScaleStages = 8;
 constexpr int kPartPitch = kLanes + 4;            // floats: no bank conflicts either way
 
 
-template <int KIND, int COLS, int STAGES, bool SPLIT>
+template <int KIND, int COLS, int STAGES, int MODE>
 struct Smem {
+    static constexpr bool SPLIT = MODE == kSplit;
     static constexpr int kA = kLanes * kRowBytes;
-    static constexpr int kB = COLS * kRowBytes;
+    static constexpr int kB = COLS * kRowBytes / (MODE == kPair ? 2 : 1);
     static constexpr int kStage = kA + kB;
     static constexpr int kScales = KIND == kE4M3 ? kScaleStages : 1;
     // accumulator buffers.  16-bit types use one for a tile, e4m3 one for a k
@@ -681,11 +706,12 @@ __device__ __forceinline__ bool add_parts(const float (&v)[2][16], float (*part)
 }
 
 // KIND: element type; OUT: output type; WHICH: product; COLS: columns of a
-// tile; STAGES: depth of the shared-memory ring; SPLIT: clusters share tiles.
-template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, bool SPLIT>
+// tile; STAGES: depth of the shared-memory ring; MODE: blocks to a tile.
+template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, int MODE>
 __global__ void __launch_bounds__(kThreads, 1)
 mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
           const __grid_constant__ Params p) {
+    constexpr bool SPLIT = MODE == kSplit, PAIR = MODE == kPair;
     constexpr bool A_MN = WHICH != kForward, B_MN = WHICH == kWgrad;
     constexpr int ESIZE = KIND == kE4M3 ? 1 : 2;
     constexpr int BK = kRowBytes / ESIZE;             // contraction per stage
@@ -696,27 +722,31 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     constexpr uint32_t A_STEP = A_MN ? KSLICE * kRowBytes : 32;
     constexpr uint32_t B_STEP = B_MN ? KSLICE * kRowBytes : 32;
     constexpr uint32_t MN_BLOCK = BK * kRowBytes;     // an MN-major block of BK rows
-    using S = Smem<KIND, COLS, STAGES, SPLIT>;
+    using S = Smem<KIND, COLS, STAGES, MODE>;
     constexpr uint32_t ACC = S::kAcc, TMEM_COLS = ACC * COLS;
     static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0 && TMEM_COLS >= 32, "");
     static_assert(!(KIND == kE4M3 && WHICH == kWgrad), "e4m3 has forward and dgrad");
-    static_assert(BK % kBoxRows == 0 && COLS % 16 == 0, "");
+    static_assert(BK % kBoxRows == 0 && COLS % 32 == 0, "");
+    static_assert(!PAIR || KIND != kE4M3, "pairs: 16-bit types");
 
     extern __shared__ unsigned char raw[];
     unsigned char *buf = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     typename S::Ctl &ctl = *reinterpret_cast<typename S::Ctl *>(buf + size_t(STAGES) * S::kStage);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = PAIR ? cluster_rank() : 0;
     volatile int *fail = &ctl.fail;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            bar_init(smem_u32(&ctl.full[i]), 1);
-            bar_init(smem_u32(&ctl.empty[i]), WHICH == kWgrad ? 2 : 1);
-            bar_init(smem_u32(&ctl.zeroed[i]), 1);
+            // a pair's rank 0 is told by both: by their loads (full), or for the
+            // weights' gradient by the warps that zero (zeroed)
+            bar_init(smem_u32(&ctl.full[i]), PAIR && !B_MN ? 2 : 1);
+            bar_init(smem_u32(&ctl.empty[i]), B_MN && !PAIR ? 2 : 1);
+            bar_init(smem_u32(&ctl.zeroed[i]), PAIR ? 2 : 1);
         }
         for (int i = 0; i < ACC; ++i) {
             bar_init(smem_u32(&ctl.tfull[i]), 1);
-            bar_init(smem_u32(&ctl.tempty[i]), kEpiWarps);
+            bar_init(smem_u32(&ctl.tempty[i]), PAIR ? 2 * kEpiWarps : kEpiWarps);
         }
         bar_init(smem_u32(&ctl.done), 1);
         if constexpr (SPLIT) bar_init(smem_u32(&ctl.pfull), kEpiWarps * cluster_size());
@@ -732,16 +762,19 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         prefetch_map(&ta);
         prefetch_map(&tb);
     }
-    if (warp == kMmaWarp) tmem_alloc(smem_u32(&ctl.tmem), TMEM_COLS);
+    if (warp == kMmaWarp) {
+        if constexpr (PAIR) pair_tmem_alloc(smem_u32(&ctl.tmem), TMEM_COLS);
+        else tmem_alloc(smem_u32(&ctl.tmem), TMEM_COLS);
+    }
     read_groups<kThreads>(ctl.groups, p);
     __syncthreads();
     if (warp == kTmaWarp) scan_groups<COLS>(ctl.groups, p, lane);
     tc_fence_before();
-    if constexpr (SPLIT) cluster_sync();
+    if constexpr (MODE != kAlone) cluster_sync();
     else __syncthreads();
     tc_fence_after();
     const uint32_t tmem = ctl.tmem;
-    Walk<WHICH, COLS, BK, SPLIT> walk(ctl.groups, p);
+    Walk<WHICH, COLS, BK, MODE> walk(ctl.groups, p);
     Tile t;
 
     if (warp >= kEpiWarps) {
@@ -750,28 +783,40 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             if (elect_one()) {
                 uint32_t it = 0, ahead = 0;
                 bool ok = true;
+                // This block's part of the lanes and of the columns, and the
+                // barrier that its loads complete on.
+                auto lanes_at = [&](const Tile &t) { return t.lane_tile * walk.LANES + int(rank) * kLanes; };
+                auto cols = [&](const Tile &t) { return PAIR ? t.ncols / 2 : t.ncols; };
+                auto full = [&](uint32_t s) {
+                    const uint32_t bar = smem_u32(&ctl.full[s]);
+                    return PAIR && !B_MN ? in_rank(bar, 0) : bar;
+                };
                 // Arms the stage's barrier for both operands and loads the one
                 // that has the output's lanes.
                 auto load_a = [&](const Tile &t, int kb, uint32_t s) {
-                    const uint32_t bar = smem_u32(&ctl.full[s]), a = smem_u32(buf + s * S::kStage);
-                    const int bboxes = B_MN ? (t.ncols + MNB - 1) / MNB : (t.ncols + kBoxRows - 1) / kBoxRows;
+                    const uint32_t bar = full(s), a = smem_u32(buf + s * S::kStage);
+                    const int boxes = (cols(t) + (B_MN ? MNB : kBoxRows) - 1) / (B_MN ? MNB : kBoxRows);
                     const int kc = t.k0 + kb * BK;
-                    bar_expect(bar, S::kA + bboxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes));
+                    const uint32_t bytes = S::kA + boxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes);
+                    if constexpr (PAIR && !B_MN) pair_expect(bar, bytes);
+                    else bar_expect(bar, bytes);
                     if constexpr (WHICH == kForward) {
-                        tma3(a, &ta, kc, t.lane_tile * kLanes, t.group, bar);
+                        if constexpr (PAIR) pair_tma3(a, &ta, kc, lanes_at(t), t.group, bar);
+                        else tma3(a, &ta, kc, lanes_at(t), t.group, bar);
                     } else {
 #pragma unroll
                         for (int j = 0; j < kLanes / MNB; ++j) {
-                            const int x = t.lane_tile * kLanes + j * MNB;
-                            if constexpr (WHICH == kDgrad) tma3(a + j * MN_BLOCK, &ta, x, kc, t.group, bar);
-                            else tma2(a + j * MN_BLOCK, &ta, x, kc, bar);
+                            const int x = lanes_at(t) + j * MNB;
+                            if constexpr (WHICH == kWgrad) tma2(a + j * MN_BLOCK, &ta, x, kc, bar);
+                            else if constexpr (PAIR) pair_tma3(a + j * MN_BLOCK, &ta, x, kc, t.group, bar);
+                            else tma3(a + j * MN_BLOCK, &ta, x, kc, t.group, bar);
                         }
                     }
                 };
                 const bool drop = p.drop && blockIdx.x == 0;      // test option: the first load is withheld
                 if (p.dependent) {
                     // the weights do not come from the kernel before this one
-                    Walk<WHICH, COLS, BK, SPLIT> first = walk;
+                    Walk<WHICH, COLS, BK, MODE> first = walk;
                     if (first.next(t))
                         for (; ahead < STAGES && ahead < t.nkb; ++ahead)
                             if (!drop || ahead) load_a(t, ahead, ahead);
@@ -788,26 +833,27 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                             if (!drop || it) load_a(t, kb, s);
                         }
                         if (drop && it == 0) continue;
-                        const uint32_t bar = smem_u32(&ctl.full[s]), b = smem_u32(buf + s * S::kStage) + S::kA;
-                        const int kc = t.k0 + kb * BK;
+                        const uint32_t bar = full(s), b = smem_u32(buf + s * S::kStage) + S::kA;
+                        const int kc = t.k0 + kb * BK, n = cols(t), c = t.col0 + int(rank) * n;
                         if constexpr (B_MN) {
-                            for (int j = 0; j * MNB < t.ncols; ++j)
-                                tma2(b + j * MN_BLOCK, &tb, t.col0 + j * MNB, kc, bar);
+                            for (int j = 0; j * MNB < n; ++j) tma2(b + j * MN_BLOCK, &tb, c + j * MNB, kc, bar);
                         } else {
-                            for (int j = 0; j * kBoxRows < t.ncols; ++j)
-                                tma2(b + j * kBoxRows * kRowBytes, &tb, kc, t.col0 + j * kBoxRows, bar);
+                            for (int j = 0; j * kBoxRows < n; ++j) {
+                                if constexpr (PAIR) pair_tma2(b + j * kBoxRows * kRowBytes, &tb, kc, c + j * kBoxRows, bar);
+                                else tma2(b + j * kBoxRows * kRowBytes, &tb, kc, c + j * kBoxRows, bar);
+                            }
                         }
                     }
                 }
-                if (!ok) {
-                    // copies in flight land before the block ends
+                if (!ok && (rank == 0 || B_MN)) {
+                    // copies in flight land before the block (the pair) ends
                     volatile int never = 0;
                     for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
                         if (!(drop && i == 0))
-                            bar_wait(smem_u32(&ctl.full[i % STAGES]), (i / STAGES) & 1, &never, nullptr);
+                            bar_wait<PAIR>(smem_u32(&ctl.full[i % STAGES]), (i / STAGES) & 1, &never, nullptr);
                 }
             }
-        } else if (warp == kMmaWarp) {
+        } else if (warp == kMmaWarp && rank == 0) {
             // MMA issuer: one thread runs the whole loop (a warp that elected a
             // thread and met again for every stage took 220 clocks more for it)
             if (elect_one()) {
@@ -815,40 +861,49 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 bool ok = true;
                 while (ok && walk.next(t)) {
                     if (t.nkb == 0) continue;
-                    const uint32_t idesc = instr_desc<KIND, A_MN, B_MN>(t.ncols);
+                    const uint32_t idesc = instr_desc<KIND, A_MN, B_MN, decltype(walk)::LANES>(t.ncols);
                     for (int kb = 0; kb < t.nkb; ++kb, ++it) {
                         const uint32_t s = it % STAGES;
                         // e4m3: every stage has an accumulator buffer of its own
                         // (scaled and added in fp32 registers); otherwise every tile
                         if (KIND == kE4M3 || kb == 0)
-                            ok = bar_wait(smem_u32(&ctl.tempty[acc % ACC]), ((acc / ACC) & 1) ^ 1, fail, p.status);
+                            ok = bar_wait<PAIR>(smem_u32(&ctl.tempty[acc % ACC]), ((acc / ACC) & 1) ^ 1, fail, p.status);
                         if (ok)
-                            ok = bar_wait(smem_u32(WHICH == kWgrad && t.depth - kb * BK < BK ? &ctl.zeroed[s] : &ctl.full[s]),
-                                          (it / STAGES) & 1, fail, p.status);
+                            ok = bar_wait<PAIR>(smem_u32(B_MN && (PAIR || t.depth - kb * BK < BK) ? &ctl.zeroed[s] : &ctl.full[s]),
+                                                (it / STAGES) & 1, fail, p.status);
                         if (!ok) break;
                         tc_fence_after();
                         const uint32_t a = smem_u32(buf + s * S::kStage);
                         const uint64_t da = operand_desc(a, MN_BLOCK), db = operand_desc(a + S::kA, MN_BLOCK);
                         const uint32_t d = tmem + (acc % ACC) * COLS;
 #pragma unroll
-                        for (int j = 0; j < SLICES; ++j)
-                            mma<KIND>(d, da + ((j * A_STEP) >> 4), db + ((j * B_STEP) >> 4), idesc,
-                                      (KIND == kE4M3 ? j > 0 : (kb | j) > 0) ? 1u : 0u);
-                        if (KIND == kE4M3 || kb == t.nkb - 1) mma_commit(smem_u32(&ctl.tfull[acc++ % ACC]));
-                        mma_commit(smem_u32(&ctl.empty[s]));
+                        for (int j = 0; j < SLICES; ++j) {
+                            const uint64_t aj = da + ((j * A_STEP) >> 4), bj = db + ((j * B_STEP) >> 4);
+                            const uint32_t add = (KIND == kE4M3 ? j > 0 : (kb | j) > 0) ? 1u : 0u;
+                            if constexpr (PAIR) pair_mma<KIND>(d, aj, bj, idesc, add);
+                            else mma<KIND>(d, aj, bj, idesc, add);
+                        }
+                        if (KIND == kE4M3 || kb == t.nkb - 1) commit<PAIR>(smem_u32(&ctl.tfull[acc++ % ACC]));
+                        commit<PAIR>(smem_u32(&ctl.empty[s]));
                     }
                 }
                 // every matrix instruction has ended before the block frees its TMEM
-                mma_commit(smem_u32(&ctl.done));
+                commit<PAIR>(smem_u32(&ctl.done));
                 volatile int never = 0;
                 bar_wait(smem_u32(&ctl.done), 0, &never, nullptr);
             }
+        } else if (PAIR && warp == kMmaWarp) {
+            // rank 1 stays until the last arrival from rank 0 is here (asked now
+            // and then: the epilogue needs the issue slots)
+            for (const long long t0 = clock64(); !bar_test(smem_u32(&ctl.done), 0) && clock64() - t0 < kWaitLimitClocks;)
+                __nanosleep(1000);
         } else if constexpr (WHICH == kWgrad) {
             // The rows of a group's last stage that belong to the next group (or
             // lie behind the last one) do not count, whatever they hold: one
             // warp makes them zero in both factors before they are multiplied.
             // It follows every stage, and a stage is loaded again only after it,
-            // so that nobody mistakes a barrier's phase.
+            // so that nobody mistakes a barrier's phase.  In a pair both blocks'
+            // warps tell rank 0 of every stage.
             uint32_t it = 0;
             bool ok = warp == kScaleWarp;
             while (ok && walk.next(t)) {
@@ -856,11 +911,11 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                     const uint32_t s = it % STAGES;
                     ok = warp_wait(smem_u32(&ctl.full[s]), (it / STAGES) & 1, fail, p.status);
                     if (!ok) break;
-                    const int rows = t.depth - kb * BK;
+                    const int rows = t.depth - kb * BK, n = PAIR ? t.ncols / 2 : t.ncols;
                     if (rows < BK) {
                         unsigned char *a = buf + s * S::kStage;
                         const int cells = (BK - rows) * (kRowBytes / 16);
-                        const int blocks = kLanes / MNB + (t.ncols + MNB - 1) / MNB;
+                        const int blocks = kLanes / MNB + (n + MNB - 1) / MNB;
                         for (int j = 0; j < blocks; ++j) {
                             uint4 *z = reinterpret_cast<uint4 *>(a + j * MN_BLOCK + rows * kRowBytes);
                             for (int i = lane; i < cells; i += 32) z[i] = make_uint4(0, 0, 0, 0);
@@ -869,8 +924,13 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                         __syncwarp();
                     }
                     if (lane == 0) {
-                        bar_arrive(smem_u32(&ctl.zeroed[s]));
-                        bar_arrive(smem_u32(&ctl.empty[s]));
+                        if constexpr (PAIR) {
+                            if (rows < BK) bar_arrive_in(smem_u32(&ctl.zeroed[s]), 0);
+                            else bar_arrive_relaxed_in(smem_u32(&ctl.zeroed[s]), 0);
+                        } else {
+                            bar_arrive(smem_u32(&ctl.zeroed[s]));
+                            bar_arrive(smem_u32(&ctl.empty[s]));
+                        }
                     }
                 }
             }
@@ -927,7 +987,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         bool ok = true;
         while (walk.next(t)) {
             const int nkb = t.nkb;
-            const int lane0 = t.lane_tile * kLanes;
+            const int lane0 = t.lane_tile * walk.LANES + int(rank) * kLanes;
             const int features = min(kLanes, p.lanes - lane0);
             OUT *out = static_cast<OUT *>(p.out) + (WHICH == kWgrad ? t.group * p.out_group : 0) +
                        static_cast<long>(t.col0) * p.ldo + lane0;
@@ -997,7 +1057,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 if constexpr (SPLIT)
                     ok = add_parts<OUT>(sum[0], ctl.part, smem_u32(&ctl.pfull), half, quad, lane, out, p.ldo, t.valid, features, ok, fail, p.status);
             } else {
-                if (nkb && ok) ok = warp_wait(smem_u32(&ctl.tfull[acc % ACC]), (acc / ACC) & 1, fail, p.status);
+                if (nkb && ok) ok = warp_wait(smem_u32(&ctl.tfull[acc % ACC]), (acc / ACC) & 1, fail, p.status, nkb);
                 tc_fence_after();
                 const uint32_t at = tmem + lanes_at + (acc % ACC) * COLS;
                 float v[2][16];
@@ -1016,29 +1076,27 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 if (nkb) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) bar_arrive_tmem(smem_u32(&ctl.tempty[acc % ACC]));
+                    if (lane == 0) {
+                        if constexpr (PAIR) bar_arrive_relaxed_in(smem_u32(&ctl.tempty[acc % ACC]), 0);
+                        else bar_arrive_tmem(smem_u32(&ctl.tempty[acc % ACC]));
+                    }
                     ++acc;
                 }
                 if constexpr (SPLIT)
                     ok = add_parts<OUT>(v, ctl.part, smem_u32(&ctl.pfull), half, quad, lane, out, p.ldo, t.valid, features, ok, fail, p.status);
             }
         }
-        if constexpr (WHICH != kWgrad) {
-            // rows of no group are zero
-            const int lo = ctl.groups.off[0], hi = ctl.groups.off[p.E];
-            const long rows = static_cast<long>(lo) + (p.T - hi);
-            for (long r = blockIdx.x; r < rows; r += gridDim.x) {
-                OUT *o = static_cast<OUT *>(p.out) + (r < lo ? r : r - lo + hi) * p.ldo;
-                for (int f = threadIdx.x; f < p.lanes; f += kEpiWarps * 32) o[f] = from_float<OUT>(0.f);
-            }
-        }
+        if constexpr (WHICH != kWgrad) zero_other_rows<OUT>(ctl.groups, p);
     }
     __syncwarp();
     tc_fence_before();
-    if constexpr (SPLIT) cluster_sync();       // nobody reads this block's sums any more
+    if constexpr (MODE != kAlone) cluster_sync();   // nobody reads this block's sums, or its operands, any more
     else __syncthreads();
     tc_fence_after();
-    if (warp == kMmaWarp) tmem_free(tmem, TMEM_COLS);
+    if (warp == kMmaWarp) {
+        if constexpr (PAIR) pair_tmem_free(tmem, TMEM_COLS);
+        else tmem_free(tmem, TMEM_COLS);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1129,22 +1187,28 @@ inline cudaError_t set_up(Kernel k, size_t bytes, int regs, std::atomic<bool> &r
     return cudaSuccess;
 }
 
-template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, bool SPLIT>
+template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, int MODE>
 cudaError_t launch(const Call &c) {
     CUtensorMap ta, tb;
     int dev = 0;
     const int sms = grid_sms(&dev);
     if (sms <= 0) return cudaErrorInvalidDevice;
     if (!make_maps<KIND, WHICH>(c, ta, tb)) return cudaErrorInvalidValue;
-    const Kernel k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES, SPLIT>;
-    constexpr size_t bytes = Smem<KIND, COLS, STAGES, SPLIT>::bytes();
+    const Kernel k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES, MODE>;
+    constexpr size_t bytes = Smem<KIND, COLS, STAGES, MODE>::bytes();
     static_assert(bytes <= 232448, "shared memory of one block");
     static std::atomic<bool> ready[kMaxDevices];
     const cudaError_t e = set_up(k, bytes, 0, ready[dev]);
     if (e != cudaSuccess) return e;
     // no more blocks than there can be tiles
     const long col_tiles = WHICH == kWgrad ? long(c.p.E) * ((c.p.cols + COLS - 1) / COLS) : max_col_tiles<COLS>(c);
-    const long tiles = (c.p.lanes + kLanes - 1L) / kLanes * col_tiles;
+    constexpr long lanes = MODE == kPair ? 2 * kLanes : kLanes;
+    const long tiles = (c.p.lanes + lanes - 1) / lanes * col_tiles;
+    constexpr bool SPLIT = MODE == kSplit;
+    if (MODE == kPair) {
+        const long pairs = sms / 2 > 0 ? sms / 2 : 1;
+        return launch_on(k, 2 * (tiles < pairs ? tiles : pairs), kThreads, 2, bytes, c, ta, tb);
+    }
     return launch_on(k, SPLIT ? tiles * c.split : tiles < sms ? tiles : sms, kThreads, SPLIT ? c.split : 1, bytes, c, ta, tb);
 }
 
@@ -1160,8 +1224,8 @@ cudaError_t launch_few(Call c) {
     const long tiles = (c.p.lanes + kLanes - 1L) / kLanes * max_col_tiles<64>(c);
     c.split = 1;
     while (c.split < kMaxSplit && tiles * c.split * 2 <= sms && nkb >= c.split * 2 * 2) c.split *= 2;
-    if (c.split == 1) return launch<KIND, OUT, WHICH, 64, 8, false>(c);
-    return launch<KIND, OUT, WHICH, 64, 6, true>(c);
+    if (c.split == 1) return launch<KIND, OUT, WHICH, 64, 8, kAlone>(c);
+    return launch<KIND, OUT, WHICH, 64, 6, kSplit>(c);
 }
 
 }  // namespace mm

@@ -140,7 +140,7 @@ def _grouped_backward(ctx, dy):
     T = x.shape[0]
     dx = x.new_empty((T, K)) if need_x else None
     dw = x.new_empty((E, N, K)) if need_w else None
-    dy, ld_dy = _rows(dy)
+    dy, ld_dy = _rows(dy if dy.dtype == x.dtype else dy.to(x.dtype))
     x, ld_x = _rows(x)
     weight = _dense(weight)
     off_ptr, off_size = _bounds(offsets)
@@ -269,8 +269,6 @@ def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
     if T == 0:
         return torch.empty((0, N), dtype=out_dtype, device=xq.device)
     xq, ld = _rows(xq)
-    if min(x_scale.stride()) < 0:
-        x_scale = x_scale.contiguous()
     q, scale = _dense(q), scale.contiguous()
     out = xq.new_empty((T, N), dtype=out_dtype)
     off_ptr, off_size = _bounds(offsets)

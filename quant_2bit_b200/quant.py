@@ -278,7 +278,10 @@ def bcjr_experts_linear(x, offsets, weights, signs_l, signs_r, codebook, T_temp,
     204-211, :309-315; the quantized weight is cast to x's type there too), with
     one launch of each kernel for all of them.  Returns (T, N); gradients flow
     to x and to every weight."""
-    assert len(weights) >= 1, "at least one expert"
+    assert len(weights) >= 1 and all(W.shape == weights[0].shape for W in weights), \
+        "at least one expert, all of one shape"
+    if x.dtype not in (torch.bfloat16, torch.float16):       # before the weights are quantized
+        raise ValueError(f"x must be torch.bfloat16 or torch.float16, got {x.dtype}")
     quantized = bcjr_quantize_layer(weights, signs_l, signs_r, codebook, T_temp, preds, succs)
     return grouped_linear(x, torch.stack(quantized).to(x.dtype), offsets)
 

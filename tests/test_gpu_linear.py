@@ -99,6 +99,8 @@ GROUPS = [
     ([0, 64, 0], 528, 512),
     ([7, 33, 0, 64, 12, 1] * 40, 144, 272),        # several tiles and short groups for each block
     ([90, 0, 3, 1, 20, 0, 0, 0, 2], 80, 208),      # more than 64 rows, few to a group
+    ([100, 0, 37, 301], 1040, 1168),               # many features: pairs of blocks
+    ([300, 5], 2064, 1024),
     ([3, 1, 4, 1, 5, 9, 2, 6, 5, 3, 5, 8, 9, 7, 9, 3] * 5, 32, 96),   # 80 groups
 ]
 
@@ -600,7 +602,23 @@ def test_a_wait_that_runs_out_is_reported(cuda_ok):
                                    32, 64, 0, y8.data_ptr(), ws.data_ptr(), ws.numel(),
                                    status.data_ptr(), stream)
 
-    for call, out in ((forward, y), (lambda: backward(1, 0), dx), (lambda: backward(0, 1), dw),
+    # pairs of blocks: the first tile of 256 features (x's rows serve as dy's too)
+    wide = torch.zeros(100, 1024, dtype=torch.bfloat16, device="cuda")
+    w_wide = torch.randn(1024, 64, device="cuda").to(torch.bfloat16)
+    x_wide = torch.randn(100, 1024, device="cuda").to(torch.bfloat16)
+    narrow = torch.randn(100, 64, device="cuda").to(torch.bfloat16)
+    dw_wide = torch.zeros(64, 1024, dtype=torch.bfloat16, device="cuda")
+
+    def forward_pair():
+        return lib.bcjr_grouped_mm(narrow.data_ptr(), 64, w_wide.data_ptr(), None, 0, 100, 1, 1024, 64, 0,
+                                   wide.data_ptr(), status.data_ptr(), stream)
+
+    def weights_pair():
+        return lib.bcjr_grouped_backward(narrow.data_ptr(), 64, x_wide.data_ptr(), 1024, None, None, 0, 100,
+                                         1, 64, 1024, 0, None, dw_wide.data_ptr(), status.data_ptr(), stream)
+
+    for call, out in ((forward_pair, wide[:, :256]), (weights_pair, dw_wide[:, :256]),
+                      (forward, y), (lambda: backward(1, 0), dx), (lambda: backward(0, 1), dw),
                       (lambda: backward(1, 1), dw), (lambda: fp8(20), y8[:20]), (lambda: fp8(70), y8)):
         with _lib.test_option(_lib.OPT_TEST_DROP_SENDS, 1):
             assert call() == 0
