@@ -33,20 +33,27 @@ _TILE = 16
 _MAX_GROUPS = 1024
 _F8 = torch.float8_e4m3fn
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+_HALVES = (torch.bfloat16, torch.float16)
 
 
-def _need_cuda(**tensors):
-    """All tensors on one GPU; returns its index."""
+# Calls with few rows take less time on the GPU than in here, so the checks of
+# the usual case are few and their messages are made only when one fails.
+
+
+def _need_cuda(names, *tensors):
+    """All tensors on one GPU (None is skipped); returns its index."""
     device = -1
-    for name, t in tensors.items():
+    for i, t in enumerate(tensors):
         if t is None:
             continue
-        if not (torch.is_tensor(t) and t.is_cuda):
-            raise RuntimeError(f"quant_2bit_b200: `{name}` must be a CUDA tensor (the B200 kernels "
-                               "have no CPU fallback)")
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise RuntimeError(f"quant_2bit_b200: `{names.split()[i]}` must be a CUDA tensor (the B200 "
+                               "kernels have no CPU fallback)")
+        d = t.get_device()
         if device < 0:
-            device = t.get_device()
-        assert t.get_device() == device, f"`{name}` is on {t.device}, not on cuda:{device}"
+            device = d
+        elif d != device:
+            raise AssertionError(f"`{names.split()[i]}` is on cuda:{d}, not on cuda:{device}")
     return device
 
 
@@ -87,16 +94,20 @@ def _rows(t):
     """(tensor, elements between rows) of a 2-D matrix as the kernels read it: the
     matrix itself when its rows are contiguous and start on 16 bytes, else a
     contiguous copy."""
-    step = t.stride(0) if t.shape[0] > 1 else t.shape[1]
-    if t.stride(1) == 1 and step >= t.shape[1] and step * t.element_size() % 16 == 0 \
-            and t.data_ptr() % 16 == 0:
-        return t, step
-    return _dense(t), t.shape[1]
+    n = t.size(1)
+    if t.data_ptr() % 16 == 0:
+        if t.is_contiguous():
+            return t, n
+        step = t.stride(0)
+        if t.stride(1) == 1 and step >= n and step * t.element_size() % 16 == 0:
+            return t, step
+    return _dense(t), n
 
 
 def _dense(t):
     """Contiguous and 16-byte aligned."""
-    t = t.contiguous()
+    if not t.is_contiguous():
+        t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
@@ -107,7 +118,7 @@ def _need_offsets(offsets, groups):
     _need_dtype(offsets, "offsets", (torch.int32, torch.int64))
     assert offsets.dim() == 1 and offsets.shape[0] == groups + 1, \
         f"offsets must have one more element than there are experts ({groups}), got {tuple(offsets.shape)}"
-    return offsets.contiguous()
+    return offsets if offsets.is_contiguous() else offsets.contiguous()
 
 
 def _bounds(offsets):
@@ -121,8 +132,8 @@ def _bounds(offsets):
 
 def _grouped_forward(x, weight, offsets):
     E, N, K = weight.shape
-    T = x.shape[0]
-    y = x.new_empty((T, N))
+    T = x.size(0)
+    y = x.new_empty(T, N)
     if T == 0:
         return y
     x, ld = _rows(x)
@@ -138,8 +149,8 @@ def _grouped_backward(ctx, dy):
     need_x, need_w, _ = ctx.needs_input_grad
     E, N, K = weight.shape
     T = x.shape[0]
-    dx = x.new_empty((T, K)) if need_x else None
-    dw = x.new_empty((E, N, K)) if need_w else None
+    dx = x.new_empty(T, K) if need_x else None
+    dw = x.new_empty(E, N, K) if need_w else None
     dy, ld_dy = _rows(dy if dy.dtype == x.dtype else dy.to(x.dtype))
     x, ld_x = _rows(x)
     weight = _dense(weight)
@@ -174,15 +185,17 @@ def grouped_linear(x, weight, offsets):
     Returns (T, N).  Groups may be empty; rows before offsets[0] and from
     offsets[E] on belong to no group: their output and gradient are zero.
     Sums are fp32, rounded once; results do not change from run to run."""
-    _need_cuda(x=x, weight=weight, offsets=offsets)
-    _need_dtype(x, "x", (torch.bfloat16, torch.float16))
-    _need_dtype(weight, "weight", (x.dtype,))
-    assert x.dim() == 2 and weight.dim() == 3 and x.shape[1] == weight.shape[2], \
+    _need_cuda("x weight offsets", x, weight, offsets)
+    _need_dtype(x, "x", _HALVES)
+    if weight.dtype != x.dtype:
+        _need_dtype(weight, "weight", (x.dtype,))
+    assert x.dim() == 2 and weight.dim() == 3 and x.size(1) == weight.size(2), \
         f"x must be (T, K) and weight (E, N, K), got {tuple(x.shape)} and {tuple(weight.shape)}"
-    assert 1 <= weight.shape[0] <= _MAX_GROUPS, f"1 to {_MAX_GROUPS} experts, got {weight.shape[0]}"
-    _need_features(weight.shape[1], "out features")
-    _need_features(weight.shape[2], "in features")
-    offsets = _need_offsets(offsets, weight.shape[0])
+    E, N, K = weight.shape
+    assert 1 <= E <= _MAX_GROUPS, f"1 to {_MAX_GROUPS} experts, got {E}"
+    _need_features(N, "out features")
+    _need_features(K, "in features")
+    offsets = _need_offsets(offsets, E)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         return _GroupedLinear.apply(x, weight, offsets)
     return _grouped_forward(x, weight, offsets)
@@ -196,52 +209,62 @@ def fp8_quantize_rows(x):
     """(q, scale) of (..., K) bf16, fp16 or fp32: q e4m3 of x's shape, scale fp32
     (..., ceil(K / 128)); q times its segment's scale stands for x.  Not
     differentiable (``fp8_linear`` is)."""
-    _need_cuda(x=x)
-    _need_dtype(x, "x", tuple(_DTYPES))
+    _need_cuda("x", x)
+    code = _DTYPES.get(x.dtype)
+    if code is None:
+        _need_dtype(x, "x", tuple(_DTYPES))
     assert x.dim() >= 1, "x must have at least one axis"
-    K = x.shape[-1]
+    K = x.size(-1)
     _need_features(K, "the last axis")
     blocks = _blocks(K)
-    q = x.new_empty(x.shape, dtype=_F8)
-    scale = x.new_empty((*x.shape[:-1], blocks), dtype=torch.float32)
-    if x.numel():
-        rows, ld = _rows(x if x.dim() == 2 else x.detach().reshape(-1, K))
-        _call(_lib.load().bcjr_fp8_quantize_rows, x.get_device(), rows.data_ptr(), ld,
-              rows.shape[0], K, _DTYPES[x.dtype], q.data_ptr(), scale.data_ptr(), blocks, 1)
-    return q, scale
+    rows = x if x.dim() == 2 else x.detach().reshape(-1, K)
+    T = rows.size(0)
+    q = x.new_empty(T, K, dtype=_F8)
+    scale = x.new_empty(T, blocks, dtype=torch.float32)
+    if T:
+        rows, ld = _rows(rows)
+        _call(_lib.load().bcjr_fp8_quantize_rows, x.get_device(), rows.data_ptr(), ld, T, K, code,
+              q.data_ptr(), scale.data_ptr(), blocks, 1)
+    if x.dim() == 2:
+        return q, scale
+    return q.view(x.shape), scale.view(*x.shape[:-1], blocks)
 
 
 def fp8_quantize_weight(weight):
     """(q, scale) of a weight (N, K), or of E weights (E, N, K), bf16, fp16 or
     fp32: q e4m3 of its shape, scale fp32 ([E,] ceil(N / 128), ceil(K / 128)),
     one for each 128 x 128 block."""
-    _need_cuda(weight=weight)
-    _need_dtype(weight, "weight", tuple(_DTYPES))
+    _need_cuda("weight", weight)
+    code = _DTYPES.get(weight.dtype)
+    if code is None:
+        _need_dtype(weight, "weight", tuple(_DTYPES))
     assert weight.dim() in (2, 3), f"weight must be (N, K) or (E, N, K), got {tuple(weight.shape)}"
-    N, K = weight.shape[-2:]
-    E = weight.shape[0] if weight.dim() == 3 else 1
+    *lead, N, K = weight.shape
     assert N >= 1, "weight must have rows"
     _need_features(K, "in features")
     w = _dense(weight)
-    q = weight.new_empty(weight.shape, dtype=_F8)
-    scale = weight.new_empty((*weight.shape[:-2], _blocks(N), _blocks(K)), dtype=torch.float32)
-    _call(_lib.load().bcjr_fp8_quantize_blocks, weight.get_device(), w.data_ptr(), E, N, K,
-          _DTYPES[w.dtype], q.data_ptr(), scale.data_ptr())
+    q = weight.new_empty(*lead, N, K, dtype=_F8)
+    scale = weight.new_empty(*lead, _blocks(N), _blocks(K), dtype=torch.float32)
+    _call(_lib.load().bcjr_fp8_quantize_blocks, weight.get_device(), w.data_ptr(),
+          lead[0] if lead else 1, N, K, code, q.data_ptr(), scale.data_ptr())
     return q, scale
 
 
 def _need_fp8_weight(q, scale, offsets):
-    _need_dtype(q, "q", (_F8,))
-    _need_dtype(scale, "scale", (torch.float32,))
+    """(E, N, K, offsets) of a weight in blocks, checked."""
+    if q.dtype != _F8:
+        _need_dtype(q, "q", (_F8,))
+    if scale.dtype != torch.float32:
+        _need_dtype(scale, "scale", (torch.float32,))
     assert q.dim() == (2 if offsets is None else 3), \
         f"q must be (N, K), or (E, N, K) with offsets, got {tuple(q.shape)}"
-    N, K = q.shape[-2:]
-    E = q.shape[0] if q.dim() == 3 else 1
+    *lead, N, K = q.shape
+    E = lead[0] if lead else 1
     assert 1 <= E <= _MAX_GROUPS, f"1 to {_MAX_GROUPS} experts, got {E}"
     _need_features(N, "out features")
     _need_features(K, "in features")
-    assert scale.shape == (*q.shape[:-2], _blocks(N), _blocks(K)), \
-        f"scale must be {(*q.shape[:-2], _blocks(N), _blocks(K))}, got {tuple(scale.shape)}"
+    assert scale.shape == (*lead, _blocks(N), _blocks(K)), \
+        f"scale must be {(*lead, _blocks(N), _blocks(K))}, got {tuple(scale.shape)}"
     assert not scale.requires_grad, "the scales of an e4m3 weight have no gradient"
     return E, N, K, _need_offsets(offsets, E)
 
@@ -256,10 +279,10 @@ def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
     Returns (T, N) in ``out_dtype`` (bf16 or fp16).  Any fp32 scales are
     accepted; the product of two scales is formed in fp32, so it should not
     underflow."""
-    _need_cuda(xq=xq, x_scale=x_scale, q=q, scale=scale, offsets=offsets)
+    _need_cuda("xq x_scale q scale offsets", xq, x_scale, q, scale, offsets)
     _need_dtype(xq, "xq", (_F8,))
     _need_dtype(x_scale, "x_scale", (torch.float32,))
-    if out_dtype not in (torch.bfloat16, torch.float16):
+    if out_dtype not in _HALVES:
         raise ValueError(f"out_dtype must be torch.bfloat16 or torch.float16, got {out_dtype}")
     E, N, K, offsets = _need_fp8_weight(q, scale, offsets)
     assert xq.dim() == 2 and xq.shape[1] == K, f"xq must be (T, {K}), got {tuple(xq.shape)}"
@@ -269,8 +292,8 @@ def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
     if T == 0:
         return torch.empty((0, N), dtype=out_dtype, device=xq.device)
     xq, ld = _rows(xq)
-    q, scale = _dense(q), scale.contiguous()
-    out = xq.new_empty((T, N), dtype=out_dtype)
+    q, scale = _dense(q), _dense(scale)
+    out = xq.new_empty(T, N, dtype=out_dtype)
     off_ptr, off_size = _bounds(offsets)
     _call(_lib.load().bcjr_fp8_mm, xq.get_device(), xq.data_ptr(), ld, x_scale.data_ptr(),
           x_scale.stride(0), x_scale.stride(1), q.data_ptr(), scale.data_ptr(), off_ptr, off_size,
@@ -281,18 +304,17 @@ def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
 def _quantized_product(x, q, scale, offsets, transpose):
     """x's rows, quantized, times the e4m3 weight (or its transpose)."""
     T, C = x.shape
-    N, K = q.shape[-2:]
-    E = q.shape[0] if q.dim() == 3 else 1
-    out = x.new_empty((T, K if transpose else N))
+    *lead, N, K = q.shape
+    E = lead[0] if lead else 1
+    out = x.new_empty(T, K if transpose else N)
     if T == 0:
         return out
-    lib = _lib.load()
-    size = lib.bcjr_fp8_linear_workspace_bytes(T, C)
+    size = T * (C + 4 * _blocks(C)) + 16          # bcjr_fp8_linear_workspace_bytes
     ws = x.new_empty(size, dtype=torch.uint8)
     x, ld = _rows(x)
-    q, scale = _dense(q), scale.contiguous()
+    q, scale = _dense(q), _dense(scale)
     off_ptr, off_size = _bounds(offsets)
-    _call(lib.bcjr_fp8_linear, x.get_device(), x.data_ptr(), ld, _DTYPES[x.dtype], q.data_ptr(),
+    _call(_lib.load().bcjr_fp8_linear, x.get_device(), x.data_ptr(), ld, _DTYPES[x.dtype], q.data_ptr(),
           scale.data_ptr(), off_ptr, off_size, T, E, N, K, transpose, out.data_ptr(),
           ws.data_ptr(), size, None)
     return out
@@ -326,17 +348,18 @@ def fp8_linear(x, q, scale, offsets=None):
     product with the stored weight, with the upstream gradient quantized in
     row segments of 128; the rounding of x counts as the identity.  The weight
     is constant."""
-    _need_cuda(x=x, q=q, scale=scale, offsets=offsets)
-    _need_dtype(x, "x", (torch.bfloat16, torch.float16))
+    _need_cuda("x q scale offsets", x, q, scale, offsets)
+    _need_dtype(x, "x", _HALVES)
     E, N, K, offsets = _need_fp8_weight(q, scale, offsets)
-    assert x.dim() >= 1 and x.shape[-1] == K, f"x must be (..., {K}), got {tuple(x.shape)}"
-    assert offsets is None or x.dim() == 2, f"x must be (T, K) with offsets, got {tuple(x.shape)}"
-    rows = x if x.dim() == 2 else x.reshape(-1, K)
+    dims = x.dim()
+    assert dims >= 1 and x.size(-1) == K, f"x must be (..., {K}), got {tuple(x.shape)}"
+    assert offsets is None or dims == 2, f"x must be (T, K) with offsets, got {tuple(x.shape)}"
+    rows = x if dims == 2 else x.reshape(-1, K)
     if torch.is_grad_enabled() and x.requires_grad:
         y = _Fp8Linear.apply(rows, q, scale, offsets)
     else:
         y = _quantized_product(rows, q, scale, offsets, False)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+    return y if dims == 2 else y.view(*x.shape[:-1], N)
 
 
 __all__ = ["grouped_linear", "fp8_quantize_rows", "fp8_quantize_weight", "fp8_matmul", "fp8_linear"]

@@ -79,6 +79,13 @@ def test_fp8_linear_refuses(lib):
     assert call(T=0, x=None, ws=None) == OK
 
 
+def test_workspace_formula(lib):
+    """The binding sizes the workspace by the library's formula."""
+    from quant_2bit_b200 import linear
+    for T, C in ((1, 16), (7, 144), (4097, 2048)):
+        assert lib.bcjr_fp8_linear_workspace_bytes(T, C) == T * (C + 4 * linear._blocks(C)) + 16
+
+
 def test_quantizers_refuse(lib):
     def rows(x=P, ld=64, n=8, k=64, dtype=0, q=P, s=P, s_row=1, s_blk=8):
         return lib.bcjr_fp8_quantize_rows(x, ld, n, k, dtype, q, s, s_row, s_blk, None)
