@@ -392,16 +392,10 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ 
                 for (int i = 0; i < 4; ++i)
 #pragma unroll
                     for (int j = 0; j < 32; ++j) sum[i][j] = 0.f;
-                for (int kb = 0; kb < nkb; ++kb, ++acc) {
-                    const float f = x0 * w0;
-                    x0 = x1;
-                    w0 = w1;
-                    if (kb + 2 < nkb) {
-                        x1 = *(xs += xs_step);
-                        w1 = *(ws += ws_step);
-                    }
+                // one k block: its sums times f, the product of its two scales
+                auto add_block = [&](float f) {
                     if (ok) ok = warp_wait(smem_u32(&ctl.tfull[half][acc & 1]), (acc >> 1) & 1, fail, p.status);
-                    if (!ok) continue;
+                    if (!ok) return;
                     tc_fence_after();
                     const uint32_t at = tmem + lanes_at + (half * 2 + (acc & 1)) * 128;
                     const float2 ff = make_float2(f, f);
@@ -423,6 +417,25 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ 
                             s[1] = r.y;
                         }
                     }
+                };
+                // (two at a time, so that a scale stays in its register from its
+                // load to its use: a move in between waited for the load)
+                for (int kb = 0; kb < nkb; kb += 2) {
+                    const float f0 = x0 * w0;
+                    if (kb + 2 < nkb) {
+                        x0 = *(xs += xs_step);
+                        w0 = *(ws += ws_step);
+                    }
+                    add_block(f0);
+                    ++acc;
+                    if (kb + 1 == nkb) break;
+                    const float f1 = x1 * w1;
+                    if (kb + 3 < nkb) {
+                        x1 = *(xs += xs_step);
+                        w1 = *(ws += ws_step);
+                    }
+                    add_block(f1);
+                    ++acc;
                 }
                 more = walk.next(t);
                 if (more) begin();
