@@ -176,7 +176,7 @@ cudaError_t run_blocks(const void *w, long blocks, int n, int k, void *q, float 
 // Each half has accumulator buffers and an issuing warp of its own, so that
 // they run out of step: one half's sums run under the other's products.
 constexpr int kRowTile = 128, kFeatTile = 256, kRowStages = 3;
-constexpr int kStorePitch = 256 + 16;             // a row of 128 features; no bank conflicts
+constexpr int kStoreBytes = 32 * 128;             // 32 rows of 64 features, as a box of the output's map
 constexpr uint32_t kBlockBytes = 128 * kRowBytes;
 // Registers: 3 warpgroups x 168 at launch; the two of the epilogue hold 128
 // sums a thread and take over most of the third one's share.
@@ -184,11 +184,12 @@ constexpr int kLaunchRegs = 168, kFewRegs = 56, kManyRegs = 224;
 static_assert(kFewRegs + 2 * kManyRegs == 3 * kLaunchRegs, "");
 
 struct RowsCtl {
+    unsigned char stage[kEpiWarps][2][kStoreBytes];      // first: on 1024 bytes
+
     unsigned long long full[kRowStages], empty[kRowStages];
     unsigned long long tfull[2][2], tempty[2][2], done[2];     // [half][buffer]
     uint32_t tmem;
     int fail;
-    alignas(16) unsigned char stage[kEpiWarps][32 * kStorePitch];
     Groups groups;
 };
 constexpr size_t kRowsBytes = 1024 + size_t(kRowStages) * 3 * kBlockBytes + sizeof(RowsCtl);
@@ -226,7 +227,7 @@ struct RowWalk {
 template <typename OUT, int WHICH>
 __global__ void __launch_bounds__(kThreads, 1)
 fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx,
-                const __grid_constant__ Params p) {
+                const __grid_constant__ CUtensorMap ty, const __grid_constant__ Params p) {
     constexpr bool W_MN = WHICH == kDgrad;
     constexpr int BK = kRowBytes, SLICES = 4;
     constexpr uint32_t W_STEP = W_MN ? BK / SLICES * kRowBytes : 32;
@@ -255,6 +256,7 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ 
     if (threadIdx.x == 32) {
         prefetch_map(&tw);
         prefetch_map(&tx);
+        prefetch_map(&ty);
     }
     if (warp == kMmaWarp) tmem_alloc(smem_u32(&ctl.tmem), 512);
     read_groups<kThreads>(ctl.groups, p);
@@ -357,7 +359,7 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ 
         regs_up<kManyRegs>();
         const int quad = warp & 3, half = warp >> 2;
         const uint32_t lanes_at = static_cast<uint32_t>(quad * 32) << 16;
-        unsigned char *stage = ctl.stage[warp];
+        unsigned char *stage = ctl.stage[warp][0];
         uint32_t acc = 0;
         bool ok = true;
         if (p.dependent) wait_for_previous();
@@ -439,13 +441,15 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ 
                 }
                 more = walk.next(t);
                 if (more) begin();
-                // Each thread's row into shared memory, and from there as one
-                // asynchronous copy: a tile's 64 KB leave under the next tile's
-                // sums.  (All blocks store at about the same time, and vector
-                // stores held the epilogue up for 5600 clocks a tile.)
-                const int r = quad * 32 + lane;
-                unsigned char *row = stage + lane * kStorePitch;
+                // Each thread's row into shared memory, laid out as two boxes of
+                // the output's map: a warp's 32 rows leave in two asynchronous
+                // stores under the next tile's sums.  (All blocks store at about
+                // the same time: vector stores held the epilogue up for 5600
+                // clocks a tile, one bulk copy per row for 1500 to issue.)
+                const int live = min(32, now.rows - quad * 32);       // rows that the group has
+                const int row0 = now.row0 + quad * 32, feat0 = now.feat0 + half * 128;
                 bulk_wait_read();
+                __syncwarp();
 #pragma unroll
                 for (int i = 0; i < 16; ++i) {
                     float *v = &sum[i >> 2][(i & 3) * 8];
@@ -453,14 +457,27 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ 
 #pragma unroll
                         for (int j = 0; j < 8; ++j) v[j] = __int_as_float(0x7fffffff);
                     }
-                    *reinterpret_cast<uint4 *>(row + i * 16) =
+                    *reinterpret_cast<uint4 *>(stage + (i >> 3) * kStoreBytes + lane * 128 + ((i ^ lane) & 7) * 16) =
                         make_uint4(pack<OUT>(v[0], v[1]), pack<OUT>(v[2], v[3]), pack<OUT>(v[4], v[5]), pack<OUT>(v[6], v[7]));
                 }
-                fence_async();
-                if (r < now.rows)
-                    bulk_store(static_cast<OUT *>(p.out) + (now.row0 + r) * p.ldo + now.feat0 + half * 128,
-                               smem_u32(row), feats * sizeof(OUT));
-                bulk_commit();
+                if (live == 32) {
+                    fence_async();
+                    __syncwarp();
+                    if (elect_one()) {
+                        tma_store2(&ty, feat0, row0, smem_u32(stage));
+                        if (feats > 64) tma_store2(&ty, feat0 + 64, row0, smem_u32(stage + kStoreBytes));
+                        bulk_commit();
+                    }
+                } else {
+                    // a group ends here: the rows behind it are another's
+                    __syncwarp();
+                    for (int i = lane; i < live * 16; i += 32) {
+                        const int r = i >> 4, c = i & 15;
+                        if (c * 8 < feats)
+                            *reinterpret_cast<uint4 *>(static_cast<OUT *>(p.out) + (row0 + r) * p.ldo + feat0 + c * 8) =
+                                *reinterpret_cast<const uint4 *>(stage + (c >> 3) * kStoreBytes + r * 128 + ((c ^ r) & 7) * 16);
+                    }
+                }
             } else {
                 more = walk.next(t);
                 if (more) begin();
@@ -479,7 +496,7 @@ fp8_rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ 
 template <typename OUT, int WHICH>
 cudaError_t launch_many(const Call &c) {
     using U = unsigned long long;
-    CUtensorMap tw, tx;
+    CUtensorMap tw, tx, ty;
     int dev = 0;
     const int sms = grid_sms(&dev);
     if (sms <= 0) return cudaErrorInvalidDevice;
@@ -487,12 +504,15 @@ cudaError_t launch_many(const Call &c) {
     const U xd[2] = {U(c.b_inner), U(c.p.T)}, xst[1] = {U(c.ld_b)};
     const unsigned wb[3] = {128, 128, 1}, xb[2] = {128, unsigned(kRowTile)};
     if (!make_map(&tw, kE4M3, 3, c.a, wd, wst, wb) || !make_map(&tx, kE4M3, 2, c.b, xd, xst, xb)) return cudaErrorInvalidValue;
-    const Kernel k = &fp8_rows_kernel<OUT, WHICH>;
+    const U yd[2] = {U(c.p.lanes), U(c.p.T)}, yst[1] = {U(c.p.ldo) * sizeof(OUT)};
+    const unsigned yb[2] = {64, 32};
+    if (!make_map(&ty, c.out_kind, 2, c.p.out, yd, yst, yb)) return cudaErrorInvalidValue;
+    const auto k = &fp8_rows_kernel<OUT, WHICH>;
     static std::atomic<bool> ready[kMaxDevices];
     const cudaError_t e = set_up(k, kRowsBytes, kLaunchRegs, ready[dev]);
     if (e != cudaSuccess) return e;
     const long tiles = max_col_tiles<kRowTile>(c) * ((c.p.lanes + kFeatTile - 1) / kFeatTile);
-    return launch_on(k, tiles < sms ? tiles : sms, kThreads, 1, kRowsBytes, c, tw, tx);
+    return launch_on(k, tiles < sms ? tiles : sms, kThreads, 1, kRowsBytes, c, tw, tx, ty, c.p);
 }
 
 template <typename OUT>
@@ -595,6 +615,7 @@ static int fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long 
     c.p.status = status;
     c.p.drop = bcjr::test_option(bcjr::kOptDropSends);
     c.p.dependent = dependent;
+    c.out_kind = out_dtype == BCJR_BF16 ? kBF16 : kF16;
     return status_of(out_dtype == BCJR_BF16 ? run_mm<__nv_bfloat16>(c) : run_mm<__half>(c));
 }
 

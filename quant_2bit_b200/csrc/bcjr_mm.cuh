@@ -272,16 +272,17 @@ __device__ __forceinline__ void st_transposed(uint32_t addr, uint32_t a, uint32_
                  ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
                  : "memory");
 }
-// Asynchronous copy of shared memory to global memory, in a group of this thread.
-__device__ __forceinline__ void bulk_store(void *dst, uint32_t src, uint32_t bytes) {
-    asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;"
-                 ::"l"(dst), "r"(src), "r"(bytes)
+// Asynchronous store of a box of a tiled map, in a bulk group of this thread;
+// what lies outside the map is not written.
+__device__ __forceinline__ void tma_store2(const CUtensorMap *map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];"
+                 ::"l"(map), "r"(x), "r"(y), "r"(src)
                  : "memory");
 }
 __device__ __forceinline__ void bulk_commit() {
     asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// This thread's copies have read their source; have been written.
+// This thread's stores have read their source; have been written.
 __device__ __forceinline__ void bulk_wait_read() {
     asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
 }
@@ -1113,6 +1114,7 @@ int grid_sms(int *device);
 
 struct Call {
     int kind, which;          // element type, product
+    int out_kind;             // e4m3: output type
     const void *a, *b;        // weights (wgrad: X) and row matrix (wgrad: dY)
     long ld_a, ld_b;          // elements between rows of wgrad's X; of the row matrix
     long a_rows, a_inner;     // weight rows (N) and row length (K); wgrad: K in a_inner
@@ -1150,9 +1152,9 @@ long max_col_tiles(const Call &c) {
     return c.p.T / COLS + (c.p.E < c.p.T ? c.p.E : c.p.T);
 }
 
-using Kernel = void (*)(CUtensorMap, CUtensorMap, Params);
-inline cudaError_t launch_on(Kernel k, long blocks, int threads, int cluster, size_t bytes, const Call &c,
-                             const CUtensorMap &ta, const CUtensorMap &tb) {
+template <typename... A>
+cudaError_t launch_on(void (*k)(A...), long blocks, int threads, int cluster, size_t bytes,
+                      const Call &c, const A &...args) {
     if (blocks > 0x7fffffffL) return cudaErrorInvalidValue;
     cudaLaunchAttribute a[2];
     cudaLaunchConfig_t cfg = {};
@@ -1171,13 +1173,14 @@ inline cudaError_t launch_on(Kernel k, long blocks, int threads, int cluster, si
     cfg.dynamicSmemBytes = bytes;
     cfg.stream = c.stream;
     cfg.attrs = a;
-    return cudaLaunchKernelEx(&cfg, k, ta, tb, c.p);
+    return cudaLaunchKernelEx(&cfg, k, args...);
 }
 
 // A kernel's settings on the current device, once: its shared memory, and for
 // one that splits registers that it was compiled for the expected number (a
 // split of more registers than a block is launched with would wait for good).
-inline cudaError_t set_up(Kernel k, size_t bytes, int regs, std::atomic<bool> &ready) {
+template <typename K>
+cudaError_t set_up(K k, size_t bytes, int regs, std::atomic<bool> &ready) {
     if (ready.load(std::memory_order_acquire)) return cudaSuccess;
     const cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
     if (e != cudaSuccess) return e;
@@ -1194,7 +1197,7 @@ cudaError_t launch(const Call &c) {
     const int sms = grid_sms(&dev);
     if (sms <= 0) return cudaErrorInvalidDevice;
     if (!make_maps<KIND, WHICH>(c, ta, tb)) return cudaErrorInvalidValue;
-    const Kernel k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES, MODE>;
+    const auto k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES, MODE>;
     constexpr size_t bytes = Smem<KIND, COLS, STAGES, MODE>::bytes();
     static_assert(bytes <= 232448, "shared memory of one block");
     static std::atomic<bool> ready[kMaxDevices];
@@ -1207,9 +1210,9 @@ cudaError_t launch(const Call &c) {
     constexpr bool SPLIT = MODE == kSplit;
     if (MODE == kPair) {
         const long pairs = sms / 2 > 0 ? sms / 2 : 1;
-        return launch_on(k, 2 * (tiles < pairs ? tiles : pairs), kThreads, 2, bytes, c, ta, tb);
+        return launch_on(k, 2 * (tiles < pairs ? tiles : pairs), kThreads, 2, bytes, c, ta, tb, c.p);
     }
-    return launch_on(k, SPLIT ? tiles * c.split : tiles < sms ? tiles : sms, kThreads, SPLIT ? c.split : 1, bytes, c, ta, tb);
+    return launch_on(k, SPLIT ? tiles * c.split : tiles < sms ? tiles : sms, kThreads, SPLIT ? c.split : 1, bytes, c, ta, tb, c.p);
 }
 
 // Forward and dgrad with few rows to a group: tiles of 64 columns and eight
