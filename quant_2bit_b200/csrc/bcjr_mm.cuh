@@ -540,14 +540,24 @@ struct Walk {
         tile = blockIdx.x / blocks;
         group = 0;
     }
+    // Column and lane tile of a group's tile `in`: bands of 2048 lanes, column
+    // by column within a band.  The blocks at work then share a part of either
+    // operand that L2 holds.  (Lane tile by lane tile, the gradients of 8192 x
+    // 8192 x 2048 read 578 MB from memory for 200 MB of operands.)
+    __device__ int place(int in, int ct, int &lane_tile) const {
+        constexpr int BAND = 2048 / LANES;
+        const int band = in / (BAND * ct), at = in - band * BAND * ct;
+        const int height = min(BAND, lane_tiles - band * BAND), c = at / height;
+        lane_tile = band * BAND + at - c * height;
+        return c;
+    }
     __device__ bool next(Tile &t) {
         if (tile >= total) return false;
         if constexpr (WHICH == kWgrad) {
             const int ct = col_tiles<COLS>(p.cols), per = lane_tiles * ct;
             t.group = tile / per;
             const int in = tile - t.group * per;
-            t.lane_tile = in / ct;
-            t.col0 = (in - t.lane_tile * ct) * COLS;
+            t.col0 = place(in, ct, t.lane_tile) * COLS;
             t.valid = min(COLS, p.cols - t.col0);
             t.ncols = (t.valid + STEP - 1) & ~(STEP - 1);
             t.k0 = g.off[t.group];
@@ -558,8 +568,7 @@ struct Walk {
             const int in = tile - g.first[group] * lane_tiles;
             const int ct = g.first[group + 1] - g.first[group];
             t.group = group;
-            t.lane_tile = in / ct;
-            const int c = in - t.lane_tile * ct;
+            const int c = place(in, ct, t.lane_tile);
             const int rows = g.off[group + 1] - g.off[group];
             // equal shares: no small tile at the end of a group
             const int share = ((rows + ct - 1) / ct + STEP - 1) & ~(STEP - 1);
