@@ -80,12 +80,16 @@ BCJR_API int bcjr_version(void);
  *                                 shapes (cross-checks of the cluster kernels)
  *   BCJR_OPT_L16_FORWARD_CLUSTER  2 or 4: cluster size of the L=16, k=2, V=1
  *   BCJR_OPT_L16_BACKWARD_CLUSTER   forward / backward (0: automatic)
+ *   BCJR_OPT_LINEAR_TILES         tiles of the linear layers: 1 few rows, 2 many
+ *                                 rows, one block to a tile, 3 many rows, two
+ *                                 blocks (16-bit types) (0: automatic)
  * Returns the previous value, or -1 for an unknown option. */
 enum {
     BCJR_OPT_TEST_DROP_SENDS = 1,
     BCJR_OPT_FORCE_GENERIC = 2,
     BCJR_OPT_L16_FORWARD_CLUSTER = 3,
-    BCJR_OPT_L16_BACKWARD_CLUSTER = 4
+    BCJR_OPT_L16_BACKWARD_CLUSTER = 4,
+    BCJR_OPT_LINEAR_TILES = 5
 };
 BCJR_API int bcjr_set_test_option(int option, int value);
 

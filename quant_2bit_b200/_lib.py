@@ -28,6 +28,7 @@ OPT_TEST_DROP_SENDS = 1
 OPT_FORCE_GENERIC = 2
 OPT_L16_FORWARD_CLUSTER = 3
 OPT_L16_BACKWARD_CLUSTER = 4
+OPT_LINEAR_TILES = 5
 
 # Every symbol include/bcjr_b200.h declares, with its ctypes signature.
 _P = ctypes.c_void_p

@@ -9,14 +9,9 @@ namespace bcjr {
 namespace mm {
 namespace {
 
-// Many features: two blocks to a tile of 256 lanes; else one block to 128.  (64
-// experts, 32768 rows, 1024 and 2048 features: 113 us forward, 115 and 139 us
-// gradients in pairs, 125, 125 and 157 us alone.  4 experts, 3000 rows, 1040
-// features: the same.  96 experts, 3079 rows, 272 features, weights' gradient:
-// 27 us in pairs, 20 alone: 272 lanes are two tiles of 256 but three of 128.)
 template <int KIND, typename T, int WHICH>
 cudaError_t launch_many(const Call &c) {
-    if (c.p.lanes >= 1024) return launch<KIND, T, WHICH, 256, 6, kPair>(c);
+    if (in_pairs(c)) return launch<KIND, T, WHICH, 256, 6, kPair>(c);
     return launch<KIND, T, WHICH, 256, 4, kAlone>(c);
 }
 

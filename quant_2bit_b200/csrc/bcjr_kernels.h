@@ -15,7 +15,8 @@ enum {
     kOptForceGeneric = 2,    // BCJR_OPT_FORCE_GENERIC
     kOptL16Forward = 3,      // BCJR_OPT_L16_FORWARD_CLUSTER
     kOptL16Backward = 4,     // BCJR_OPT_L16_BACKWARD_CLUSTER
-    kOptCount = 5
+    kOptLinearTiles = 5,     // BCJR_OPT_LINEAR_TILES
+    kOptCount = 6
 };
 int test_option(int which);   // bcjr_capi.cu
 // SMs the cluster kernels leave free for concurrent kernels (collectives),

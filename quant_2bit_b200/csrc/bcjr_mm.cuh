@@ -20,12 +20,30 @@
 // any multiple of 16 up to 256 and is chosen per tile: one token and 256
 // tokens run the same code, and a group of 300 rows costs 304 columns, not
 // 3 x 128.
+//
+// Warp roles: one TMA producer, one issuer of matrix instructions, eight warps
+// that empty the accumulators, two that fetch scales (e4m3) or zero the ragged
+// ends (wgrad); accumulators and operand stages are rings between them, and
+// the blocks are persistent, so loads, products and stores of neighbouring
+// tiles overlap.
+//
+// Measured on a B200 (cold L2; 1.62 PFLOP/s is cuBLAS bf16 at the same size):
+//   8192 x 8192 x 2048 bf16  forward 168 us = 1.64 PFLOP/s, gradients 180 us
+//     each = 1.53; the tensor pipe is busy 87 % of the forward: bound by it.
+//   64 experts, 32768 rows, 1024 x 2048 bf16  113 us forward, 115 and 139 us:
+//     ragged tiles, 0.47 GB of memory traffic a product (4.2 TB/s).
+//   64 experts, 488 rows, 2048 x 1024 fp16  48 us = 5.6 TB/s of weights: bound
+//     by memory.
+//   8 rows by 8 of 64 experts, 1024 x 2048  14 us (34 MB): launch, set-up and
+//     the first loads' latency are half of it.
 #pragma once
 
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
+
+#include "bcjr_kernels.h"
 
 #include <atomic>
 #include <cstdint>
@@ -305,11 +323,6 @@ __device__ __forceinline__ void copy4(uint32_t dst, const float *src, bool real)
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;"
                  ::"r"(dst), "l"(src), "r"(real ? 4 : 0)
                  : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All but the LEFT youngest groups of this thread's copies have landed.
-template <int LEFT> __device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
 }
 // One arrival of this thread on `bar` when its copies so far have landed.
 __device__ __forceinline__ void copy_arrive(uint32_t bar) {
@@ -620,9 +633,9 @@ struct Smem {
     static constexpr int kStage = kA + kB;
     static constexpr int kScales = KIND == kE4M3 ? kScaleStages : 1;
     // accumulator buffers.  16-bit types use one for a tile, e4m3 one for a k
-    // block: with few columns eight of them fit, and the tensor core runs ahead
-    // of the epilogue (one token, 8192 x 2048: 740 clocks a block with two).
-    static constexpr int kAcc = KIND == kE4M3 && COLS <= 64 ? 8 : 2;
+    // block: eight of them, so that the tensor core runs ahead of the epilogue
+    // (one token, 8192 x 2048: 740 clocks a block with two, 630 with eight).
+    static constexpr int kAcc = KIND == kE4M3 ? 8 : 2;
     struct Ctl {
         unsigned long long full[STAGES], empty[STAGES], zeroed[STAGES], tfull[kAcc], tempty[kAcc], done;
         unsigned long long sfull[kScaleStages], sempty[kScaleStages];
@@ -735,7 +748,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     using S = Smem<KIND, COLS, STAGES, MODE>;
     constexpr uint32_t ACC = S::kAcc, TMEM_COLS = ACC * COLS;
     static_assert(TMEM_COLS <= 512 && (TMEM_COLS & (TMEM_COLS - 1)) == 0 && TMEM_COLS >= 32, "");
-    static_assert(!(KIND == kE4M3 && WHICH == kWgrad), "e4m3 has forward and dgrad");
+    static_assert(KIND != kE4M3 || (WHICH != kWgrad && COLS == 64), "e4m3: few rows, forward and dgrad");
     static_assert(BK % kBoxRows == 0 && COLS % 32 == 0, "");
     static_assert(!PAIR || KIND != kE4M3, "pairs: 16-bit types");
 
@@ -987,12 +1000,10 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         }
     } else {
         // epilogue: warp w has lanes 32 (w % 4).., column chunks w / 4, w / 4 + 2, ...
-        constexpr int CHUNKS = COLS / (2 * kChunk);
-        static_assert(COLS % (2 * kChunk) == 0, "");
+        static_assert(COLS == 2 * kChunk || (KIND != kE4M3 && !SPLIT && COLS % (2 * kChunk) == 0), "");
         const int quad = warp & 3, half = warp >> 2;
         const uint32_t lanes_at = static_cast<uint32_t>(quad * 32) << 16;
         unsigned char *stage = ctl.stage[half];
-        static_assert(!SPLIT || CHUNKS == 1, "");
         uint32_t acc = 0;
         bool ok = true;
         while (walk.next(t)) {
@@ -1002,34 +1013,23 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             OUT *out = static_cast<OUT *>(p.out) + (WHICH == kWgrad ? t.group * p.out_group : 0) +
                        static_cast<long>(t.col0) * p.ldo + lane0;
             if constexpr (KIND == kE4M3) {
-                float sum[CHUNKS][2][16];
+                float sum[2][16];
 #pragma unroll
-                for (int i = 0; i < CHUNKS; ++i)
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) sum[i][j >> 4][j & 15] = 0.f;
+                for (int j = 0; j < 32; ++j) sum[j >> 4][j & 15] = 0.f;
+                const int c0 = half * kChunk;
                 for (int kb = 0; kb < nkb; ++kb, ++acc) {
                     const uint32_t s = acc % kScaleStages;
                     if (ok) ok = warp_wait(smem_u32(&ctl.sfull[s]), (acc / kScaleStages) & 1, fail, p.status);
                     if (ok) ok = warp_wait(smem_u32(&ctl.tfull[acc % ACC]), (acc / ACC) & 1, fail, p.status);
                     if (!ok) continue;
                     tc_fence_after();
-                    const float ws = ctl.ws[s];
-                    const uint32_t at = tmem + lanes_at + (acc % ACC) * COLS;
-                    // the next chunk's load runs under this chunk's sums
-                    float v[2][2][16];
-                    if (half * kChunk < t.ncols) {
-                        tmem_ld(v[0][0], at + half * kChunk);
-                        tmem_ld(v[0][1], at + half * kChunk + (16u << 16));
-                    }
-#pragma unroll
-                    for (int i = 0; i < CHUNKS; ++i) {
-                        const int c0 = (half + 2 * i) * kChunk;
-                        if (c0 >= t.ncols) break;
-                        tmem_wait(v[i & 1][0], v[i & 1][1]);
-                        if (i + 1 < CHUNKS && c0 + 2 * kChunk < t.ncols) {
-                            tmem_ld(v[(i + 1) & 1][0], at + c0 + 2 * kChunk);
-                            tmem_ld(v[(i + 1) & 1][1], at + c0 + 2 * kChunk + (16u << 16));
-                        }
+                    if (c0 < t.ncols) {
+                        float v[2][16];
+                        const uint32_t at = tmem + lanes_at + (acc % ACC) * COLS + c0;
+                        tmem_ld(v[0], at);
+                        tmem_ld(v[1], at + (16u << 16));
+                        tmem_wait(v[0], v[1]);
+                        const float ws = ctl.ws[s];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             float2 f = *reinterpret_cast<const float2 *>(&ctl.xs[s][c0 + 8 * j + 2 * (lane & 3)]);
@@ -1037,12 +1037,11 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
 #pragma unroll
                             for (int h = 0; h < 2; ++h)
 #pragma unroll
-                                for (int q = 0; q < 4; q += 2) {
-                                    const int k = 4 * j + q;
-                                    const float2 r = __ffma2_rn(make_float2(v[i & 1][h][k], v[i & 1][h][k + 1]), f,
-                                                                make_float2(sum[i][h][k], sum[i][h][k + 1]));
-                                    sum[i][h][k] = r.x;
-                                    sum[i][h][k + 1] = r.y;
+                                for (int k = 4 * j; k < 4 * j + 4; k += 2) {
+                                    const float2 r = __ffma2_rn(make_float2(v[h][k], v[h][k + 1]), f,
+                                                                make_float2(sum[h][k], sum[h][k + 1]));
+                                    sum[h][k] = r.x;
+                                    sum[h][k + 1] = r.y;
                                 }
                         }
                     }
@@ -1053,19 +1052,15 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                         bar_arrive(smem_u32(&ctl.sempty[s]));
                     }
                 }
+                if (!ok) {
 #pragma unroll
-                for (int i = 0; i < CHUNKS; ++i) {
-                    const int c0 = (half + 2 * i) * kChunk;
-                    if (!SPLIT && c0 >= t.valid) break;
-                    if (!ok) {
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) sum[i][j >> 4][j & 15] = __int_as_float(0x7fffffff);
-                    }
-                    if constexpr (!SPLIT)
-                        store_chunk<OUT>(sum[i], stage, half, quad, lane, out, p.ldo, c0, t.valid, features);
+                    for (int j = 0; j < 32; ++j) sum[j >> 4][j & 15] = __int_as_float(0x7fffffff);
                 }
                 if constexpr (SPLIT)
-                    ok = add_parts<OUT>(sum[0], ctl.part, smem_u32(&ctl.pfull), half, quad, lane, out, p.ldo, t.valid, features, ok, fail, p.status);
+                    ok = add_parts<OUT>(sum, ctl.part, smem_u32(&ctl.pfull), half, quad, lane, out, p.ldo, t.valid,
+                                        features, ok, fail, p.status);
+                else if (c0 < t.valid)
+                    store_chunk<OUT>(sum, stage, half, quad, lane, out, p.ldo, c0, t.valid, features);
             } else {
                 if (nkb && ok) ok = warp_wait(smem_u32(&ctl.tfull[acc % ACC]), (acc / ACC) & 1, fail, p.status, nkb);
                 tc_fence_after();
@@ -1093,7 +1088,8 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                     ++acc;
                 }
                 if constexpr (SPLIT)
-                    ok = add_parts<OUT>(v, ctl.part, smem_u32(&ctl.pfull), half, quad, lane, out, p.ldo, t.valid, features, ok, fail, p.status);
+                    ok = add_parts<OUT>(v, ctl.part, smem_u32(&ctl.pfull), half, quad, lane, out, p.ldo, t.valid,
+                                        features, ok, fail, p.status);
             }
         }
         if constexpr (WHICH != kWgrad) zero_other_rows<OUT>(ctl.groups, p);
@@ -1224,18 +1220,53 @@ cudaError_t launch(const Call &c) {
     return launch_on(k, SPLIT ? tiles * c.split : tiles < sms ? tiles : sms, kThreads, SPLIT ? c.split : 1, bytes, c, ta, tb, c.p);
 }
 
-// Forward and dgrad with few rows to a group: tiles of 64 columns and eight
-// stages (16 KB of weights each, against 64 KB in all with 256 columns).  With
-// few tiles the blocks of a cluster share each one.
-inline bool few_rows(const Call &c) { return c.p.T <= 64 || c.p.T / 32 <= c.p.E; }
+// Two ways for forward and dgrad: few rows to a tile (64 columns, eight stages
+// of 16 KB of weights each; with few tiles up to four blocks of a cluster share
+// one's contraction), or many (256 columns, or the e4m3 kernel's 128 rows by
+// 256 features).  Estimated by the stages that a block works through one after
+// the other: a stage of the small tile costs about 0.6 of a large one's, in
+// e4m3 about 0.5.  Measured, small against large tiles:
+//   1 group,   8 x 2048 x 8192    16-bit 18 | 39 us   e4m3 16 | 37 us
+//   1 group, 192 x 2048 x 8192    16-bit 29 | 43      e4m3 23 | 37
+//   1 group, 192 x 8192 x 2048    16-bit 25 | 21      e4m3 21 | 18
+//   64 groups of about 32, 1024 x 2048   16-bit 49 | 55   e4m3 35 | 35
+//   64 groups of about 96, 1024 x 2048   16-bit 72 | 55   e4m3 53 | 43
+inline int k_blocks(const Call &c) {
+    return (c.p.depth * (c.kind == kE4M3 ? 1 : 2) + kRowBytes - 1) / kRowBytes;
+}
+inline long few_tiles(const Call &c) { return (c.p.lanes + kLanes - 1L) / kLanes * max_col_tiles<64>(c); }
+inline int few_split(const Call &c, int sms) {
+    const long tiles = few_tiles(c);
+    const int nkb = k_blocks(c);
+    int split = 1;
+    while (split < kMaxSplit && tiles * split * 2 <= sms && nkb >= split * 2 * 2) split *= 2;
+    return split;
+}
+// Many features: pairs of blocks.  (64 experts, 32768 rows, 1024 and 2048
+// features: 113 us forward, 115 and 139 us gradients in pairs, 125, 125 and 157
+// us alone.  4 experts, 3000 rows, 1040 features: the same.  96 experts, 3079
+// rows, 272 features, weights' gradient: 27 us in pairs, 20 alone: 272 lanes are
+// two tiles of 256 but three of 128.)
+inline bool in_pairs(const Call &c) {
+    const int forced = test_option(kOptLinearTiles);
+    return c.kind != kE4M3 && (forced ? forced == 3 : c.p.lanes >= 1024);
+}
+inline bool few_rows(const Call &c) {
+    if (const int forced = test_option(kOptLinearTiles)) return forced == 1;
+    int dev = 0;
+    const long sms = grid_sms(&dev);
+    if (sms <= 0) return true;
+    auto waves = [](long tiles, long slots) { return (tiles + slots - 1) / slots; };
+    const long nkb = k_blocks(c), split = few_split(c, int(sms));
+    const long few = waves(few_tiles(c) * split, sms) * ((nkb + split - 1) / split);
+    if (c.kind == kE4M3) return few <= 2 * waves((c.p.lanes + 255L) / 256 * max_col_tiles<128>(c), sms) * nkb;
+    const long lanes = in_pairs(c) ? 2 * kLanes : kLanes, slots = in_pairs(c) ? (sms > 1 ? sms / 2 : 1) : sms;
+    return 3 * few < 5 * waves((c.p.lanes + lanes - 1) / lanes * max_col_tiles<256>(c), slots) * nkb;
+}
 template <int KIND, typename OUT, int WHICH>
 cudaError_t launch_few(Call c) {
     int dev = 0;
-    const int sms = grid_sms(&dev);
-    const int nkb = (c.p.depth * (KIND == kE4M3 ? 1 : 2) + kRowBytes - 1) / kRowBytes;
-    const long tiles = (c.p.lanes + kLanes - 1L) / kLanes * max_col_tiles<64>(c);
-    c.split = 1;
-    while (c.split < kMaxSplit && tiles * c.split * 2 <= sms && nkb >= c.split * 2 * 2) c.split *= 2;
+    c.split = few_split(c, grid_sms(&dev));
     if (c.split == 1) return launch<KIND, OUT, WHICH, 64, 8, kAlone>(c);
     return launch<KIND, OUT, WHICH, 64, 6, kSplit>(c);
 }

@@ -105,17 +105,32 @@ GROUPS = [
 ]
 
 
+# tiles: 0 as the library chooses, 1 few rows, 2 many rows, 3 many rows in pairs of blocks
+@pytest.mark.parametrize("tiles", [0, 1, 2, 3])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("counts,N,K", GROUPS)
-def test_grouped_forward_and_gradients(cuda_ok, counts, N, K, dtype):
+def test_grouped_forward_and_gradients(cuda_ok, counts, N, K, dtype, tiles):
+    from quant_2bit_b200 import _lib
     T = sum(counts)
     x, w, dy = _inputs(T, len(counts), N, K, dtype, seed=T)
-    _check_grouped(x, w, dy, _counts_to_offsets(counts))
+    with _lib.test_option(_lib.OPT_LINEAR_TILES, tiles):
+        _check_grouped(x, w, dy, _counts_to_offsets(counts))
 
 
+def test_many_rows_and_features(cuda_ok):
+    """Sizes for which the library takes the large tiles by itself."""
+    for counts, N, K, dtype in (([3000, 0, 1501, 77], 1040, 1024, torch.bfloat16),
+                                ([2500, 2500], 528, 400, torch.float16)):
+        x, w, dy = _inputs(sum(counts), len(counts), N, K, dtype)
+        _check_grouped(x, w, dy, _counts_to_offsets(counts))
+    x, q, s, w64, dy = _fp8_operands(5000, 0, 1040, 656, torch.bfloat16)
+    _check_fp8(x, q, s, w64, dy, None)
+
+
+@pytest.mark.parametrize("tiles", [1, 2, 3])
 @pytest.mark.parametrize("off_dtype", [torch.int32, torch.int64])
 @pytest.mark.parametrize("head,tail", [(7, 0), (0, 9), (70, 130)])
-def test_rows_of_no_group_are_zero_and_do_not_count(cuda_ok, head, tail, off_dtype):
+def test_rows_of_no_group_are_zero_and_do_not_count(cuda_ok, head, tail, off_dtype, tiles):
     """Rows before the first and behind the last group: zero output and zero
     gradient, whatever they hold."""
     counts = [33, 0, 70, 5]
@@ -125,13 +140,16 @@ def test_rows_of_no_group_are_zero_and_do_not_count(cuda_ok, head, tail, off_dty
     for t in (x, dy):
         t[:head] = float("nan")
         t[T - tail:] = float("inf")
-    _check_grouped(x, w, dy, offsets)
+    from quant_2bit_b200 import _lib
+    with _lib.test_option(_lib.OPT_LINEAR_TILES, tiles):
+        _check_grouped(x, w, dy, offsets)
 
 
-def test_non_finite_rows_stay_in_their_group(cuda_ok):
+@pytest.mark.parametrize("tiles", [1, 2, 3])
+def test_non_finite_rows_stay_in_their_group(cuda_ok, tiles):
     """A NaN or infinity in one group's rows reaches that group only, in every
     direction (tiles end inside the next group's rows)."""
-    from quant_2bit_b200 import grouped_linear
+    from quant_2bit_b200 import _lib, grouped_linear
     counts = [40, 24, 100, 30]
     x, w, dy = _inputs(194, 4, 48, 80, torch.bfloat16)
     offsets = _counts_to_offsets(counts)
@@ -139,8 +157,9 @@ def test_non_finite_rows_stay_in_their_group(cuda_ok):
     dy[64:164] = float("inf")
     x.requires_grad_()
     w.requires_grad_()
-    y = grouped_linear(x, w, offsets)
-    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    with _lib.test_option(_lib.OPT_LINEAR_TILES, tiles):
+        y = grouped_linear(x, w, offsets)
+        dx, dw = torch.autograd.grad(y, (x, w), dy)
     clean = torch.ones(194, dtype=torch.bool, device="cuda")
     clean[64:164] = False
     for t in (y.detach(), dx):
@@ -442,20 +461,24 @@ def _check_fp8(x, q, s, w64, dy, offsets):
     assert y.dtype == dx.dtype == x.dtype
 
 
+@pytest.mark.parametrize("tiles", [0, 1, 2])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,N,K", [(1, 16, 16), (1, 128, 256), (17, 144, 272), (64, 2000, 400),
                                    (65, 48, 128), (300, 272, 1040), (513, 128, 144), (37, 48, 4240), (1, 2064, 528),
                                    (64, 144, 1280), (200, 656, 304), (129, 16, 16)])
-def test_fp8_linear_forward_and_gradient(cuda_ok, T, N, K, dtype):
+def test_fp8_linear_forward_and_gradient(cuda_ok, T, N, K, dtype, tiles):
+    from quant_2bit_b200 import _lib
     x, q, s, w64, dy = _fp8_operands(T, 0, N, K, dtype, seed=T)
-    _check_fp8(x, q, s, w64, dy, None)
+    with _lib.test_option(_lib.OPT_LINEAR_TILES, tiles):
+        _check_fp8(x, q, s, w64, dy, None)
 
 
+@pytest.mark.parametrize("tiles", [0, 1, 2])
 @pytest.mark.parametrize("counts,N,K", [([3, 0, 1, 12], 144, 272), ([130, 0, 300, 70], 272, 144),
                                         ([0, 0], 128, 128), ([257, 1], 128, 384),
                                         ([9, 0, 1], 144, 2064),
                                         ([90, 0, 3, 1, 20, 0, 0, 0, 2], 208, 272)])
-def test_fp8_linear_by_expert(cuda_ok, counts, N, K):
+def test_fp8_linear_by_expert(cuda_ok, counts, N, K, tiles):
     T = sum(counts) + 6
     x, q, s, w64, dy = _fp8_operands(T, len(counts), N, K, torch.bfloat16, seed=T)
     x[:2] = float("nan")
@@ -463,10 +486,11 @@ def test_fp8_linear_by_expert(cuda_ok, counts, N, K):
     dy[:2] = float("inf")
     offsets = _counts_to_offsets(counts, head=2, dtype=torch.int64)
     inside = slice(2, T - 4)
-    from quant_2bit_b200 import fp8_linear
+    from quant_2bit_b200 import _lib, fp8_linear
     xg = x.detach().requires_grad_()
-    y = fp8_linear(xg, q, s, offsets)
-    dx = torch.autograd.grad(y, xg, dy)[0]
+    with _lib.test_option(_lib.OPT_LINEAR_TILES, tiles):
+        y = fp8_linear(xg, q, s, offsets)
+        dx = torch.autograd.grad(y, xg, dy)[0]
     assert not y[:2].any() and not y[T - 4:].any() and not dx[:2].any() and not dx[T - 4:].any()
     for got, rows, w, depth in ((y.detach(), x, w64, K), (dx, dy, w64.transpose(1, 2), N)):
         rows64 = _expand(*_quantize_plain(rows[inside].contiguous(), 1), 1)
@@ -617,9 +641,16 @@ def test_a_wait_that_runs_out_is_reported(cuda_ok):
         return lib.bcjr_grouped_backward(narrow.data_ptr(), 64, x_wide.data_ptr(), 1024, None, None, 0, 100,
                                          1, 64, 1024, 0, None, dw_wide.data_ptr(), status.data_ptr(), stream)
 
-    for call, out in ((forward_pair, wide[:, :256]), (weights_pair, dw_wide[:, :256]),
+    def forced(tiles, call):
+        def run():
+            with _lib.test_option(_lib.OPT_LINEAR_TILES, tiles):
+                return call()
+        return run
+
+    for call, out in ((forced(3, forward_pair), wide[:, :256]), (weights_pair, dw_wide[:, :256]),
+                      (forced(2, forward), y), (forced(2, lambda: fp8(70)), y8),
                       (forward, y), (lambda: backward(1, 0), dx), (lambda: backward(0, 1), dw),
-                      (lambda: backward(1, 1), dw), (lambda: fp8(20), y8[:20]), (lambda: fp8(70), y8)):
+                      (lambda: backward(1, 1), dw), (lambda: fp8(20), y8[:20])):
         with _lib.test_option(_lib.OPT_TEST_DROP_SENDS, 1):
             assert call() == 0
             assert lib.bcjr_ws_status(ctypes.c_void_p(status.data_ptr()), stream) == _lib.BCJR_ERR_TIMEOUT
