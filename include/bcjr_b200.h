@@ -295,8 +295,7 @@ BCJR_API int bcjr_hyb_codebook(const float *lut, int Q, int L, float *cb_out, bc
  * Linear layers around the quantizers: products grouped by expert (16-bit
  * types) and an 8-bit floating point product with a scale for each block of
  * 128.  No counterpart in the reference, whose QuantizedLinear multiplies with
- * torch (src/qat/quantized_linear.py:309-315) and whose MoE layers loop over
- * the experts (src/qat/qat_moe_layer.py).
+ * torch (src/qat/quantized_linear.py:309-315).
  *
  * Common to the entry points: T rows (0 <= T < 2^31 - 256) in E groups
  * (1 <= E <= 1024); group e holds rows offsets[e] .. offsets[e + 1] - 1.

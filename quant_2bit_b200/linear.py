@@ -2,8 +2,7 @@
 8-bit floating point with a scale for each block of 128.
 
 The reference's QuantizedLinear multiplies its quantized weight with torch
-(src/qat/quantized_linear.py:309-315), and its MoE layers loop over the experts
-(src/qat/qat_moe_layer.py).  Here one launch serves all experts of a layer
+(src/qat/quantized_linear.py:309-315).  Here one launch serves all experts of a layer
 (``quant.bcjr_quantize_layer`` quantizes them in one launch too), and layers
 that are not being trained -- the teacher, the frozen layers around the one in
 training -- can hold their weights in e4m3 and still pass gradients on.
