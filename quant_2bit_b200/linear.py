@@ -21,6 +21,9 @@ Every op runs the sm_100a kernels of libbcjr_b200.so on the caller's current
 stream, reads ``offsets`` on the device only, and never synchronises.  There is
 no CPU path: CPU tensors raise RuntimeError, wrong shapes AssertionError, wrong
 types ValueError.  Feature counts are multiples of 16 (the quantizers' tile).
+All of it can be captured into CUDA graphs, backward passes included; as for
+any torch op, no eager graph of the same leaves may be alive during the capture
+(torch then makes the capturing stream wait for the leaf's own and raises).
 """
 import torch
 from torch.autograd.function import once_differentiable

@@ -295,6 +295,34 @@ def test_captured_and_replayed_with_other_rows_and_groups(cuda_ok):
         assert all(torch.equal(a, b) for a, b in zip(got, step()))
 
 
+def test_two_graphs_in_turn_and_other_streams(cuda_ok):
+    """Two captured graphs of the 8-bit layer (quantizer, workspace, dependent
+    launch) replayed in turn, back to back, each keep their own results."""
+    from quant_2bit_b200 import fp8_linear, fp8_quantize_weight
+    ops = []
+    for seed, (T, N, K) in enumerate(((40, 528, 1040), (700, 272, 400))):
+        x, w, _ = _inputs(T, 1, N, K, torch.bfloat16, seed)
+        q, s = fp8_quantize_weight(w[0])
+        want = fp8_linear(x, q, s)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = fp8_linear(x, q, s)
+        ops.append((graph, out, want, (x, q, s)))
+    for _ in range(20):
+        for graph, out, _, _ in ops:
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for _, out, want, _ in ops)
+    side = torch.cuda.Stream()
+    for _ in range(20):
+        ops[0][0].replay()
+        with torch.cuda.stream(side):
+            ops[1][0].replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(out, want) for _, out, want, _ in ops)
+
+
 def test_other_streams_side_by_side(cuda_ok):
     from quant_2bit_b200 import grouped_linear
     x, w, _ = _inputs(600, 3, 256, 512, torch.bfloat16)
