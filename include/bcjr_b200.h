@@ -358,7 +358,8 @@ BCJR_API int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale
 
 /* Both steps: the rows of x (T x depth, depth = K or, with transpose_w, N;
  * BCJR_BF16 or BCJR_F16, the type of `out` too) quantized by rows into the
- * workspace, and bcjr_fp8_mm.  The workspace (16-byte aligned, of
+ * workspace, and bcjr_fp8_mm; up to 32 rows in one kernel, which uses no
+ * workspace (it may be NULL).  The workspace (16-byte aligned, of
  * bcjr_fp8_linear_workspace_bytes(T, depth) bytes, 0 for a bad size) is free
  * again when the call has run on the stream. */
 BCJR_API size_t bcjr_fp8_linear_workspace_bytes(long T, int depth);

@@ -23,61 +23,6 @@ namespace bcjr {
 namespace mm {
 namespace {
 
-constexpr float kMax = 448.f;
-
-// Maximum that keeps a NaN.
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float block_amax(float a) { return max_nan(a, 0x1p-100f); }
-__device__ __forceinline__ float block_scale(float amax) { return __fmul_rn(amax, 1.f / kMax); }
-__device__ __forceinline__ float block_inv(float amax) { return __fmul_rn(kMax, __frcp_rn(amax)); }
-
-template <typename T> __device__ __forceinline__ void load8(const T *p, float (&v)[8]);
-template <> __device__ __forceinline__ void load8(const float *p, float (&v)[8]) {
-    const float4 a = __ldcs(reinterpret_cast<const float4 *>(p));
-    const float4 b = __ldcs(reinterpret_cast<const float4 *>(p) + 1);
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-template <> __device__ __forceinline__ void load8(const __nv_bfloat16 *p, float (&v)[8]) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = __uint_as_float(w[i] << 16);
-        v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-    }
-}
-template <> __device__ __forceinline__ void load8(const __half *p, float (&v)[8]) {
-    const uint4 u = __ldcs(reinterpret_cast<const uint4 *>(p));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-    }
-}
-
-__device__ __forceinline__ float amax8(const float (&v)[8]) {
-    float m = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max_nan(m, fabsf(v[i]));
-    return m;
-}
-__device__ __forceinline__ uint2 to_e4m3(const float (&v)[8], float inv) {
-    uint16_t h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
-            : "=h"(h[i])
-            : "f"(__fmul_rn(v[2 * i + 1], inv)), "f"(__fmul_rn(v[2 * i], inv)));
-    return make_uint2(h[0] | uint32_t(h[1]) << 16, h[2] | uint32_t(h[3]) << 16);
-}
-
 constexpr int kQThreads = 256, kUnroll = 4, kQRows = kQThreads / 16;
 
 // 16 lanes per segment, 8 elements per lane (the width is a multiple of 16).
@@ -531,6 +476,11 @@ cudaError_t run_mm(const Call &c) {
     return c.which == kForward ? launch_many<OUT, kForward>(c) : launch_many<OUT, kDgrad>(c);
 }
 
+template <typename OUT>
+cudaError_t run_raw(const Call &c) {
+    return c.which == kForward ? launch_few<kE4M3, OUT, kForward, true>(c) : launch_few<kE4M3, OUT, kDgrad, true>(c);
+}
+
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 bool float_type(int d) { return d == BCJR_BF16 || d == BCJR_F16 || d == BCJR_F32; }
 int status_of(cudaError_t e) {
@@ -580,20 +530,23 @@ int bcjr_fp8_quantize_blocks(const void *w, int E, int N, int K, int dtype, void
     }
 }
 
+// How the rows of a product come: quantized; quantized by the kernel launched
+// just before; in 16 bits, for the product to quantize.
+enum { kReady = 0, kFollows = 1, kRaw = 2 };
 static int fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long scale_row,
                   long scale_block, const void *w, const float *w_scale, const void *offsets,
                   int offsets_bytes, long T, int E, int N, int K, int transpose_w, void *out,
-                  int out_dtype, int *status, bcjr_stream_t stream, int dependent) {
+                  int out_dtype, int *status, bcjr_stream_t stream, int come) {
     if (T < 0 || T > 0x7fffff00L || E < 1 || E > kMaxGroups || N < 16 || K < 16 || N % 16 || K % 16 ||
         N > (1 << 24) || K > (1 << 24))
         return BCJR_ERR_BAD_SHAPE;
     if (out_dtype != BCJR_BF16 && out_dtype != BCJR_F16) return BCJR_ERR_UNSUPPORTED;
     if (offsets ? (offsets_bytes != 4 && offsets_bytes != 8) : E != 1) return BCJR_ERR_BAD_SHAPE;
     if (T == 0) return BCJR_OK;
-    if (!rows || !rows_scale || !w || !w_scale || !out) return BCJR_ERR_NULL_POINTER;
+    if (!rows || (!rows_scale && come != kRaw) || !w || !w_scale || !out) return BCJR_ERR_NULL_POINTER;
     const int depth = transpose_w ? N : K, lanes = transpose_w ? K : N;
     if (ld_rows < depth || ld_rows > (1L << 32) || scale_row < 0 || scale_block < 0) return BCJR_ERR_BAD_SHAPE;
-    if (!aligned(rows, 16) || ld_rows % 16 || !aligned(w, 16) || !aligned(out, 16) || !aligned(status, 4) ||
+    if (!aligned(rows, 16) || ld_rows % (come == kRaw ? 8 : 16) || !aligned(w, 16) || !aligned(out, 16) || !aligned(status, 4) ||
         !aligned(rows_scale, 4) || !aligned(w_scale, 4) || (offsets && !aligned(offsets, size_t(offsets_bytes))))
         return BCJR_ERR_ALIGNMENT;
     const long kb = (K + 127) / 128, nb = (N + 127) / 128;
@@ -603,9 +556,14 @@ static int fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long 
     c.a = w;
     c.a_rows = N;
     c.a_inner = K;
-    c.b = rows;
-    c.ld_b = ld_rows;
-    c.b_inner = depth;
+    if (come == kRaw) {
+        c.p.raw = rows;
+        c.p.ld_raw = ld_rows;
+    } else {
+        c.b = rows;
+        c.ld_b = ld_rows;
+        c.b_inner = depth;
+    }
     c.stream = reinterpret_cast<cudaStream_t>(stream);
     c.p.offsets = offsets;
     c.p.offsets64 = offsets_bytes == 8;
@@ -624,8 +582,9 @@ static int fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long 
     c.p.ws_blk = transpose_w ? kb : 1;
     c.p.status = status;
     c.p.drop = bcjr::test_option(bcjr::kOptDropSends);
-    c.p.dependent = dependent;
+    c.p.dependent = come == kFollows;
     c.out_kind = out_dtype == BCJR_BF16 ? kBF16 : kF16;
+    if (come == kRaw) return status_of(out_dtype == BCJR_BF16 ? run_raw<__nv_bfloat16>(c) : run_raw<__half>(c));
     return status_of(out_dtype == BCJR_BF16 ? run_mm<__nv_bfloat16>(c) : run_mm<__half>(c));
 }
 
@@ -634,19 +593,23 @@ int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long sc
                 int offsets_bytes, long T, int E, int N, int K, int transpose_w, void *out,
                 int out_dtype, int *status, bcjr_stream_t stream) {
     return fp8_mm(rows, ld_rows, rows_scale, scale_row, scale_block, w, w_scale, offsets, offsets_bytes, T, E,
-                  N, K, transpose_w, out, out_dtype, status, stream, 0);
+                  N, K, transpose_w, out, out_dtype, status, stream, kReady);
 }
 
 // The quantized rows first, then their scales, block by block, so that a tile
 // reads those of its rows side by side.
 size_t bcjr_fp8_linear_workspace_bytes(long T, int depth) {
     if (T < 0 || T > 0x7fffff00L || depth < 16 || depth % 16 || depth > (1 << 24)) return 0;
+    if (T <= kRawRows) return 16;
     return size_t(T) * depth + size_t(T) * ((depth + 127) / 128) * 4 + 16;
 }
 
-// The product is launched to overlap the end of the quantizer: its set-up and
-// its first weight loads run before it waits for the quantized rows.  The
-// quantizer itself is an ordinary launch, so everything before it has ended.
+// Up to kRawRows rows one kernel quantizes and multiplies (one row, 8192 x 2048:
+// 12.7 us a call with its host time, 17.5 as two kernels; 9.5 and 10.4 on the
+// GPU).  With more the
+// product is launched to overlap the end of the quantizer: its set-up and its
+// first weight loads run before it waits for the quantized rows.  The quantizer
+// itself is an ordinary launch, so everything before it has ended.
 int bcjr_fp8_linear(const void *x, long ld, int dtype, const void *w, const float *w_scale,
                     const void *offsets, int offsets_bytes, long T, int E, int N, int K,
                     int transpose_w, void *out, void *ws, size_t ws_bytes, int *status,
@@ -655,13 +618,16 @@ int bcjr_fp8_linear(const void *x, long ld, int dtype, const void *w, const floa
     const int depth = transpose_w ? N : K;
     const size_t need = bcjr_fp8_linear_workspace_bytes(T, depth);
     if (!need) return BCJR_ERR_BAD_SHAPE;
-    if (T > 0 && (!ws || ws_bytes < need)) return BCJR_ERR_WORKSPACE;
+    if (T <= kRawRows)
+        return fp8_mm(x, ld, nullptr, 0, 0, w, w_scale, offsets, offsets_bytes, T, E, N, K, transpose_w, out,
+                      dtype, status, stream, kRaw);
+    if (!ws || ws_bytes < need) return BCJR_ERR_WORKSPACE;
     if (!aligned(ws, 16)) return BCJR_ERR_ALIGNMENT;
     float *scale = reinterpret_cast<float *>(static_cast<char *>(ws) + size_t(T) * depth);
     const int st = bcjr_fp8_quantize_rows(x, ld, T, depth, dtype, ws, scale, 1, T, stream);
     if (st) return st;
     return fp8_mm(ws, depth, scale, 1, T, w, w_scale, offsets, offsets_bytes, T, E, N, K, transpose_w, out,
-                  dtype, status, stream, 1);
+                  dtype, status, stream, kFollows);
 }
 
 }  // extern "C"

@@ -43,6 +43,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include "bcjr_e4m3.cuh"
 #include "bcjr_kernels.h"
 
 #include <atomic>
@@ -66,6 +67,7 @@ constexpr int kChunk = 32;                        // columns that a half of the 
 constexpr int kPitch = kLanes * 2 + 16;           // bytes of a staged output row: 16-byte pieces of
                                                   // 8 rows fall into different banks
 constexpr int kMaxGroups = 1024;
+constexpr int kRawRows = 32;                      // rows that the e4m3 product quantizes itself
 constexpr int kMaxSplit = 4;                      // blocks of a cluster that share a tile
 constexpr int kBoxRows = 64;                      // rows of one TMA box
 constexpr long long kWaitLimitClocks = 2000000000ll;   // about 1 s
@@ -79,6 +81,8 @@ struct Params {
     void *out;
     long ldo;                 // elements between output rows (columns of D)
     long out_group;           // elements between groups of the output (wgrad)
+    const void *raw;          // e4m3, quantized here: the rows, of the output's type,
+    long ld_raw;              // and the elements between them
     const float *xs;          // e4m3: row scales, element (row, block) at row xs_row + block xs_blk
     long xs_row, xs_blk;
     const float *ws;          // e4m3: weight scales, (group, lane block, contraction block)
@@ -729,8 +733,9 @@ __device__ __forceinline__ bool add_parts(const float (&v)[2][16], float (*part)
 }
 
 // KIND: element type; OUT: output type; WHICH: product; COLS: columns of a
-// tile; STAGES: depth of the shared-memory ring; MODE: blocks to a tile.
-template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, int MODE>
+// tile; STAGES: depth of the shared-memory ring; MODE: blocks to a tile; RAW: the
+// rows are 16-bit and the kernel quantizes them (e4m3, at most kRawRows).
+template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, int MODE, bool RAW>
 __global__ void __launch_bounds__(kThreads, 1)
 mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb,
           const __grid_constant__ Params p) {
@@ -751,6 +756,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     static_assert(KIND != kE4M3 || (WHICH != kWgrad && COLS == 64), "e4m3: few rows, forward and dgrad");
     static_assert(BK % kBoxRows == 0 && COLS % 32 == 0, "");
     static_assert(!PAIR || KIND != kE4M3, "pairs: 16-bit types");
+    static_assert(!RAW || KIND == kE4M3, "");
 
     extern __shared__ unsigned char raw[];
     unsigned char *buf = reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -761,9 +767,10 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
-            // a pair's rank 0 is told by both: by their loads (full), or for the
-            // weights' gradient by the warps that zero (zeroed)
-            bar_init(smem_u32(&ctl.full[i]), PAIR && !B_MN ? 2 : 1);
+            // full: the loads, and with RAW the warp that quantizes.  A pair's
+            // rank 0 is told by both blocks: by their loads, or for the weights'
+            // gradient by the warps that zero (zeroed).
+            bar_init(smem_u32(&ctl.full[i]), RAW || (PAIR && !B_MN) ? 2 : 1);
             bar_init(smem_u32(&ctl.empty[i]), B_MN && !PAIR ? 2 : 1);
             bar_init(smem_u32(&ctl.zeroed[i]), PAIR ? 2 : 1);
         }
@@ -774,7 +781,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
         bar_init(smem_u32(&ctl.done), 1);
         if constexpr (SPLIT) bar_init(smem_u32(&ctl.pfull), kEpiWarps * cluster_size());
         for (int i = 0; i < kScaleStages; ++i) {
-            bar_init(smem_u32(&ctl.sfull[i]), 64);
+            bar_init(smem_u32(&ctl.sfull[i]), RAW ? 1 : 64);
             bar_init(smem_u32(&ctl.sempty[i]), kEpiWarps);
         }
         ctl.fail = 0;
@@ -820,7 +827,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                     const uint32_t bar = full(s), a = smem_u32(buf + s * S::kStage);
                     const int boxes = (cols(t) + (B_MN ? MNB : kBoxRows) - 1) / (B_MN ? MNB : kBoxRows);
                     const int kc = t.k0 + kb * BK;
-                    const uint32_t bytes = S::kA + boxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes);
+                    const uint32_t bytes = S::kA + (RAW ? 0 : boxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes));
                     if constexpr (PAIR && !B_MN) pair_expect(bar, bytes);
                     else bar_expect(bar, bytes);
                     if constexpr (WHICH == kForward) {
@@ -855,7 +862,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                             }
                             if (!drop || it) load_a(t, kb, s);
                         }
-                        if (drop && it == 0) continue;
+                        if (RAW || (drop && it == 0)) continue;
                         const uint32_t bar = full(s), b = smem_u32(buf + s * S::kStage) + S::kA;
                         const int kc = t.k0 + kb * BK, n = cols(t), c = t.col0 + int(rank) * n;
                         if constexpr (B_MN) {
@@ -956,6 +963,68 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                         }
                     }
                 }
+            }
+        } else if constexpr (RAW) {
+            // The rows of a k block, quantized into the stage by one of two warps
+            // in turn: half a warp per row, 8 elements a lane, loaded two k blocks
+            // ahead.  Every block does its own (a few KB of rows for 16 KB of
+            // weights a stage); a kernel of their own would cost a launch and its
+            // workspace.
+            constexpr int PASSES = kRawRows / 2;
+            const int odd = warp - kScaleWarp, sub = lane & 15, first = lane >> 4;
+            uint32_t it0 = 0;                       // stages of the tiles before
+            bool ok = true;
+            while (ok && walk.next(t)) {
+                const float *ws = p.ws + t.group * p.ws_group + t.lane_tile * p.ws_lane + t.k0 / BK * p.ws_blk;
+                const OUT *x = static_cast<const OUT *>(p.raw) + (t.col0 + first) * p.ld_raw + t.k0 + sub * 8;
+                uint4 v[PASSES];
+                float w = 0.f;
+                auto fetch = [&](int kb) {
+                    if (kb >= t.nkb) return;
+                    w = ws[kb * p.ws_blk];
+#pragma unroll
+                    for (int i = 0; i < PASSES; ++i) {
+                        if (i * 2 >= t.valid) break;
+                        v[i] = make_uint4(0, 0, 0, 0);
+                        if (i * 2 + first < t.valid && kb * BK + sub * 8 < t.depth)
+                            v[i] = __ldg(reinterpret_cast<const uint4 *>(x + i * 2 * p.ld_raw + kb * BK));
+                    }
+                };
+                int kb = (odd ^ it0) & 1;           // the warp of an even (odd) count of stages
+                fetch(kb);
+                for (; kb < t.nkb; kb += 2) {
+                    const uint32_t it = it0 + kb, s = it % STAGES, z = it % kScaleStages;
+                    ok = warp_wait(smem_u32(&ctl.empty[s]), ((it / STAGES) & 1) ^ 1, fail, p.status) &&
+                         warp_wait(smem_u32(&ctl.sempty[z]), ((it / kScaleStages) & 1) ^ 1, fail, p.status);
+                    if (!ok) break;
+                    unsigned char *b = buf + s * S::kStage + S::kA;
+#pragma unroll
+                    for (int i = 0; i < PASSES; ++i) {
+                        if (i * 2 >= t.valid) break;
+                        float f[8];
+                        unpack8<OUT>(v[i], f);
+                        float m = amax8(f);
+#pragma unroll
+                        for (int d = 8; d; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+                        m = block_amax(m);
+                        const int r = i * 2 + first;
+                        if (r < t.valid) {
+                            // 16-byte pieces of a row change places by the row (128-byte swizzle)
+                            *reinterpret_cast<uint2 *>(b + r * kRowBytes + (((sub >> 1) ^ r) & 7) * 16 + (sub & 1) * 8) =
+                                to_e4m3(f, block_inv(m));
+                            if (sub == 0) ctl.xs[z][r] = block_scale(m);
+                        }
+                    }
+                    if (lane == 0) ctl.ws[z] = w;
+                    fence_async();
+                    __syncwarp();
+                    if (lane == 0) {
+                        bar_arrive(smem_u32(&ctl.full[s]));
+                        bar_arrive(smem_u32(&ctl.sfull[z]));
+                    }
+                    fetch(kb + 2);
+                }
+                it0 += t.nkb;
             }
         } else if constexpr (KIND == kE4M3) {
             // Scales of the rows and of the weight block, one slot for each k
@@ -1132,7 +1201,7 @@ struct Call {
 
 // Both operand maps of a call.
 template <int KIND, int WHICH>
-bool make_maps(const Call &c, CUtensorMap &ta, CUtensorMap &tb) {
+bool make_maps(const Call &c, CUtensorMap &ta, CUtensorMap &tb, bool raw) {
     constexpr unsigned es = KIND == kE4M3 ? 1 : 2, inner = kRowBytes / es;
     using U = unsigned long long;
     if (WHICH == kWgrad) {
@@ -1144,6 +1213,10 @@ bool make_maps(const Call &c, CUtensorMap &ta, CUtensorMap &tb) {
         const U st[2] = {U(c.a_inner) * es, U(c.a_inner) * U(c.a_rows) * es};
         const unsigned box[3] = {inner, WHICH == kForward ? unsigned(kLanes) : inner, 1};
         if (!make_map(&ta, KIND, 3, c.a, dims, st, box)) return false;
+    }
+    if (raw) {                 // the kernel loads the rows itself
+        tb = ta;
+        return true;
     }
     const U dims[2] = {U(c.b_inner), U(c.p.T)}, st[1] = {U(c.ld_b) * es};
     const unsigned box[2] = {inner, WHICH == kWgrad ? inner : unsigned(kBoxRows)};
@@ -1195,14 +1268,14 @@ cudaError_t set_up(K k, size_t bytes, int regs, std::atomic<bool> &ready) {
     return cudaSuccess;
 }
 
-template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, int MODE>
+template <int KIND, typename OUT, int WHICH, int COLS, int STAGES, int MODE, bool RAW = false>
 cudaError_t launch(const Call &c) {
     CUtensorMap ta, tb;
     int dev = 0;
     const int sms = grid_sms(&dev);
     if (sms <= 0) return cudaErrorInvalidDevice;
-    if (!make_maps<KIND, WHICH>(c, ta, tb)) return cudaErrorInvalidValue;
-    const auto k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES, MODE>;
+    if (!make_maps<KIND, WHICH>(c, ta, tb, RAW)) return cudaErrorInvalidValue;
+    const auto k = &mm_kernel<KIND, OUT, WHICH, COLS, STAGES, MODE, RAW>;
     constexpr size_t bytes = Smem<KIND, COLS, STAGES, MODE>::bytes();
     static_assert(bytes <= 232448, "shared memory of one block");
     static std::atomic<bool> ready[kMaxDevices];
@@ -1263,12 +1336,12 @@ inline bool few_rows(const Call &c) {
     const long lanes = in_pairs(c) ? 2 * kLanes : kLanes, slots = in_pairs(c) ? (sms > 1 ? sms / 2 : 1) : sms;
     return 3 * few < 5 * waves((c.p.lanes + lanes - 1) / lanes * max_col_tiles<256>(c), slots) * nkb;
 }
-template <int KIND, typename OUT, int WHICH>
+template <int KIND, typename OUT, int WHICH, bool RAW = false>
 cudaError_t launch_few(Call c) {
     int dev = 0;
     c.split = few_split(c, grid_sms(&dev));
-    if (c.split == 1) return launch<KIND, OUT, WHICH, 64, 8, kAlone>(c);
-    return launch<KIND, OUT, WHICH, 64, 6, kSplit>(c);
+    if (c.split == 1) return launch<KIND, OUT, WHICH, 64, 8, kAlone, RAW>(c);
+    return launch<KIND, OUT, WHICH, 64, 6, kSplit, RAW>(c);
 }
 
 }  // namespace mm

@@ -33,6 +33,7 @@ from . import _lib
 _BLOCK = 128
 _TILE = 16
 _MAX_GROUPS = 1024
+_RAW_ROWS = 32             # up to here the 8-bit layer needs no workspace
 _F8 = torch.float8_e4m3fn
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
 _HALVES = (torch.bfloat16, torch.float16)
@@ -311,14 +312,16 @@ def _quantized_product(x, q, scale, offsets, transpose):
     out = x.new_empty(T, K if transpose else N)
     if T == 0:
         return out
-    size = T * (C + 4 * _blocks(C)) + 16          # bcjr_fp8_linear_workspace_bytes
-    ws = x.new_empty(size, dtype=torch.uint8)
+    size, ws = 0, None
+    if T > _RAW_ROWS:
+        size = T * (C + 4 * _blocks(C)) + 16      # bcjr_fp8_linear_workspace_bytes
+        ws = x.new_empty(size, dtype=torch.uint8)
     x, ld = _rows(x)
     q, scale = _dense(q), _dense(scale)
     off_ptr, off_size = _bounds(offsets)
     _call(_lib.load().bcjr_fp8_linear, x.get_device(), x.data_ptr(), ld, _DTYPES[x.dtype], q.data_ptr(),
           scale.data_ptr(), off_ptr, off_size, T, E, N, K, transpose, out.data_ptr(),
-          ws.data_ptr(), size, None)
+          None if ws is None else ws.data_ptr(), size, None)
     return out
 
 

@@ -493,7 +493,8 @@ def _check_fp8(x, q, s, w64, dy, offsets):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("T,N,K", [(1, 16, 16), (1, 128, 256), (17, 144, 272), (64, 2000, 400),
                                    (65, 48, 128), (300, 272, 1040), (513, 128, 144), (37, 48, 4240), (1, 2064, 528),
-                                   (64, 144, 1280), (200, 656, 304), (129, 16, 16)])
+                                   (64, 144, 1280), (200, 656, 304), (129, 16, 16), (2, 1040, 2064),
+                                   (31, 272, 4112), (32, 4112, 144), (33, 144, 4112)])
 def test_fp8_linear_forward_and_gradient(cuda_ok, T, N, K, dtype, tiles):
     from quant_2bit_b200 import _lib
     x, q, s, w64, dy = _fp8_operands(T, 0, N, K, dtype, seed=T)
@@ -504,7 +505,7 @@ def test_fp8_linear_forward_and_gradient(cuda_ok, T, N, K, dtype, tiles):
 @pytest.mark.parametrize("tiles", [0, 1, 2])
 @pytest.mark.parametrize("counts,N,K", [([3, 0, 1, 12], 144, 272), ([130, 0, 300, 70], 272, 144),
                                         ([0, 0], 128, 128), ([257, 1], 128, 384),
-                                        ([9, 0, 1], 144, 2064),
+                                        ([9, 0, 1], 144, 2064), ([1, 5, 0, 20], 400, 272), ([0, 26], 2064, 656),
                                         ([90, 0, 3, 1, 20, 0, 0, 0, 2], 208, 272)])
 def test_fp8_linear_by_expert(cuda_ok, counts, N, K, tiles):
     T = sum(counts) + 6
@@ -540,11 +541,36 @@ def test_fp8_matmul_takes_any_scales(cuda_ok):
         a = _expand(xq, s, 1)
         for dt in (torch.bfloat16, torch.float16):
             _close(fp8_matmul(xq, s, q, ws, out_dtype=dt), a @ b.t(), a.abs() @ b.abs().t(), K, "y", extra=4)
+    for t in (1, 17):          # few quantized rows (the layer quantizes those itself)
+        _close(fp8_matmul(xq[:t], xs[:t], q, ws), _expand(xq[:t], xs[:t], 1) @ b.t(),
+               _expand(xq[:t], xs[:t], 1).abs() @ b.abs().t(), K, "y", extra=4)
     wide = torch.zeros(T, K + 48, dtype=torch.uint8, device="cuda").view(F8)
     wide[:, 16:16 + K] = xq
     assert torch.equal(fp8_matmul(wide[:, 16:16 + K], xs, q, ws), fp8_matmul(xq, xs, q, ws))
     assert torch.equal(fp8_matmul(wide[:, 16:16 + K], xs[:1].expand(T, 4), q, ws),
                        fp8_matmul(xq, xs[:1].repeat(T, 1), q, ws))
+
+
+def test_few_and_many_rows_of_the_fp8_layer_agree(cuda_ok):
+    """Up to 32 rows one kernel quantizes and multiplies, above two do: the same
+    codes, scales and (in 64 columns) sums, also for strided rows, extreme and
+    non-finite values."""
+    from quant_2bit_b200 import _lib, fp8_linear, fp8_matmul, fp8_quantize_rows, fp8_quantize_weight
+    g = torch.Generator(device="cuda").manual_seed(9)
+    for T, N, K in ((1, 144, 272), (13, 528, 2064), (32, 16, 144)):
+        wide = torch.randn(T, K + 24, generator=g, device="cuda").to(torch.bfloat16)
+        x = wide[:, 8:8 + K]
+        x[0, :16] = 0
+        x[T // 2, 3] = 3e38
+        if T > 2:
+            x[1], x[2, 5] = 1e-40, float("inf")
+            x[T - 1, K - 1] = float("nan")
+        q, s = fp8_quantize_weight(torch.randn(N, K, generator=g, device="cuda"))
+        with _lib.test_option(_lib.OPT_LINEAR_TILES, 1):
+            want = fp8_matmul(*fp8_quantize_rows(x), q, s)
+        got = fp8_linear(x, q, s)
+        assert torch.equal(got.isnan(), want.isnan())
+        assert torch.equal(got.nan_to_num(0.0), want.nan_to_num(0.0))
 
 
 def test_fp8_leading_axes_and_empty(cuda_ok):

@@ -66,23 +66,29 @@ def test_products_refuse_bad_pointers_and_strides(lib):
 
 
 def test_fp8_linear_refuses(lib):
-    def call(x=P, ld=64, dtype=0, w=P, s=P, T=8, N=32, K=64, tr=0, out=P, ws=P, size=1 << 20):
+    def call(x=P, ld=64, dtype=0, w=P, s=P, T=40, N=32, K=64, tr=0, out=P, ws=P, size=1 << 20):
         return lib.bcjr_fp8_linear(x, ld, dtype, w, s, P, 4, T, 2, N, K, tr, out, ws, size, None, None)
 
-    need = lib.bcjr_fp8_linear_workspace_bytes(8, 64)
-    assert need >= 8 * 64 + 8 * 4 and lib.bcjr_fp8_linear_workspace_bytes(8, 40) == 0
+    need = lib.bcjr_fp8_linear_workspace_bytes(40, 64)
+    assert need >= 40 * 64 + 40 * 4 and lib.bcjr_fp8_linear_workspace_bytes(8, 40) == 0
     assert call(size=need - 1) == call(ws=None) == 5
     assert call(dtype=2) == UNSUPPORTED
     assert call(K=40) == call(T=-1) == call(ld=32) == SHAPE
     assert call(x=P + 8) == call(ws=P + 8) == ALIGN
     assert call(x=None) == NULL
     assert call(T=0, x=None, ws=None) == OK
+    # few rows: no workspace, the other checks as before
+    assert call(T=8, ws=None, size=0, dtype=2) == UNSUPPORTED
+    assert call(T=8, ws=None, size=0, x=P + 8) == call(T=8, ws=None, ld=68) == ALIGN
+    assert call(T=8, ws=None, w=None) == call(T=8, ws=None, x=None) == NULL
+    assert call(T=8, ws=None, ld=32) == SHAPE
 
 
 def test_workspace_formula(lib):
     """The binding sizes the workspace by the library's formula."""
     from quant_2bit_b200 import linear
-    for T, C in ((1, 16), (7, 144), (4097, 2048)):
+    assert lib.bcjr_fp8_linear_workspace_bytes(linear._RAW_ROWS, 144) == 16      # not used
+    for T, C in ((linear._RAW_ROWS + 1, 16), (64, 144), (4097, 2048)):
         assert lib.bcjr_fp8_linear_workspace_bytes(T, C) == T * (C + 4 * linear._blocks(C)) + 16
 
 
