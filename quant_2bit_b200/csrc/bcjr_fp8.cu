@@ -606,10 +606,10 @@ size_t bcjr_fp8_linear_workspace_bytes(long T, int depth) {
 
 // Up to kRawRows rows one kernel quantizes and multiplies (one row, 8192 x 2048:
 // 12.7 us a call with its host time, 17.5 as two kernels; 9.5 and 10.4 on the
-// GPU).  With more the
-// product is launched to overlap the end of the quantizer: its set-up and its
-// first weight loads run before it waits for the quantized rows.  The quantizer
-// itself is an ordinary launch, so everything before it has ended.
+// GPU).  With more the product is launched to overlap the end of the quantizer:
+// its set-up and its first weight loads run before it waits for the quantized
+// rows.  The quantizer itself is an ordinary launch, so everything before it has
+// ended.
 int bcjr_fp8_linear(const void *x, long ld, int dtype, const void *w, const float *w_scale,
                     const void *offsets, int offsets_bytes, long T, int E, int N, int K,
                     int transpose_w, void *out, void *ws, size_t ws_bytes, int *status,
