@@ -641,7 +641,7 @@ struct Smem {
     // (one token, 8192 x 2048: 740 clocks a block with two, 630 with eight).
     static constexpr int kAcc = KIND == kE4M3 ? 8 : 2;
     struct Ctl {
-        unsigned long long full[STAGES], empty[STAGES], zeroed[STAGES], tfull[kAcc], tempty[kAcc], done;
+        unsigned long long full[STAGES], empty[STAGES], zeroed[STAGES], ragged[STAGES], tfull[kAcc], tempty[kAcc], done;
         unsigned long long sfull[kScaleStages], sempty[kScaleStages];
         uint32_t tmem;
         int fail;
@@ -768,11 +768,12 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     if (threadIdx.x == 0) {
         for (int i = 0; i < STAGES; ++i) {
             // full: the loads, and with RAW the warp that quantizes.  A pair's
-            // rank 0 is told by both blocks: by their loads, or for the weights'
-            // gradient by the warps that zero (zeroed).
-            bar_init(smem_u32(&ctl.full[i]), RAW || (PAIR && !B_MN) ? 2 : 1);
+            // rank 0 is told by both blocks: by their loads, or by the warps that
+            // zero the end of a group (which the loads tell first, on `ragged`).
+            bar_init(smem_u32(&ctl.full[i]), RAW || PAIR ? 2 : 1);
             bar_init(smem_u32(&ctl.empty[i]), B_MN && !PAIR ? 2 : 1);
-            bar_init(smem_u32(&ctl.zeroed[i]), PAIR ? 2 : 1);
+            bar_init(smem_u32(&ctl.zeroed[i]), 1);
+            bar_init(smem_u32(&ctl.ragged[i]), 1);
         }
         for (int i = 0; i < ACC; ++i) {
             bar_init(smem_u32(&ctl.tfull[i]), 1);
@@ -819,7 +820,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 auto cols = [&](const Tile &t) { return PAIR ? t.ncols / 2 : t.ncols; };
                 auto full = [&](uint32_t s) {
                     const uint32_t bar = smem_u32(&ctl.full[s]);
-                    return PAIR && !B_MN ? in_rank(bar, 0) : bar;
+                    return PAIR ? in_rank(bar, 0) : bar;
                 };
                 // Arms the stage's barrier for both operands and loads the one
                 // that has the output's lanes.
@@ -828,7 +829,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                     const int boxes = (cols(t) + (B_MN ? MNB : kBoxRows) - 1) / (B_MN ? MNB : kBoxRows);
                     const int kc = t.k0 + kb * BK;
                     const uint32_t bytes = S::kA + (RAW ? 0 : boxes * (B_MN ? MN_BLOCK : kBoxRows * kRowBytes));
-                    if constexpr (PAIR && !B_MN) pair_expect(bar, bytes);
+                    if constexpr (PAIR) pair_expect(bar, bytes);
                     else bar_expect(bar, bytes);
                     if constexpr (WHICH == kForward) {
                         if constexpr (PAIR) pair_tma3(a, &ta, kc, lanes_at(t), t.group, bar);
@@ -837,11 +838,26 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
 #pragma unroll
                         for (int j = 0; j < kLanes / MNB; ++j) {
                             const int x = lanes_at(t) + j * MNB;
-                            if constexpr (WHICH == kWgrad) tma2(a + j * MN_BLOCK, &ta, x, kc, bar);
+                            if constexpr (PAIR && B_MN) pair_tma2(a + j * MN_BLOCK, &ta, x, kc, bar);
+                            else if constexpr (B_MN) tma2(a + j * MN_BLOCK, &ta, x, kc, bar);
                             else if constexpr (PAIR) pair_tma3(a + j * MN_BLOCK, &ta, x, kc, t.group, bar);
                             else tma3(a + j * MN_BLOCK, &ta, x, kc, t.group, bar);
                         }
                     }
+                };
+                // The end of a group in a pair's weights' gradient: both operands,
+                // complete on a barrier of this block, for the warp that zeroes.
+                // `own` has a bit for every stage whose last load was such an
+                // end, `turn` the phase of its next one.
+                uint32_t own = 0, turn = 0;
+                auto load_end = [&](const Tile &t, int kb, uint32_t s) {
+                    const uint32_t bar = smem_u32(&ctl.ragged[s]), a = smem_u32(buf + s * S::kStage);
+                    const int kc = t.k0 + kb * BK, n = cols(t), c = t.col0 + int(rank) * n;
+                    bar_expect(bar, S::kA + (n + MNB - 1) / MNB * MN_BLOCK);
+                    for (int j = 0; j < kLanes / MNB; ++j) tma2(a + j * MN_BLOCK, &ta, lanes_at(t) + j * MNB, kc, bar);
+                    for (int j = 0; j * MNB < n; ++j) tma2(a + S::kA + j * MN_BLOCK, &tb, c + j * MNB, kc, bar);
+                    own |= 1u << s;
+                    turn ^= 1u << s;
                 };
                 const bool drop = p.drop && blockIdx.x == 0;      // test option: the first load is withheld
                 if (p.dependent) {
@@ -860,13 +876,21 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                                 ok = false;
                                 break;
                             }
+                            if (PAIR && B_MN && t.depth - kb * BK < BK) {
+                                if (!drop || it) load_end(t, kb, s);
+                                continue;
+                            }
+                            own &= ~(1u << s);
                             if (!drop || it) load_a(t, kb, s);
                         }
                         if (RAW || (drop && it == 0)) continue;
                         const uint32_t bar = full(s), b = smem_u32(buf + s * S::kStage) + S::kA;
                         const int kc = t.k0 + kb * BK, n = cols(t), c = t.col0 + int(rank) * n;
                         if constexpr (B_MN) {
-                            for (int j = 0; j * MNB < n; ++j) tma2(b + j * MN_BLOCK, &tb, c + j * MNB, kc, bar);
+                            for (int j = 0; j * MNB < n; ++j) {
+                                if constexpr (PAIR) pair_tma2(b + j * MN_BLOCK, &tb, c + j * MNB, kc, bar);
+                                else tma2(b + j * MN_BLOCK, &tb, c + j * MNB, kc, bar);
+                            }
                         } else {
                             for (int j = 0; j * kBoxRows < n; ++j) {
                                 if constexpr (PAIR) pair_tma2(b + j * kBoxRows * kRowBytes, &tb, kc, c + j * kBoxRows, bar);
@@ -875,12 +899,16 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                         }
                     }
                 }
-                if (!ok && (rank == 0 || B_MN)) {
-                    // copies in flight land before the block (the pair) ends
+                if (!ok) {
+                    // copies in flight land before the block (the pair) ends:
+                    // rank 0 knows of the loads that complete on its barriers
                     volatile int never = 0;
-                    for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i)
-                        if (!(drop && i == 0))
-                            bar_wait<PAIR>(smem_u32(&ctl.full[i % STAGES]), (i / STAGES) & 1, &never, nullptr);
+                    for (uint32_t i = it > STAGES ? it - STAGES : 0; i < it; ++i) {
+                        const uint32_t s = i % STAGES;
+                        if (drop && i == 0) continue;
+                        if (own >> s & 1) bar_wait(smem_u32(&ctl.ragged[s]), (turn >> s & 1) ^ 1, &never, nullptr);
+                        else if (rank == 0) bar_wait<PAIR>(smem_u32(&ctl.full[s]), (i / STAGES) & 1, &never, nullptr);
+                    }
                 }
             }
         } else if (warp == kMmaWarp && rank == 0) {
@@ -899,7 +927,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                         if (KIND == kE4M3 || kb == 0)
                             ok = bar_wait<PAIR>(smem_u32(&ctl.tempty[acc % ACC]), ((acc / ACC) & 1) ^ 1, fail, p.status);
                         if (ok)
-                            ok = bar_wait<PAIR>(smem_u32(B_MN && (PAIR || t.depth - kb * BK < BK) ? &ctl.zeroed[s] : &ctl.full[s]),
+                            ok = bar_wait<PAIR>(smem_u32(B_MN && !PAIR && t.depth - kb * BK < BK ? &ctl.zeroed[s] : &ctl.full[s]),
                                                 (it / STAGES) & 1, fail, p.status);
                         if (!ok) break;
                         tc_fence_after();
@@ -931,33 +959,54 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
             // The rows of a group's last stage that belong to the next group (or
             // lie behind the last one) do not count, whatever they hold: one
             // warp makes them zero in both factors before they are multiplied.
-            // It follows every stage, and a stage is loaded again only after it,
-            // so that nobody mistakes a barrier's phase.  In a pair both blocks'
-            // warps tell rank 0 of every stage.
+            auto zero_end = [&](uint32_t s, int rows, int n) {
+                unsigned char *a = buf + s * S::kStage;
+                const int cells = (BK - rows) * (kRowBytes / 16);
+                const int blocks = kLanes / MNB + (n + MNB - 1) / MNB;
+                for (int j = 0; j < blocks; ++j) {
+                    uint4 *z = reinterpret_cast<uint4 *>(a + j * MN_BLOCK + rows * kRowBytes);
+                    for (int i = lane; i < cells; i += 32) z[i] = make_uint4(0, 0, 0, 0);
+                }
+                fence_async();
+                __syncwarp();
+            };
             uint32_t it = 0;
             bool ok = warp == kScaleWarp;
-            while (ok && walk.next(t)) {
-                for (int kb = 0; kb < t.nkb; ++kb, ++it) {
-                    const uint32_t s = it % STAGES;
-                    ok = warp_wait(smem_u32(&ctl.full[s]), (it / STAGES) & 1, fail, p.status);
+            if constexpr (PAIR) {
+                // Both blocks' warps tell rank 0 of a group's last stage, with a
+                // release: the zeros and the loads that the warp saw are there.
+                // All other stages' loads complete on rank 0's barrier by
+                // themselves: a warp that handed those on as well would need
+                // such a release for every stage (a relaxed arrival orders no
+                // load before rank 0's products), which takes longer than the
+                // stage's products.  A wait may last as long as the tiles since
+                // the last one, with 32 stages' time for each one's stores.
+                uint32_t turn = 0;                  // phase of each stage's `ragged`
+                int passed = 0;
+                while (ok && walk.next(t)) {
+                    it += t.nkb;
+                    passed += t.nkb + 32;
+                    const int rows = t.depth - (t.nkb - 1) * BK;
+                    if (t.nkb == 0 || rows == BK) continue;
+                    const uint32_t s = (it - 1) % STAGES;
+                    ok = warp_wait(smem_u32(&ctl.ragged[s]), turn >> s & 1, fail, p.status, passed);
                     if (!ok) break;
-                    const int rows = t.depth - kb * BK, n = PAIR ? t.ncols / 2 : t.ncols;
-                    if (rows < BK) {
-                        unsigned char *a = buf + s * S::kStage;
-                        const int cells = (BK - rows) * (kRowBytes / 16);
-                        const int blocks = kLanes / MNB + (n + MNB - 1) / MNB;
-                        for (int j = 0; j < blocks; ++j) {
-                            uint4 *z = reinterpret_cast<uint4 *>(a + j * MN_BLOCK + rows * kRowBytes);
-                            for (int i = lane; i < cells; i += 32) z[i] = make_uint4(0, 0, 0, 0);
-                        }
-                        fence_async();
-                        __syncwarp();
-                    }
-                    if (lane == 0) {
-                        if constexpr (PAIR) {
-                            if (rows < BK) bar_arrive_in(smem_u32(&ctl.zeroed[s]), 0);
-                            else bar_arrive_relaxed_in(smem_u32(&ctl.zeroed[s]), 0);
-                        } else {
+                    turn ^= 1u << s;
+                    passed = 0;
+                    zero_end(s, rows, t.ncols / 2);
+                    if (lane == 0) bar_arrive_in(smem_u32(&ctl.full[s]), 0);
+                }
+            } else {
+                // It follows every stage, and a stage is loaded again only after
+                // it, so that nobody mistakes a barrier's phase.
+                while (ok && walk.next(t)) {
+                    for (int kb = 0; kb < t.nkb; ++kb, ++it) {
+                        const uint32_t s = it % STAGES;
+                        ok = warp_wait(smem_u32(&ctl.full[s]), (it / STAGES) & 1, fail, p.status);
+                        if (!ok) break;
+                        const int rows = t.depth - kb * BK;
+                        if (rows < BK) zero_end(s, rows, t.ncols);
+                        if (lane == 0) {
                             bar_arrive(smem_u32(&ctl.zeroed[s]));
                             bar_arrive(smem_u32(&ctl.empty[s]));
                         }

@@ -1,0 +1,60 @@
+"""GPU tests of the linear layers beyond test_gpu_linear.py (whose plain products
+and tolerances they use): hand-overs inside pairs of blocks, results of a whole
+training step, what is kept and refused, and failures of shared tiles."""
+import pytest
+import torch
+
+from test_gpu_linear import _check_grouped, _close, _counts_to_offsets, _grouped64, _inputs, _wgrad64
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("counts,N,K", [
+    ([64, 1, 128, 63, 0, 65, 192, 7, 640, 64, 64, 2] * 4, 528, 1040),     # six tiles to a pair of blocks
+    ([64] * 30, 272, 1024),                                               # no stage ends inside a group
+    ([3] * 60, 1040, 272),                                                # every stage does
+    ([1000, 24, 0, 999], 32, 16),
+])
+def test_full_and_ragged_stages_of_paired_blocks(cuda_ok, counts, N, K, dtype):
+    """Contractions over the rows of a group whose last stage is full, ragged or
+    the only one, in every order, so that each stage of the ring is both; the
+    results do not change from run to run."""
+    from quant_2bit_b200 import _lib, grouped_linear
+    x, w, dy = _inputs(sum(counts), len(counts), N, K, dtype, seed=N)
+    offsets = _counts_to_offsets(counts)
+    with _lib.test_option(_lib.OPT_LINEAR_TILES, 3):
+        _check_grouped(x, w, dy, offsets)
+        w.requires_grad_()
+        first = None
+        for _ in range(20):
+            dw, = torch.autograd.grad(grouped_linear(x, w, offsets), w, dy)
+            first = dw if first is None else first
+            assert torch.equal(dw, first)
+
+
+def test_training_step_of_a_layer_repeats_itself(cuda_ok):
+    """64 experts, 32768 rows, 1024 x 2048: forward and both gradients within
+    their bounds of the 64-bit products, and the same bits every time."""
+    from quant_2bit_b200 import grouped_linear
+    E, T, N, K = 64, 32768, 1024, 2048
+    g = torch.Generator(device="cuda").manual_seed(4)
+    counts = torch.bincount(torch.multinomial(torch.rand(E, generator=g, device="cuda"), T, True,
+                                              generator=g), minlength=E).tolist()
+    offsets = _counts_to_offsets(counts)
+    x, w, dy = _inputs(T, E, N, K, torch.bfloat16)
+    x.requires_grad_()
+    w.requires_grad_()
+    first = None
+    for _ in range(10):
+        y = grouped_linear(x, w, offsets)
+        out = [y.detach(), *torch.autograd.grad(y, (x, w), dy)]
+        first = first or out
+        assert all(torch.equal(a, b) for a, b in zip(first, out))
+    y, dx, dw = first
+    ref, mag = _grouped64(x.detach(), w.detach(), offsets)
+    _close(y, ref, mag, K, "y")
+    ref, mag = _grouped64(dy, w.detach().transpose(1, 2), offsets)
+    _close(dx, ref, mag, N, "dx")
+    ref, mag = _wgrad64(dy, x.detach(), offsets, E)
+    _close(dw, ref, mag, max(counts), "dw")
