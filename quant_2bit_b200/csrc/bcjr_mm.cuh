@@ -133,17 +133,6 @@ __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Without waiting for it (try_wait may suspend the thread).
-__device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{ .reg .pred p; mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;"
-        " selp.u32 %0, 1, 0, p; }"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
 // The same for a barrier that other blocks of the cluster arrive on.
 __device__ __forceinline__ bool bar_try_cluster(uint32_t bar, uint32_t parity) {
     uint32_t ok;
@@ -950,11 +939,6 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                 volatile int never = 0;
                 bar_wait(smem_u32(&ctl.done), 0, &never, nullptr);
             }
-        } else if (PAIR && warp == kMmaWarp) {
-            // rank 1 stays until the last arrival from rank 0 is here (asked now
-            // and then: the epilogue needs the issue slots)
-            for (const long long t0 = clock64(); !bar_test(smem_u32(&ctl.done), 0) && clock64() - t0 < kWaitLimitClocks;)
-                __nanosleep(1000);
         } else if constexpr (WHICH == kWgrad) {
             // The rows of a group's last stage that belong to the next group (or
             // lie behind the last one) do not count, whatever they hold: one
@@ -1214,6 +1198,17 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
     }
     __syncwarp();
     tc_fence_before();
+    if constexpr (PAIR) {
+        // Rank 1 stays until the last arrival from rank 0 is here: when all of its
+        // own work is done that is a few products away, however long the launch
+        // has run.  (After a failure rank 0 may still be in a wait of its own.)
+        __syncthreads();
+        if (rank == 1 && threadIdx.x == 0) {
+            volatile int never = 0;
+            bar_wait<true>(smem_u32(&ctl.done), 0, &never, nullptr, int(2 * kWaitLimitClocks / 4096));
+        }
+        __syncwarp();
+    }
     if constexpr (MODE != kAlone) cluster_sync();   // nobody reads this block's sums, or its operands, any more
     else __syncthreads();
     tc_fence_after();

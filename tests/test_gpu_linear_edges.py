@@ -58,3 +58,26 @@ def test_training_step_of_a_layer_repeats_itself(cuda_ok):
     _close(dx, ref, mag, N, "dx")
     ref, mag = _wgrad64(dy, x.detach(), offsets, E)
     _close(dw, ref, mag, max(counts), "dw")
+
+
+def test_a_product_longer_than_a_wait_may_last(cuda_ok):
+    """A weights' gradient in pairs of blocks that runs for about two seconds:
+    limits count from each wait's start and grow with the work waited for.
+    (393216 rows of whole numbers up to 2 serve as both factors, so that all
+    sums are exact in fp32; 64 x 64 of the 65536 x 65536 are checked.)"""
+    import ctypes
+    from quant_2bit_b200 import _lib
+    T, N = 393216, 65536
+    lib = _lib.load()
+    x = torch.empty(T, N, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(8)
+    for rows in x.split(32768):
+        rows.random_(0, 5, generator=g).sub_(2)
+    dw = torch.zeros(N, N, dtype=torch.bfloat16, device="cuda")
+    status = torch.full((1,), 77, dtype=torch.int32, device="cuda")
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.bcjr_grouped_backward(x.data_ptr(), N, x.data_ptr(), N, None, None, 0, T, 1, N, N, 0, None,
+                                     dw.data_ptr(), status.data_ptr(), stream) == 0
+    assert lib.bcjr_ws_status(ctypes.c_void_p(status.data_ptr()), stream) == 0
+    exact = x[:, 1000:1064].double().t() @ x[:, -64:].double()
+    assert float(exact.abs().max()) < 2 ** 24 and torch.equal(dw[1000:1064, -64:], exact.to(torch.bfloat16))

@@ -18,3 +18,17 @@ def test_relaxed_arrivals_in_other_blocks_announce_no_data():
     loaded, need a release, or loads that complete on that barrier themselves."""
     barriers = re.findall(r"bar_arrive_relaxed_in\(smem_u32\(&ctl\.(\w+)", _source("bcjr_mm.cuh"))
     assert set(barriers) <= {"tempty"}, barriers
+
+
+def test_every_wait_has_its_limit_from_its_own_start():
+    """Waits are bounded in one place, by the time since the wait began and the
+    work waited for.  One bounded by the time since the kernel began would give
+    up in a healthy launch that runs longer."""
+    source = _source("bcjr_mm.cuh")
+    uses = [line.strip() for line in source.splitlines() if "kWaitLimitClocks" in line]
+    assert uses[0].startswith("constexpr long long kWaitLimitClocks")
+    for line in uses[1:]:
+        assert "clock64() - t0 > kWaitLimitClocks + 4096ll * stages" in line or "bar_wait" in line, line
+    body = source[source.index("bool bar_wait"):]
+    assert body.index("t0 = clock64()") < body.index("while (true)")
+    assert "clock64" not in source[source.index("mm_kernel("):]
