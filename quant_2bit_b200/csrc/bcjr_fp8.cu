@@ -497,7 +497,7 @@ extern "C" {
 
 int bcjr_fp8_quantize_rows(const void *x, long ld, long rows, int k, int dtype, void *q,
                            float *scale, long scale_row, long scale_block, bcjr_stream_t stream) {
-    if (rows < 0 || rows > 0x7fffff00L || k < 16 || k % 16 || k > (1 << 24) || ld < k || scale_row < 0 ||
+    if (rows < 0 || rows > kMaxRows || k < 16 || k % 16 || k > (1 << 24) || ld < k || scale_row < 0 ||
         scale_block < 0)
         return BCJR_ERR_BAD_SHAPE;
     if (!float_type(dtype)) return BCJR_ERR_UNSUPPORTED;
@@ -537,7 +537,7 @@ static int fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long 
                   long scale_block, const void *w, const float *w_scale, const void *offsets,
                   int offsets_bytes, long T, int E, int N, int K, int transpose_w, void *out,
                   int out_dtype, int *status, bcjr_stream_t stream, int come) {
-    if (T < 0 || T > 0x7fffff00L || E < 1 || E > kMaxGroups || N < 16 || K < 16 || N % 16 || K % 16 ||
+    if (T < 0 || T > kMaxRows || E < 1 || E > kMaxGroups || N < 16 || K < 16 || N % 16 || K % 16 ||
         N > (1 << 24) || K > (1 << 24))
         return BCJR_ERR_BAD_SHAPE;
     if (out_dtype != BCJR_BF16 && out_dtype != BCJR_F16) return BCJR_ERR_UNSUPPORTED;
@@ -599,7 +599,7 @@ int bcjr_fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long sc
 // The quantized rows first, then their scales, block by block, so that a tile
 // reads those of its rows side by side.
 size_t bcjr_fp8_linear_workspace_bytes(long T, int depth) {
-    if (T < 0 || T > 0x7fffff00L || depth < 16 || depth % 16 || depth > (1 << 24)) return 0;
+    if (T < 0 || T > kMaxRows || depth < 16 || depth % 16 || depth > (1 << 24)) return 0;
     if (T <= kRawRows) return 16;
     return size_t(T) * depth + size_t(T) * ((depth + 127) / 128) * 4 + 16;
 }

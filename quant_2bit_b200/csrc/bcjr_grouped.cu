@@ -25,7 +25,7 @@ cudaError_t launch_which(const Call &c) {
 bool aligned(const void *p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 int check(const void *offsets, int offsets_bytes, long T, int E, int N, int K, int dtype) {
-    if (T < 0 || T > 0x7fffff00L || E < 1 || E > kMaxGroups || N < 16 || K < 16 || N % 16 || K % 16 ||
+    if (T < 0 || T > kMaxRows || E < 1 || E > kMaxGroups || N < 16 || K < 16 || N % 16 || K % 16 ||
         N > (1 << 24) || K > (1 << 24))
         return BCJR_ERR_BAD_SHAPE;
     if (dtype != BCJR_BF16 && dtype != BCJR_F16) return BCJR_ERR_UNSUPPORTED;

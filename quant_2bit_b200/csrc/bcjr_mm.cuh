@@ -45,6 +45,7 @@
 
 #include "bcjr_e4m3.cuh"
 #include "bcjr_kernels.h"
+#include "bcjr_tiles.cuh"
 
 #include <atomic>
 #include <cstdint>
@@ -467,9 +468,6 @@ struct Groups {
     int first[kMaxGroups + 1];
 };
 
-template <int COLS>
-__device__ __forceinline__ int col_tiles(int rows) { return (rows + COLS - 1) / COLS; }
-
 // Two steps: the whole block reads the bounds, then (after a block barrier)
 // one warp makes them monotone and counts tiles.
 template <int THREADS>
@@ -576,8 +574,7 @@ struct Walk {
             t.group = group;
             const int c = place(in, ct, t.lane_tile);
             const int rows = g.off[group + 1] - g.off[group];
-            // equal shares: no small tile at the end of a group
-            const int share = ((rows + ct - 1) / ct + STEP - 1) & ~(STEP - 1);
+            const int share = tile_share(rows, ct, STEP);
             t.col0 = g.off[group] + c * share;
             t.valid = min(share, g.off[group + 1] - t.col0);
             t.ncols = (t.valid + STEP - 1) & ~(STEP - 1);
@@ -1267,12 +1264,7 @@ bool make_maps(const Call &c, CUtensorMap &ta, CUtensorMap &tb, bool raw) {
     return make_map(&tb, KIND, 2, c.b, dims, st, box);
 }
 
-// No more column tiles than this can T rows in E groups make.
-template <int COLS>
-long max_col_tiles(const Call &c) {
-    if (c.p.E == 1) return (c.p.T + COLS - 1) / COLS;
-    return c.p.T / COLS + (c.p.E < c.p.T ? c.p.E : c.p.T);
-}
+template <int COLS> long max_col_tiles(const Call &c) { return max_col_tiles<COLS>(c.p.T, c.p.E); }
 
 template <typename... A>
 cudaError_t launch_on(void (*k)(A...), long blocks, int threads, int cluster, size_t bytes,
