@@ -21,11 +21,14 @@ Every op runs the sm_100a kernels of libbcjr_b200.so on the caller's current
 stream, reads ``offsets`` on the device only, and never synchronises.  There is
 no CPU path: CPU tensors raise RuntimeError, wrong shapes AssertionError, wrong
 types ValueError.  Feature counts are multiples of 16 (the quantizers' tile).
+There is no second and no forward-mode derivative: asking for one raises
+RuntimeError (NotImplementedError for a dual tensor).
 All of it can be captured into CUDA graphs, backward passes included; as for
 any torch op, no eager graph of the same leaves may be alive during the capture
 (torch then makes the capturing stream wait for the leaf's own and raises).
 """
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -87,6 +90,12 @@ def _differentiate(backward, ctx, dy):
     if torch.is_grad_enabled():
         backward = once_differentiable(backward)
     return backward(ctx, dy)
+
+
+def _forward_mode():
+    """Inside torch.autograd.forward_ad.dual_level: an operand with a tangent does
+    not require a gradient, and the autograd Function has to refuse it."""
+    return forward_ad._current_level >= 0
 
 
 def _blocks(n):
@@ -199,7 +208,7 @@ def grouped_linear(x, weight, offsets):
     _need_features(N, "out features")
     _need_features(K, "in features")
     offsets = _need_offsets(offsets, E)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled() or _forward_mode():
         return _GroupedLinear.apply(x, weight, offsets)
     return _grouped_forward(x, weight, offsets)
 
@@ -360,7 +369,7 @@ def fp8_linear(x, q, scale, offsets=None):
     assert dims >= 1 and x.size(-1) == K, f"x must be (..., {K}), got {tuple(x.shape)}"
     assert offsets is None or dims == 2, f"x must be (T, K) with offsets, got {tuple(x.shape)}"
     rows = x if dims == 2 else x.reshape(-1, K)
-    if torch.is_grad_enabled() and x.requires_grad:
+    if x.requires_grad and torch.is_grad_enabled() or _forward_mode():
         y = _Fp8Linear.apply(rows, q, scale, offsets)
     else:
         y = _quantized_product(rows, q, scale, offsets, False)

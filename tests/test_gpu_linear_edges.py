@@ -81,3 +81,19 @@ def test_a_product_longer_than_a_wait_may_last(cuda_ok):
     assert lib.bcjr_ws_status(ctypes.c_void_p(status.data_ptr()), stream) == 0
     exact = x[:, 1000:1064].double().t() @ x[:, -64:].double()
     assert float(exact.abs().max()) < 2 ** 24 and torch.equal(dw[1000:1064, -64:], exact.to(torch.bfloat16))
+
+
+def test_forward_mode_derivatives_are_refused(cuda_ok):
+    from torch.autograd import forward_ad
+    from quant_2bit_b200 import fp8_linear, fp8_quantize_weight, grouped_linear
+    x, w, _ = _inputs(20, 2, 32, 64, torch.bfloat16)
+    offsets = _counts_to_offsets([5, 15])
+    q, s = fp8_quantize_weight(w[0])
+    want = grouped_linear(x, w, offsets), fp8_linear(x, q, s)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for f, args in ((grouped_linear, (dual, w, offsets)), (fp8_linear, (dual, q, s)),
+                        (grouped_linear, (x, forward_ad.make_dual(w, torch.ones_like(w)), offsets))):
+            with pytest.raises(NotImplementedError):
+                f(*args)
+        assert torch.equal(grouped_linear(x, w, offsets), want[0]) and torch.equal(fp8_linear(x, q, s), want[1])

@@ -2,6 +2,7 @@
 any device work, and that CPU tensors raise (there is no CPU path)."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from quant_2bit_b200 import _lib
 
@@ -119,3 +120,41 @@ def test_cpu_tensors_raise():
                     (q.fp8_matmul, (f8, torch.ones(16, 1), f8, torch.ones(1, 1)))):
         with pytest.raises(RuntimeError, match="CUDA"):
             f(*args)
+
+
+@pytest.fixture
+def stubbed(monkeypatch):
+    """The Python layer alone: CPU tensors pass and no C call is made."""
+    from quant_2bit_b200 import build, linear
+    build.build()
+    calls = []
+    monkeypatch.setattr(linear, "_need_cuda", lambda *a: -1)
+    monkeypatch.setattr(linear, "_call", lambda fn, *a: calls.append(fn.__name__))
+    return calls
+
+
+def _operands():
+    x, w = torch.zeros(4, 32, dtype=torch.bfloat16), torch.zeros(2, 16, 32, dtype=torch.bfloat16)
+    return x, w, torch.tensor([0, 1, 4]), torch.zeros(16, 32).to(torch.float8_e4m3fn), torch.ones(1, 1)
+
+
+@pytest.mark.parametrize("grad_mode", [True, False])
+def test_forward_mode_derivatives_are_refused(stubbed, grad_mode):
+    """A dual tensor does not require a gradient; its tangent must not be lost."""
+    import quant_2bit_b200 as q
+    x, w, off, f8, s = _operands()
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad_mode):
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for f, args in ((q.grouped_linear, (dual(x), w, off)), (q.grouped_linear, (x, dual(w), off)),
+                        (q.fp8_linear, (dual(x), f8, s)), (q.fp8_linear, (dual(x.view(2, 2, 32)), f8, s)),
+                        (q.fp8_linear, (x, f8, dual(s)))):
+            with pytest.raises(NotImplementedError):
+                f(*args)
+        assert q.grouped_linear(x, w, off).shape == (4, 16)          # nothing to lose
+        assert q.fp8_linear(x, f8, s).shape == (4, 16)
+    with pytest.raises(RuntimeError):
+        torch.func.jvp(lambda a: q.grouped_linear(a, w, off), (x,), (x,))
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda a: q.grouped_linear(a, w, off))(x.view(2, 2, 32))
