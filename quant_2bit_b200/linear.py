@@ -98,6 +98,14 @@ def _forward_mode():
     return forward_ad._current_level >= 0
 
 
+def _need_constant(names, *tensors):
+    """No derivative is asked for that the operator would lose."""
+    for i, t in enumerate(tensors):
+        assert not (t.requires_grad and torch.is_grad_enabled()), f"`{names.split()[i]}` has no gradient here"
+        assert not _forward_mode() or forward_ad.unpack_dual(t).tangent is None, \
+            f"`{names.split()[i]}` has no forward-mode derivative here"
+
+
 def _blocks(n):
     return -(-n // _BLOCK)
 
@@ -245,7 +253,7 @@ def fp8_quantize_rows(x):
 def fp8_quantize_weight(weight):
     """(q, scale) of a weight (N, K), or of E weights (E, N, K), bf16, fp16 or
     fp32: q e4m3 of its shape, scale fp32 ([E,] ceil(N / 128), ceil(K / 128)),
-    one for each 128 x 128 block."""
+    one for each 128 x 128 block.  Not differentiable."""
     _need_cuda("weight", weight)
     code = _DTYPES.get(weight.dtype)
     if code is None:
@@ -290,7 +298,8 @@ def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
                  with ``offsets`` (see ``grouped_linear``) (E, N, K) and theirs
     Returns (T, N) in ``out_dtype`` (bf16 or fp16).  Any fp32 scales are
     accepted; the product of two scales is formed in fp32, so it should not
-    underflow."""
+    underflow.  Not differentiable (``fp8_linear`` is): rows and scales that
+    require a gradient are refused, and the weight is constant."""
     _need_cuda("xq x_scale q scale offsets", xq, x_scale, q, scale, offsets)
     _need_dtype(xq, "xq", (_F8,))
     _need_dtype(x_scale, "x_scale", (torch.float32,))
@@ -300,6 +309,7 @@ def fp8_matmul(xq, x_scale, q, scale, offsets=None, out_dtype=torch.bfloat16):
     assert xq.dim() == 2 and xq.shape[1] == K, f"xq must be (T, {K}), got {tuple(xq.shape)}"
     assert x_scale.shape == (xq.shape[0], _blocks(K)), \
         f"x_scale must be {(xq.shape[0], _blocks(K))}, got {tuple(x_scale.shape)}"
+    _need_constant("xq x_scale scale", xq, x_scale, scale)
     T = xq.shape[0]
     if T == 0:
         return torch.empty((0, N), dtype=out_dtype, device=xq.device)

@@ -158,3 +158,23 @@ def test_forward_mode_derivatives_are_refused(stubbed, grad_mode):
         torch.func.jvp(lambda a: q.grouped_linear(a, w, off), (x,), (x,))
     with pytest.raises(RuntimeError):
         torch.func.vmap(lambda a: q.grouped_linear(a, w, off))(x.view(2, 2, 32))
+
+
+def test_fp8_matmul_refuses_derivatives(stubbed):
+    """It has none: what would need one is refused, not dropped."""
+    import quant_2bit_b200 as q
+    x, _, _, f8, s = _operands()
+    xq, xs = x.to(torch.float8_e4m3fn), torch.ones(4, 1)
+    for args in ((xq, xs.clone().requires_grad_(), f8, s), (xq.clone().requires_grad_(), xs, f8, s),
+                 (xq, xs, f8, s.clone().requires_grad_())):
+        with pytest.raises(AssertionError):
+            q.fp8_matmul(*args)
+    with forward_ad.dual_level(), torch.no_grad():
+        for args in ((xq, forward_ad.make_dual(xs, xs.clone()), f8, s),
+                     (xq, xs, f8, forward_ad.make_dual(s, s.clone()))):
+            with pytest.raises(AssertionError):
+                q.fp8_matmul(*args)
+        assert q.fp8_matmul(xq, xs, f8, s).shape == (4, 16)
+    with torch.no_grad():
+        assert q.fp8_matmul(xq, xs.clone().requires_grad_(), f8, s).shape == (4, 16)
+    assert stubbed == ["bcjr_fp8_mm"] * 2
