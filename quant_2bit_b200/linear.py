@@ -167,24 +167,33 @@ def _grouped_forward(x, weight, offsets):
 def _grouped_backward(ctx, dy):
     x, weight, offsets = ctx.saved_tensors
     need_x, need_w, _ = ctx.needs_input_grad
-    E, N, K = weight.shape
-    T = x.shape[0]
-    dx = x.new_empty(T, K) if need_x else None
-    dw = x.new_empty(E, N, K) if need_w else None
-    dy, ld_dy = _rows(dy if dy.dtype == x.dtype else dy.to(x.dtype))
-    x, ld_x = _rows(x)
-    weight = _dense(weight)
+    E, N, K = ctx.sizes
+    T = dy.shape[0]
+    dy, ld_dy = _rows(dy if dy.dtype == ctx.dtype else dy.to(ctx.dtype))
+    dx = dw = x_ptr = weight_ptr = dx_ptr = dw_ptr = None
+    ld_x = 0
+    if need_x:
+        weight = _dense(weight)
+        dx = dy.new_empty(T, K)
+        weight_ptr, dx_ptr = weight.data_ptr(), dx.data_ptr()
+    if need_w:
+        x, ld_x = _rows(x)
+        dw = dy.new_empty(E, N, K)
+        x_ptr, dw_ptr = x.data_ptr(), dw.data_ptr()
     off_ptr, off_size = _bounds(offsets)
-    _call(_lib.load().bcjr_grouped_backward, x.get_device(), dy.data_ptr(), ld_dy, x.data_ptr(), ld_x,
-          weight.data_ptr(), off_ptr, off_size, T, E, N, K, _DTYPES[x.dtype],
-          dx.data_ptr() if need_x else None, dw.data_ptr() if need_w else None, None)
+    _call(_lib.load().bcjr_grouped_backward, dy.get_device(), dy.data_ptr(), ld_dy, x_ptr, ld_x, weight_ptr,
+          off_ptr, off_size, T, E, N, K, _DTYPES[ctx.dtype], dx_ptr, dw_ptr, None)
     return dx, dw, None
 
 
 class _GroupedLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, offsets):
-        ctx.save_for_backward(x, weight, offsets)
+        # each gradient reads the other operand only: what no gradient reads is
+        # not kept alive, and may change before the backward pass
+        need_x, need_w, _ = ctx.needs_input_grad
+        ctx.save_for_backward(x if need_w else None, weight if need_x else None, offsets)
+        ctx.sizes, ctx.dtype = weight.shape, x.dtype
         return _grouped_forward(x, weight, offsets)
 
     @staticmethod

@@ -97,3 +97,22 @@ def test_forward_mode_derivatives_are_refused(cuda_ok):
             with pytest.raises(NotImplementedError):
                 f(*args)
         assert torch.equal(grouped_linear(x, w, offsets), want[0]) and torch.equal(fp8_linear(x, q, s), want[1])
+
+
+@pytest.mark.parametrize("frozen", ["x", "weight"])
+def test_gradient_of_one_operand_keeps_the_other_only(cuda_ok, frozen):
+    """With one operand frozen its gradient's partner is not kept: it may be
+    changed in place before the backward pass, and its memory is not held."""
+    from quant_2bit_b200 import grouped_linear
+    counts = [70, 0, 31]
+    offsets = _counts_to_offsets(counts)
+    x, w, dy = _inputs(101, 3, 64, 112, torch.bfloat16)
+    x0, w0 = x.clone(), w.clone()
+    leaf = w if frozen == "x" else x
+    leaf.requires_grad_()
+    y = grouped_linear(x, w, offsets)
+    with torch.no_grad():
+        leaf.zero_()                     # read by neither gradient
+    grad, = torch.autograd.grad(y, leaf, dy)
+    ref, mag = _wgrad64(dy, x0, offsets, 3) if frozen == "x" else _grouped64(dy, w0.transpose(1, 2), offsets)
+    _close(grad, ref, mag, 70 if frozen == "x" else 64, "gradient")

@@ -178,3 +178,26 @@ def test_fp8_matmul_refuses_derivatives(stubbed):
     with torch.no_grad():
         assert q.fp8_matmul(xq, xs.clone().requires_grad_(), f8, s).shape == (4, 16)
     assert stubbed == ["bcjr_fp8_mm"] * 2
+
+
+def test_only_what_the_backward_pass_reads_is_kept(stubbed):
+    """The rows' gradient reads the weight only, the weight's the rows only:
+    the other operand is not held, and may be changed in place."""
+    import quant_2bit_b200 as q
+    x, w, off, _, _ = _operands()
+    for need_x, need_w in ((True, False), (False, True), (True, True)):
+        x, w = x.detach().clone().requires_grad_(need_x), w.detach().clone().requires_grad_(need_w)
+        kept = []
+
+        def pack(t):
+            kept.append(t)
+            return t
+
+        with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+            y = q.grouped_linear(x, w, off)
+        assert [any(t.data_ptr() == k.data_ptr() for k in kept) for t in (x, w)] == [need_w, need_x]
+        if not (need_x and need_w):
+            (w if need_w else x).detach().zero_()      # the one that has the gradient: not read by it
+        grads = torch.autograd.grad(y, [t for t in (x, w) if t.requires_grad], torch.zeros_like(y))
+        assert [g.shape for g in grads] == [t.shape for t in (x, w) if t.requires_grad]
+    assert stubbed == ["bcjr_grouped_mm", "bcjr_grouped_backward"] * 3
