@@ -36,6 +36,7 @@ from . import _lib
 _BLOCK = 128
 _TILE = 16
 _MAX_GROUPS = 1024
+_MAX_STEP = 1 << 32        # elements between rows
 _RAW_ROWS = 32             # up to here the 8-bit layer needs no workspace
 _F8 = torch.float8_e4m3fn
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
@@ -112,14 +113,14 @@ def _blocks(n):
 
 def _rows(t):
     """(tensor, elements between rows) of a 2-D matrix as the kernels read it: the
-    matrix itself when its rows are contiguous and start on 16 bytes, else a
-    contiguous copy."""
+    matrix itself when its rows are contiguous, start on 16 bytes and lie no
+    further apart than the C entry points accept, else a contiguous copy."""
     n = t.size(1)
     if t.data_ptr() % 16 == 0:
         if t.is_contiguous():
             return t, n
         step = t.stride(0)
-        if t.stride(1) == 1 and step >= n and step * t.element_size() % 16 == 0:
+        if t.stride(1) == 1 and n <= step <= _MAX_STEP and step * t.element_size() % 16 == 0:
             return t, step
     return _dense(t), n
 

@@ -201,3 +201,12 @@ def test_only_what_the_backward_pass_reads_is_kept(stubbed):
         grads = torch.autograd.grad(y, [t for t in (x, w) if t.requires_grad], torch.zeros_like(y))
         assert [g.shape for g in grads] == [t.shape for t in (x, w) if t.requires_grad]
     assert stubbed == ["bcjr_grouped_mm", "bcjr_grouped_backward"] * 3
+
+
+def test_rows_further_apart_than_the_library_takes_are_copied():
+    from quant_2bit_b200 import linear
+    near = torch.empty(2, 1 << 32, device="meta", dtype=torch.bfloat16)[:, :32]
+    far = torch.empty(2, (1 << 32) + 8, device="meta", dtype=torch.bfloat16)[:, :32]
+    assert linear._rows(near)[1] == 1 << 32
+    rows, step = linear._rows(far)
+    assert step == 32 and rows.is_contiguous()
