@@ -7,6 +7,7 @@ the CUDA runtime statically and has no torch dependency.
 """
 import concurrent.futures
 import os
+import re
 import subprocess
 import sys
 
@@ -19,6 +20,11 @@ SOURCES = ["bcjr_capi.cu", "bcjr_generic.cu", "bcjr_l16.cu", "bcjr_b4.cu", "bcjr
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
               "-Xcompiler", "-fvisibility=hidden"]
+
+# Kernels that share their registers out among warpgroups are launched with the
+# number that the source is written for, or not at all (another one would leave
+# a share waiting for registers for good): {source: (kernel, its constant there)}.
+LAUNCH_REGISTERS = {"bcjr_fp8.cu": ("fp8_rows_kernel", "kLaunchRegs")}
 
 
 def _nvcc():
@@ -37,6 +43,28 @@ def _stale():
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
+def registers(ptxas, kernel):
+    """Registers of every instance of `kernel` in ptxas -v output."""
+    return [int(n) for name, n in re.findall(r"Compiling entry function '(\w+)'.*?Used (\d+) registers", ptxas, re.S)
+            if kernel in name]
+
+
+def _compile(cmd, src, ptxas_info):
+    run = subprocess.run(cmd + ["-Xptxas", "-v"] if ptxas_info or src in LAUNCH_REGISTERS else cmd,
+                         stderr=subprocess.PIPE, text=True)
+    for line in run.stderr.splitlines():
+        if ptxas_info or run.returncode or not line.startswith("ptxas info") and " bytes stack frame" not in line:
+            print(line, file=sys.stderr)
+    run.check_returncode()
+    if src in LAUNCH_REGISTERS:
+        kernel, constant = LAUNCH_REGISTERS[src]
+        with open(os.path.join(CSRC, src)) as f:
+            want = int(re.search(constant + r" = (\d+)", f.read()).group(1))
+        got = registers(run.stderr, kernel)
+        if not got or set(got) != {want}:
+            raise RuntimeError(f"{src}: {kernel} was compiled for {got} registers, its shares add up to {want}")
+
+
 def build(force=False, verbose=False, ptxas_info=False):
     """Compile every source into one shared library (skipped when up to date)."""
     if not force and not _stale():
@@ -46,15 +74,13 @@ def build(force=False, verbose=False, ptxas_info=False):
     for s in srcs:
         obj = os.path.join(CSRC, s.replace(".cu", ".o"))
         cmd = [_nvcc(), *ARCH, *NVCC_FLAGS, "-c", os.path.join(CSRC, s), "-o", obj]
-        if ptxas_info:
-            cmd += ["-Xptxas", "-v"]
         if verbose:
             print(" ".join(cmd), flush=True)
         cmds.append(cmd)
         objs.append(obj)
     # the translation units are independent: compile them side by side
     with concurrent.futures.ThreadPoolExecutor(max_workers=min(len(cmds), os.cpu_count() or 1)) as ex:
-        for f in [ex.submit(subprocess.run, c, check=True) for c in cmds]:
+        for f in [ex.submit(_compile, c, s, ptxas_info) for c, s in zip(cmds, srcs)]:
             f.result()
     cmd = [_nvcc(), *ARCH, "-shared", "-Xcompiler", "-fPIC", *objs, "-o", LIB]
     if verbose:
