@@ -229,9 +229,6 @@ __device__ __forceinline__ void tc_fence_before() {
 __device__ __forceinline__ void tc_fence_after() {
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
 // 16 lanes and 32 columns: v[4 j + i] of thread t is lane t / 4 + 8 (i / 2),
 // column 8 j + 2 (t % 4) + i % 2.
 __device__ __forceinline__ void tmem_ld(float (&v)[16], uint32_t addr) {
@@ -350,21 +347,14 @@ __device__ __forceinline__ void pair_tma3(uint32_t dst, const CUtensorMap *map, 
         ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar0)
         : "memory");
 }
-template <int KIND>
+// (16-bit types only: e4m3 has no pairs.)
 __device__ __forceinline__ void pair_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc,
                                          uint32_t accumulate) {
-    if constexpr (KIND == kE4M3)
-        asm volatile(
-            "{ .reg .pred p; setp.ne.b32 p, %4, 0;"
-            " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p; }"
-            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-            : "memory");
-    else
-        asm volatile(
-            "{ .reg .pred p; setp.ne.b32 p, %4, 0;"
-            " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }"
-            ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-            : "memory");
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0;"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p; }"
+        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+        : "memory");
 }
 __device__ __forceinline__ void pair_commit(uint32_t bar) {
     asm volatile(
@@ -924,7 +914,7 @@ mm_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtens
                         for (int j = 0; j < SLICES; ++j) {
                             const uint64_t aj = da + ((j * A_STEP) >> 4), bj = db + ((j * B_STEP) >> 4);
                             const uint32_t add = (KIND == kE4M3 ? j > 0 : (kb | j) > 0) ? 1u : 0u;
-                            if constexpr (PAIR) pair_mma<KIND>(d, aj, bj, idesc, add);
+                            if constexpr (PAIR) pair_mma(d, aj, bj, idesc, add);
                             else mma<KIND>(d, aj, bj, idesc, add);
                         }
                         if (KIND == kE4M3 || kb == t.nkb - 1) commit<PAIR>(smem_u32(&ctl.tfull[acc++ % ACC]));
