@@ -4,7 +4,9 @@ training step, what is kept and refused, and failures of shared tiles."""
 import pytest
 import torch
 
-from test_gpu_linear import _check_grouped, _close, _counts_to_offsets, _grouped64, _inputs, _wgrad64
+from test_linear import difference_holds
+from test_gpu_linear import (_check_grouped, _close, _counts_to_offsets, _expand, _grouped64, _inputs,
+                             _quantize_plain, _wgrad64)
 
 pytestmark = pytest.mark.gpu
 
@@ -116,3 +118,127 @@ def test_gradient_of_one_operand_keeps_the_other_only(cuda_ok, frozen):
     grad, = torch.autograd.grad(y, leaf, dy)
     ref, mag = _wgrad64(dy, x0, offsets, 3) if frozen == "x" else _grouped64(dy, w0.transpose(1, 2), offsets)
     _close(grad, ref, mag, 70 if frozen == "x" else 64, "gradient")
+
+
+@pytest.mark.parametrize("tiles", [1, 2, 3])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gradients_against_differences_along_the_gradient(cuda_ok, dtype, tiles):
+    """<dy, f(d)> = <gradient, d> with d the 64-bit gradient, where both sides are
+    a sum of squares (a displacement of its own leaves a sum of signed terms, in
+    which the tolerance hides a missing gradient)."""
+    from quant_2bit_b200 import _lib, grouped_linear
+    counts = [70, 0, 31, 200]
+    offsets = _counts_to_offsets(counts)
+    x, w, dy = _inputs(301, 4, 96, 112, dtype, seed=5)
+    dx64, dx_mag = _grouped64(dy, w.transpose(1, 2), offsets)
+    dw64, dw_mag = _wgrad64(dy, x, offsets, 4)
+    d_x, d_w = dx64.to(dtype), dw64.to(dtype)
+    leaves = x.clone().requires_grad_(), w.clone().requires_grad_()
+    with _lib.test_option(_lib.OPT_LINEAR_TILES, tiles):
+        dx, dw = torch.autograd.grad(grouped_linear(*leaves, offsets), leaves, dy)
+        f_x, f_w = grouped_linear(d_x, w, offsets), grouped_linear(x, d_w, offsets)
+    assert difference_holds(dy, f_x, _grouped64(d_x, w, offsets)[1], 112, dx, dx_mag, 96, d_x)
+    assert difference_holds(dy, f_w, _grouped64(x, d_w, offsets)[1], 112, dw, dw_mag, 200, d_w)
+
+
+def test_a_wait_that_runs_out_in_shared_and_long_tiles(cuda_ok):
+    """The first load of block 0 withheld where blocks of a cluster share a
+    tile's contraction, where the 8-bit product overlaps its quantizer in small
+    tiles, and where a contraction is longer than the ring of stages: the call
+    reports it, the first tile's outputs are NaN, the next call is clean."""
+    import ctypes
+    from quant_2bit_b200 import _lib, fp8_quantize_weight
+    lib = _lib.load()
+    stream = torch.cuda.current_stream().cuda_stream
+    status = torch.full((1,), 77, dtype=torch.int32, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+
+    def rand(*shape):
+        return torch.randn(*shape, generator=g, device="cuda").to(torch.bfloat16)
+
+    x, w = rand(1000, 4096), rand(272, 4096)
+    q, s = fp8_quantize_weight(w)
+    out = torch.zeros(1000, 272, dtype=torch.bfloat16, device="cuda")
+    narrow, dw = rand(1000, 272), torch.zeros(272, 4096, dtype=torch.bfloat16, device="cuda")
+    ws = torch.empty(lib.bcjr_fp8_linear_workspace_bytes(1000, 4096), dtype=torch.uint8, device="cuda")
+
+    def forward(rows, K):
+        return lambda: lib.bcjr_grouped_mm(x.data_ptr(), 4096, w.data_ptr(), None, 0, rows, 1, 272, K, 0,
+                                           out.data_ptr(), status.data_ptr(), stream)
+
+    def fp8(rows, K):
+        return lambda: lib.bcjr_fp8_linear(x.data_ptr(), 4096, 0, q.data_ptr(), s.data_ptr(), None, 0, rows, 1,
+                                           272, K, 0, out.data_ptr(), ws.data_ptr(), ws.numel(),
+                                           status.data_ptr(), stream)
+
+    def weights():
+        return lib.bcjr_grouped_backward(narrow.data_ptr(), 272, x.data_ptr(), 4096, None, None, 0, 1000, 1, 272,
+                                         4096, 0, None, dw.data_ptr(), status.data_ptr(), stream)
+
+    # (tiles, call, the outputs of block 0's tile)
+    for tiles, call, hit in ((1, forward(20, 1040), out[:20, :128]), (1, forward(20, 4096), out[:20, :128]),
+                             (1, fp8(20, 1040), out[:20, :128]), (1, fp8(20, 4096), out[:20, :128]),
+                             (1, fp8(40, 1040), out[:40, :128]), (1, fp8(40, 4096), out[:40, :128]),
+                             (2, forward(200, 4096), out[:200, :128]), (3, forward(200, 4096), out[:200, :256]),
+                             (2, fp8(128, 4096), out[:128, :256]), (2, weights, dw[:256, :128]),
+                             (3, weights, dw[:256, :256])):
+        with _lib.test_option(_lib.OPT_LINEAR_TILES, tiles):
+            with _lib.test_option(_lib.OPT_TEST_DROP_SENDS, 1):
+                assert call() == 0
+                assert lib.bcjr_ws_status(ctypes.c_void_p(status.data_ptr()), stream) == _lib.BCJR_ERR_TIMEOUT
+            assert hit.isnan().all()
+            assert call() == 0
+            assert lib.bcjr_ws_status(ctypes.c_void_p(status.data_ptr()), stream) == 0
+            assert torch.isfinite(hit).all()
+
+
+def test_8_bit_layers_beyond_32_bits(cuda_ok):
+    """Rows, outputs, codes and weights of more than 2^31 elements."""
+    from quant_2bit_b200 import _lib, fp8_linear, fp8_matmul, fp8_quantize_rows, fp8_quantize_weight
+    g = torch.Generator(device="cuda").manual_seed(3)
+    T, N, K = 2_150_000, 16, 1008
+    x = torch.empty(T, K, dtype=torch.bfloat16, device="cuda").normal_(generator=g)
+    assert x.numel() > 2 ** 31
+    q, s = fp8_quantize_weight(torch.randn(N, K, generator=g, device="cuda"))
+    w64 = _expand(q, s, 128)
+    xq, xs = fp8_quantize_rows(x)
+    y = fp8_matmul(xq, xs, q, s)
+    ends = (slice(0, 300), slice(T - 300, T))
+    for rows in ends:
+        a, b = _quantize_plain(x[rows], 1)
+        assert torch.equal(xq[rows].view(torch.uint8), a.contiguous().view(torch.uint8)) and torch.equal(xs[rows], b)
+        a = _expand(a, b, 1)
+        _close(y[rows], a @ w64.t(), a.abs() @ w64.abs().t(), K, "y", extra=4)
+    del xq, xs
+    assert torch.equal(fp8_linear(x, q, s), y)
+    # the gradient: T x 1008 out
+    x.requires_grad_()
+    dy = torch.randn(T, N, generator=g, device="cuda").to(torch.bfloat16)
+    dx, = torch.autograd.grad(fp8_linear(x, q, s), x, dy)
+    for rows in ends:
+        a = _expand(*_quantize_plain(dy[rows], 1), 1)
+        _close(dx[rows], a @ w64, a.abs() @ w64.abs(), N, "dx", extra=4)
+    del x, y, dx
+
+    E, N, K = 1024, 2064, 1024
+    w = torch.zeros(E, N, K, dtype=torch.bfloat16, device="cuda")
+    w[-2:] = torch.randn(2, N, K, generator=g, device="cuda")
+    q, s = fp8_quantize_weight(w)
+    assert q.numel() > 2 ** 31
+    for e in (E - 2, E - 1):
+        a, b = _quantize_plain(w[e], 128)
+        assert torch.equal(q[e].view(torch.uint8), a.contiguous().view(torch.uint8)) and torch.equal(s[e], b)
+    del w
+    w64 = torch.stack([_expand(q[e], s[e], 128) for e in (E - 2, E - 1)])
+    for T, tiles in ((30, 0), (40, 1), (300, 2)):
+        x, dy = (torch.randn(T, n, generator=g, device="cuda").to(torch.bfloat16) for n in (K, N))
+        offsets = torch.zeros(E + 1, dtype=torch.int32, device="cuda")
+        offsets[-2], offsets[-1] = 17, T
+        x.requires_grad_()
+        with _lib.test_option(_lib.OPT_LINEAR_TILES, tiles):
+            y = fp8_linear(x, q, s, offsets)
+            dx, = torch.autograd.grad(y, x, dy)
+        two = torch.tensor([0, 17, T])
+        for got, rows, weight, depth in ((y.detach(), x.detach(), w64, K), (dx, dy, w64.transpose(1, 2), N)):
+            ref, mag = _grouped64(_expand(*_quantize_plain(rows, 1), 1), weight, two)
+            _close(got, ref, mag, depth, "fp8", extra=4)

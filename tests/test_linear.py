@@ -210,3 +210,40 @@ def test_rows_further_apart_than_the_library_takes_are_copied():
     assert linear._rows(near)[1] == 1 << 32
     rows, step = linear._rows(far)
     assert step == 32 and rows.is_contiguous()
+
+
+# A gradient against differences: the product f is linear in each operand, so
+# <dy, f(d)> = <gradient, d> for every displacement d.  Along the gradient itself
+# (64 bits, rounded to the type) both sides are a sum of squares, and what the
+# roundings can move them by is about 1 % of it in bf16: every f and every
+# gradient is off by half a step, eps / 2 of its size, and by 2^-23 of the
+# products' magnitudes for each of its `depth` products.
+
+
+def difference_holds(dy, f, f_mag, f_depth, grad, grad_mag, grad_depth, d):
+    lhs, rhs = dy.double() * f.double(), grad.double() * d.double()
+    half = torch.finfo(f.dtype).eps / 2
+    tol = half * float(lhs.abs().sum() + rhs.abs().sum()) * (1 + 2 * half)
+    tol += 2.0 ** -23 * float((dy.double().abs() * f_mag * f_depth).sum() + (d.double().abs() * grad_mag * grad_depth).sum())
+    return abs(float(lhs.sum() - rhs.sum())) <= tol
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_the_difference_check_tells_wrong_gradients(dtype):
+    """The check that the GPU test uses: right gradients pass; a zero, negated,
+    halved, doubled or partly missing one does not, for several inputs."""
+    for seed in range(20):
+        g = torch.Generator().manual_seed(seed)
+        x, w, dy = torch.randn(301, 112, generator=g), torch.randn(96, 112, generator=g) / 112 ** 0.5, torch.randn(301, 96, generator=g)
+        x, w, dy = (t.to(dtype).double() for t in (x, w, dy))
+        for grad64, mag, depth, product, product_depth in (
+                (dy @ w, dy.abs() @ w.abs(), 96, lambda d: d @ w.t(), 112),
+                (dy.t() @ x, dy.abs().t() @ x.abs(), 301, lambda d: x @ d.t(), 112)):
+            d = grad64.to(dtype)
+            f_mag = d.double().abs() @ w.abs().t() if depth == 96 else x.abs() @ d.double().abs().t()
+            f, grad = product(d.double()).to(dtype), grad64.to(dtype)
+            missing = grad.clone()
+            missing[-len(grad) // 5:] = 0
+            assert difference_holds(dy, f, f_mag, product_depth, grad, mag, depth, d)
+            for wrong in (torch.zeros_like(grad), -grad, grad / 2, grad * 2, missing):
+                assert not difference_holds(dy, f, f_mag, product_depth, wrong, mag, depth, d)
