@@ -533,10 +533,10 @@ int bcjr_fp8_quantize_blocks(const void *w, int E, int N, int K, int dtype, void
 // How the rows of a product come: quantized; quantized by the kernel launched
 // just before; in 16 bits, for the product to quantize.
 enum { kReady = 0, kFollows = 1, kRaw = 2 };
-static int fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long scale_row,
-                  long scale_block, const void *w, const float *w_scale, const void *offsets,
-                  int offsets_bytes, long T, int E, int N, int K, int transpose_w, void *out,
-                  int out_dtype, int *status, bcjr_stream_t stream, int come) {
+static int check_mm(const void *rows, long ld_rows, const float *rows_scale, long scale_row,
+                    long scale_block, const void *w, const float *w_scale, const void *offsets,
+                    int offsets_bytes, long T, int E, int N, int K, int transpose_w, const void *out,
+                    int out_dtype, const int *status, int come) {
     if (T < 0 || T > kMaxRows || E < 1 || E > kMaxGroups || N < 16 || K < 16 || N % 16 || K % 16 ||
         N > (1 << 24) || K > (1 << 24))
         return BCJR_ERR_BAD_SHAPE;
@@ -544,11 +544,22 @@ static int fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long 
     if (offsets ? (offsets_bytes != 4 && offsets_bytes != 8) : E != 1) return BCJR_ERR_BAD_SHAPE;
     if (T == 0) return BCJR_OK;
     if (!rows || (!rows_scale && come != kRaw) || !w || !w_scale || !out) return BCJR_ERR_NULL_POINTER;
-    const int depth = transpose_w ? N : K, lanes = transpose_w ? K : N;
+    const int depth = transpose_w ? N : K;
     if (ld_rows < depth || ld_rows > (1L << 32) || scale_row < 0 || scale_block < 0) return BCJR_ERR_BAD_SHAPE;
     if (!aligned(rows, 16) || ld_rows % (come == kRaw ? 8 : 16) || !aligned(w, 16) || !aligned(out, 16) || !aligned(status, 4) ||
         !aligned(rows_scale, 4) || !aligned(w_scale, 4) || (offsets && !aligned(offsets, size_t(offsets_bytes))))
         return BCJR_ERR_ALIGNMENT;
+    return BCJR_OK;
+}
+
+static int fp8_mm(const void *rows, long ld_rows, const float *rows_scale, long scale_row,
+                  long scale_block, const void *w, const float *w_scale, const void *offsets,
+                  int offsets_bytes, long T, int E, int N, int K, int transpose_w, void *out,
+                  int out_dtype, int *status, bcjr_stream_t stream, int come) {
+    const int st = check_mm(rows, ld_rows, rows_scale, scale_row, scale_block, w, w_scale, offsets, offsets_bytes,
+                            T, E, N, K, transpose_w, out, out_dtype, status, come);
+    if (st || T == 0) return st;
+    const int depth = transpose_w ? N : K, lanes = transpose_w ? K : N;
     const long kb = (K + 127) / 128, nb = (N + 127) / 128;
     Call c = {};
     c.kind = kE4M3;
@@ -624,7 +635,11 @@ int bcjr_fp8_linear(const void *x, long ld, int dtype, const void *w, const floa
     if (!ws || ws_bytes < need) return BCJR_ERR_WORKSPACE;
     if (!aligned(ws, 16)) return BCJR_ERR_ALIGNMENT;
     float *scale = reinterpret_cast<float *>(static_cast<char *>(ws) + size_t(T) * depth);
-    const int st = bcjr_fp8_quantize_rows(x, ld, T, depth, dtype, ws, scale, 1, T, stream);
+    // nothing is launched for a call that the product will refuse
+    int st = check_mm(ws, depth, scale, 1, T, w, w_scale, offsets, offsets_bytes, T, E, N, K, transpose_w, out,
+                      dtype, status, kFollows);
+    if (st) return st;
+    st = bcjr_fp8_quantize_rows(x, ld, T, depth, dtype, ws, scale, 1, T, stream);
     if (st) return st;
     return fp8_mm(ws, depth, scale, 1, T, w, w_scale, offsets, offsets_bytes, T, E, N, K, transpose_w, out,
                   dtype, status, stream, kFollows);

@@ -247,3 +247,17 @@ def test_the_difference_check_tells_wrong_gradients(dtype):
             assert difference_holds(dy, f, f_mag, product_depth, grad, mag, depth, d)
             for wrong in (torch.zeros_like(grad), -grad, grad / 2, grad * 2, missing):
                 assert not difference_holds(dy, f, f_mag, product_depth, wrong, mag, depth, d)
+
+
+def test_fp8_linear_refuses_before_its_quantizer_runs(lib):
+    """What only the product can refuse is refused first too: the workspace of a
+    refused call is not written (without a GPU a launch would be the error)."""
+    def call(x=P, ld=64, w=P, s=P, off=P, off_size=4, T=40, E=2, N=32, K=64, out=P, status=None):
+        return lib.bcjr_fp8_linear(x, ld, 0, w, s, off, off_size, T, E, N, K, 0, out, P, 1 << 20, status, None)
+
+    for bad in (dict(w=None), dict(s=None), dict(out=None)):
+        assert call(**bad) == NULL, bad
+    for bad in (dict(N=24), dict(N=1 << 25), dict(E=0), dict(E=1025), dict(off=None), dict(off_size=2)):
+        assert call(**bad) == SHAPE, bad
+    for bad in (dict(w=P + 8), dict(out=P + 8), dict(s=P + 2), dict(off=P + 4, off_size=8), dict(status=P + 2)):
+        assert call(**bad) == ALIGN, bad
