@@ -26,7 +26,8 @@ namespace {
 constexpr int kQThreads = 256, kUnroll = 4, kQRows = kQThreads / 16;
 
 // 16 lanes per segment, 8 elements per lane (the width is a multiple of 16).
-// Bound by memory: 8192 x 2048 bf16 (50 MB) 12.6 us, one row 2 us a launch.
+// 8192 x 2048 bf16 (50 MB) 12.6 us = 4.0 TB/s of 6.5, one row 2 us a launch.
+// Bound by issue and latency: the issue slots are 54 % busy, memory 41 %.
 // A block has 16 rows and kUnroll neighbouring segments of each, all loaded
 // before the first is used; the scales of a column of segments, side by side
 // when they are stored block by block, leave together.
@@ -59,8 +60,9 @@ quantize_rows(const T *__restrict__ x, long ld, long rows, int k, uint8_t *__res
 }
 
 // One block of 128 x 128 per thread block, held in registers between its
-// maximum and its rounding: read once.  Bound by memory: 2048 x 8192 fp32
-// (84 MB) 14.3 us = 5.9 TB/s.
+// maximum and its rounding: read once.  2048 x 8192 fp32 (84 MB) 14.3 us = 5.9
+// TB/s, bound by memory; in bf16 (50 MB) 13.3 us = 3.8 TB/s, bound by latency:
+// the same number of elements in flight are half the bytes.
 template <typename T>
 __global__ void __launch_bounds__(kQThreads)
 quantize_blocks(const T *__restrict__ w, int n, int k, uint8_t *__restrict__ q,
@@ -123,8 +125,8 @@ cudaError_t run_blocks(const void *w, long blocks, int n, int k, void *q, float 
 // Each half has accumulator buffers and an issuing warp of its own, so that
 // they run out of step: one half's sums run under the other's products.
 //
-// 8192 x 8192 x 2048: 129 us = 2.1 PFLOP/s (one accumulator chain with a column's
-// factor for each sum: 234 us); 64 experts, 32768 rows, 2048 x 1024: 96 us.  The
+// 8192 x 8192 x 2048: 127 us = 2.2 PFLOP/s (one accumulator chain with a column's
+// factor for each sum: 234 us); 64 experts, 32768 rows, 2048 x 1024: 94 us.  The
 // tensor pipe is busy 54 %, the issue slots 46 %: each k block's hand-over
 // (barrier, TMEM loads, 128 fp32 sums a thread, barrier) bounds it.  Two blocks
 // to a tile of 256 rows measured the same on one large matrix and 8 % slower

@@ -29,9 +29,10 @@
 //
 // Measured on a B200 (cold L2; 1.62 PFLOP/s is cuBLAS bf16 at the same size):
 //   8192 x 8192 x 2048 bf16  forward 168 us = 1.64 PFLOP/s, gradients 180 us
-//     each = 1.53; the tensor pipe is busy 87 % of the forward: bound by it.
-//   64 experts, 32768 rows, 1024 x 2048 bf16  113 us forward, 115 and 139 us:
-//     ragged tiles, 0.47 GB of memory traffic a product (4.2 TB/s).
+//     each = 1.53; the tensor pipe is busy 86 and 78 % of the time: bound by it.
+//   64 experts, 32768 rows, 1024 x 2048 bf16  113 us forward, 113 and 135 us:
+//     ragged tiles, 0.47 GB of memory traffic a product (4.2 TB/s).  Back to
+//     back for seconds 152, 153 and 167 us: power (1000 W at 1.18 GHz).
 //   64 experts, 488 rows, 2048 x 1024 fp16  48 us = 5.6 TB/s of weights: bound
 //     by memory.
 //   8 rows by 8 of 64 experts, 1024 x 2048  14 us (34 MB): launch, set-up and
@@ -69,7 +70,8 @@ constexpr int kPitch = kLanes * 2 + 16;           // bytes of a staged output ro
                                                   // 8 rows fall into different banks
 constexpr int kMaxGroups = 1024;
 constexpr int kRawRows = 32;                      // rows that the e4m3 product quantizes itself
-constexpr int kMaxSplit = 4;                      // blocks of a cluster that share a tile
+constexpr int kMaxSplit = 4;                      // blocks of a cluster that share a tile (eight: 37 rows x 2048 x
+                                                  // 8192 in e4m3 16 -> 25 us, 64 rows x 2048 x 2048 14 -> 23)
 constexpr int kBoxRows = 64;                      // rows of one TMA box
 constexpr long long kWaitLimitClocks = 2000000000ll;   // about 1 s
 
@@ -400,6 +402,9 @@ __device__ __forceinline__ void bar_arrive_in(uint32_t bar, uint32_t r) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_rank(bar, r))
                  : "memory");
 }
+// For accumulators of the other block's products that have been read, as
+// bar_arrive_tmem above.  (A release would wait for the output's stores as well:
+// 64 experts of 512 rows forward 113 -> 115 us, weights' gradient 135 -> 147.)
 __device__ __forceinline__ void bar_arrive_relaxed_in(uint32_t bar, uint32_t r) {
     asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(in_rank(bar, r))
                  : "memory");
@@ -1342,10 +1347,16 @@ inline int few_split(const Call &c, int sms) {
     return split;
 }
 // Many features: pairs of blocks.  (64 experts, 32768 rows, 1024 and 2048
-// features: 113 us forward, 115 and 139 us gradients in pairs, 125, 125 and 157
+// features: 113 us forward, 113 and 135 us gradients in pairs, 125, 125 and 157
 // us alone.  4 experts, 3000 rows, 1040 features: the same.  96 experts, 3079
 // rows, 272 features, weights' gradient: 27 us in pairs, 20 alone: 272 lanes are
-// two tiles of 256 but three of 128.)
+// two tiles of 256 but three of 128.)  64 experts, 32768 rows, lanes x the other
+// feature axis, us alone | in pairs:
+//                      512 x 2048  640 x 1024  768 x 2048  896 x 1024  1040 x 1024  1408 x 1024
+//   forward             78 |  70    53 |  53   102 |  90    66 |  66     78 |  76     96 |  88
+//   weights' gradient   88 |  84    59 |  76   131 | 121    78 |  76     91 |  94    115 | 117
+// Pairs gain where the lanes fill tiles of 256; where they do not, the weights'
+// gradient loses a quarter below 1024 lanes and a few per cent from there on.
 inline bool in_pairs(const Call &c) {
     const int forced = test_option(kOptLinearTiles);
     return c.kind != kE4M3 && (forced ? forced == 3 : c.p.lanes >= 1024);

@@ -276,8 +276,8 @@ def bcjr_experts_linear(x, offsets, weights, signs_l, signs_r, codebook, T_temp,
     weight (``linear.grouped_linear``; ``offsets`` as there).  What
     QuantizedLinear.forward does for each expert (src/qat/quantized_linear.py:
     204-211, :309-315; the quantized weight is cast to x's type there too), with
-    one launch of each kernel for all of them.  Returns (T, N); gradients flow
-    to x and to every weight."""
+    one launch of each kernel for all of them; torch stacks and casts the fp32
+    weights in between.  Returns (T, N); gradients flow to x and to every weight."""
     assert len(weights) >= 1 and all(W.shape == weights[0].shape for W in weights), \
         "at least one expert, all of one shape"
     if x.dtype not in (torch.bfloat16, torch.float16):       # before the weights are quantized
